@@ -141,6 +141,39 @@ int ntb_attention_dropout(int devID, void * stream,
                           long long maskBlockStride, float scale, float keepScale);
 
 /*
+ * Attention of a decoder's positions to an encoder's states of another length, on half tensors:
+ *
+ *        out[b, h, i] = sum_j exp(scale * q_i . k_j - lse_i) v_j,   lse_i = log sum_j exp(scale * q_i . k_j)
+ *
+ * over the keys j < keyLens[b], with k and v of head h / (headsQ / headsKV) (headsKV divides
+ * headsQ; equal counts are the ordinary form). q, out: [batch, headsQ, lenQ, dim]; k, v: [batch,
+ * headsKV, lenK, dim], addressed through layouts[0..3] = those of q, k, v, out, in elements, so
+ * that a projection's [batch, len, heads * dim] is used without splitting heads into a copy
+ * (source/sample/transformer/submodel/Attention.cpp:198-206). Rows are dense; bases and strides are
+ * multiples of 16 bytes (the stride of an extent of one may be anything), else NTB_ERR_ARG; a batch or
+ * head stride of 0 broadcasts q, k or v. dim: a multiple of 8 up to 128, else NTB_ERR_LIMIT.
+ * dtype X_FLOAT16, else NTB_ERR_DTYPE. scale: positive and finite.
+ *
+ * queryLens, keyLens: device arrays of `batch` ints, or NULL for whole lengths; values are clamped to
+ * [0, lenQ] and [0, lenK]. They stand for the padding masks of a batch of sentences: rows of q, k and v
+ * past a length may hold anything, infinities and NaN too. Rows of out past queryLens[b] and rows
+ * without any key are written as zeros. lse: NULL or [batch, headsQ, lenQ] packed fp32; minus infinity
+ * in the rows that are zeros. It is what the gradient call needs.
+ *
+ * Calls with at most 32 query rows for a key head ((headsQ / headsKV) * lenQ: a decoding step, the
+ * hypotheses of a beam as lenQ rows of one sentence) read k and v once for all of them; fewer rows
+ * than fill the GPU split the keys over a cluster. Sums and statistics are fp32; weights are
+ * rounded to half for the second product. Results do not depend on timing. No workspace.
+ */
+typedef struct ntb_heads_layout {
+    long long batch, head, row;      /* strides in elements */
+} ntb_heads_layout;
+int ntb_cross_attention(int devID, void * stream,
+                        const void * q, const void * k, const void * v, void * out, float * lse,
+                        int dtype, int batch, int headsQ, int headsKV, int lenQ, int lenK, int dim,
+                        const ntb_heads_layout * layouts, const int * queryLens, const int * keyLens, float scale);
+
+/*
  * Row-wise log-softmax over the last dimension in two halves, for logits whose rows are
  * spread over several GPUs (vocabulary shards of the output layer,
  * source/sample/transformer/submodel/Output.cpp:86-101, LogSoftmax.cpp:40-170).

@@ -26,12 +26,19 @@ _i = ctypes.c_int
 _ll = ctypes.c_longlong
 _f = ctypes.c_float
 
+
+class HeadsLayout(ctypes.Structure):
+    """ntb_heads_layout: strides in elements"""
+    _fields_ = [("batch", _ll), ("head", _ll), ("row", _ll)]
+
+
 #: every symbol include/ntb_gemm.h declares, with its argument types
 PROTOTYPES = {
     "ntb_gemm": (_i, [_i, _vp, _vp, _i, _vp, _i, _vp, _i, _i] + [_i] * 6 + [_ll] * 3 + [_f, _f]),
     "ntb_gemm_bias_act": (_i, [_i, _vp, _vp, _i, _vp, _i, _vp, _vp, _i, _i] + [_i] * 6 + [_ll] * 3 + [_f, _f, _i]),
     "ntb_attention": (_i, [_i, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _ll, _f]),
     "ntb_attention_dropout": (_i, [_i, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _ll, _f, _f]),
+    "ntb_cross_attention": (_i, [_i] + [_vp] * 6 + [_i] * 7 + [ctypes.POINTER(HeadsLayout), _vp, _vp, _f]),
     "ntb_row_stats": (_i, [_i, _vp, _vp, _i, _i, _i, _ll, _vp, _vp]),
     "ntb_logsoftmax_apply": (_i, [_i, _vp, _vp, _vp, _i, _i, _i, _ll, _ll, _vp, _vp]),
     "ntb_gemm_grad": (_i, [_i, _vp, _vp, _i, _vp, _i, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _f]),

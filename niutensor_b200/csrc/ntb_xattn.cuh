@@ -1,0 +1,286 @@
+/*
+ * Pieces shared by the cross-attention kernels (forward, single-token step, gradients):
+ * tensor maps over [batch, heads, rows, dim] operands of any strides, 4-D TMA copies,
+ * tensor-memory transfers, and the rule by which queries and keys past a sequence's end
+ * are kept out of the sums.
+ */
+#ifndef NTB_XATTN_CUH
+#define NTB_XATTN_CUH
+
+#include "ntb_internal.h"
+#include "ntb_ptx.cuh"
+#include <cuda_fp16.h>
+#include <cstring>
+
+namespace ntb {
+
+struct XattnShape {
+    int batch, headsQ, headsKV, group, lenQ, lenK, dim;
+    const int * queryLens;
+    const int * keyLens;
+};
+
+/* a forward call after its checks */
+struct XattnCall {
+    XattnShape sh;
+    const void * q;
+    const void * k;
+    const void * v;
+    void * out;
+    float * lse;
+    ntb_heads_layout lQ, lK, lV, lOut;
+    float scale;
+};
+
+constexpr int XATTN_STEP_ROWS = 32;      /* query rows a key head up to which the step kernel is used */
+
+namespace {
+
+constexpr int XT = 128;                               /* rows of a query tile and keys of a key tile */
+constexpr int XBOX_BYTES = XT * ROW_BYTES;            /* 128 rows x 64 halves: one swizzled box of an operand tile */
+constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
+
+/* how an operand's tensor map is addressed: a broadcast extent (stride 0) is mapped with one
+   element and its coordinate multiplied by 0 */
+struct HeadsAddr {
+    int mulBatch, mulHead;
+};
+
+__device__ __forceinline__ int ClampLen(const int * lens, int b, int longest)
+{
+    if (lens == nullptr)
+        return longest;
+    const int n = lens[b];
+    return n < 0 ? 0 : n > longest ? longest : n;
+}
+
+__device__ __forceinline__ void TmaLoad4D(uint32_t dst, const CUtensorMap * map, uint32_t bar, int c0, int c1, int c2, int c3)
+{
+    asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes"
+                 " [%0], [%1, {%3, %4, %5, %6}], [%2];"
+                 :: "r"(dst), "l"(map), "r"(bar), "r"(c0), "r"(c1), "r"(c2), "r"(c3) : "memory");
+}
+
+__device__ __forceinline__ void TmaStore4D(const CUtensorMap * map, uint32_t src, int c0, int c1, int c2, int c3)
+{
+    asm volatile("cp.async.bulk.tensor.4d.global.shared::cta.bulk_group [%0, {%2, %3, %4, %5}], [%1];"
+                 :: "l"(map), "r"(src), "r"(c0), "r"(c1), "r"(c2), "r"(c3) : "memory");
+}
+
+/* D += A * B with A in tensor memory (two halves per 32-bit column) and B in shared memory */
+__device__ __forceinline__ void TcMmaTmemA(uint32_t dTmem, uint32_t aTmem, uint64_t bDesc, uint32_t iDesc, uint32_t accumulate)
+{
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+                 :: "r"(dTmem), "r"(aTmem), "l"(bDesc), "r"(iDesc), "r"(accumulate) : "memory");
+}
+
+/* 32 columns of this thread's lane, without waiting for completion */
+__device__ __forceinline__ void TmemLoad32Async(uint32_t taddr, uint32_t * r)
+{
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+                 "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+                 "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+                   "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+                   "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+                   "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+                 : "r"(taddr) : "memory");
+}
+__device__ __forceinline__ void TmemWaitLoad() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void TmemWaitStore() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+/* 16 registers into 16 columns of this thread's lane, without waiting for completion */
+__device__ __forceinline__ void TmemStore16Async(uint32_t taddr, const uint32_t * v)
+{
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+                 "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
+                 :: "r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]),
+                    "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+                 : "memory");
+}
+
+__device__ __forceinline__ float Exp2(float x)
+{
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+__device__ __forceinline__ uint32_t PackHalf2(float lo, float hi)
+{
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *(const uint32_t *)&h;
+}
+
+__device__ __forceinline__ void StoreShared16(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d)
+{
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" :: "r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+
+/* rows [from, 128) of an operand tile of `boxes` boxes become zeros, by the calling warp; the caller
+   fences before the tensor core reads them. Rows past a sequence's end hold whatever the caller's
+   buffer holds there; their weights are 0, and 0 * NaN would still reach every sum. */
+__device__ __forceinline__ void ZeroTileRows(uint32_t tile, int boxes, int from, int lane)
+{
+    const int n = (XT - from) * 8;
+    for (int box = 0; box < boxes; box++)
+        for (int i = lane; i < n; i += 32)
+            StoreShared16(tile + box * XBOX_BYTES + from * ROW_BYTES + i * 16, 0u, 0u, 0u, 0u);
+}
+
+__device__ __forceinline__ void ClusterSync()
+{
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+__device__ __forceinline__ uint32_t ClusterRank()
+{
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+
+__device__ __forceinline__ uint32_t MapShared(uint32_t addr, uint32_t rank)
+{
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+    return r;
+}
+
+__device__ __forceinline__ float LoadRemote(uint32_t addr)
+{
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+    return v;
+}
+
+__device__ __forceinline__ float4 LoadRemote4(uint32_t addr)
+{
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+    return v;
+}
+
+/* one MMA instruction descriptor: fp16 operands, fp32 accumulator, 128 rows, n columns */
+__device__ constexpr uint32_t XattnDesc(int n, int bMN)
+{
+    return (1u << 4) | ((uint32_t)bMN << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(BM >> 4) << 24);
+}
+
+/*
+ * The map of a [batch, heads, rows, dim] operand as (dim, rows, heads, batch) with boxes of 64
+ * columns x boxRows rows. Strides in elements. Columns past dim read as zeros and are not
+ * written. An extent of one takes any stride; a stride of 0 is a broadcast (inputs only).
+ */
+int EncodeHeads(CUtensorMap * map, HeadsAddr * addr, const void * base, int dim, int rows, int heads, int batch,
+                const ntb_heads_layout & l, int boxRows)
+{
+    EncodeTiledFn enc = GetEncodeTiled();
+    if (!enc)
+        return NTB_ERR_CUDA;
+    addr->mulBatch = l.batch == 0 ? 0 : 1;
+    addr->mulHead = l.head == 0 ? 0 : 1;
+    const int nb = addr->mulBatch ? batch : 1, nh = addr->mulHead ? heads : 1;
+    const long long any = 16;                 /* the stride of an extent of one */
+    cuuint64_t dims[4] = { (cuuint64_t)dim, (cuuint64_t)rows, (cuuint64_t)nh, (cuuint64_t)nb };
+    cuuint64_t strides[3] = { (cuuint64_t)(rows > 1 ? l.row * 2 : any), (cuuint64_t)(nh > 1 ? l.head * 2 : any),
+                              (cuuint64_t)(nb > 1 ? l.batch * 2 : any) };
+    cuuint32_t box[4] = { 64, (cuuint32_t)boxRows, 1, 1 };
+    cuuint32_t estr[4] = { 1, 1, 1, 1 };
+    const CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, (void *)base, dims, strides, box, estr,
+                           CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? NTB_OK : NTB_ERR_ARG;
+}
+
+/* what TMA can address: 16-byte base and strides, strides below 2^40 bytes; broadcast only where allowed */
+inline bool LayoutOk(const void * base, const ntb_heads_layout & l, int dim, int rows, int heads, int batch, bool broadcast)
+{
+    if ((uintptr_t)base & 15)
+        return false;
+    const long long limit = 1LL << 39;        /* elements */
+    if (rows > 1 && (l.row < dim || l.row % 8 != 0 || l.row >= limit))
+        return false;
+    if (heads > 1 && !(broadcast && l.head == 0) && (l.head < dim || l.head % 8 != 0 || l.head >= limit))
+        return false;
+    if (batch > 1 && !(broadcast && l.batch == 0) && (l.batch < dim || l.batch % 8 != 0 || l.batch >= limit))
+        return false;
+    return true;
+}
+
+/* the checks both entry points share; fills the shape */
+inline int XattnShapeOf(XattnShape & s, int dtype, int batch, int headsQ, int headsKV, int lenQ, int lenK, int dim,
+                        const int * queryLens, const int * keyLens, float scale)
+{
+    if (batch < 0 || headsQ < 0 || headsKV < 0 || lenQ < 0 || lenK < 0 || dim < 0)
+        return NTB_ERR_ARG;
+    if (dtype != NTB_X_FLOAT16)
+        return NTB_ERR_DTYPE;
+    if (!(scale > 0.f) || scale > 3.0e38f)
+        return NTB_ERR_ARG;
+    if (headsQ > 0 && (headsKV == 0 || headsQ % headsKV != 0))
+        return NTB_ERR_SHAPE;
+    if (dim < 8 || dim > 128 || dim % 8 != 0)
+        return NTB_ERR_LIMIT;
+    /* row and key indices run up to a tile past the end in 32 bits */
+    if (lenQ > 0x7fffff00 || lenK > 0x7fffff00)
+        return NTB_ERR_LIMIT;
+    s.batch = batch; s.headsQ = headsQ; s.headsKV = headsKV; s.group = headsKV ? headsQ / headsKV : 1;
+    s.lenQ = lenQ; s.lenK = lenK; s.dim = dim;
+    s.queryLens = queryLens; s.keyLens = keyLens;
+    return NTB_OK;
+}
+
+/* launch in clusters of `cluster` CTAs along x, with programmatic stream serialisation as LaunchPdl */
+template <typename... Params, typename... Args>
+cudaError_t LaunchClusterPdl(void (*kern)(Params...), unsigned grid, int block, int smem, int cluster, cudaStream_t stream, Args... args)
+{
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(grid, 1, 1);
+    cfg.blockDim = dim3((unsigned)block, 1, 1);
+    cfg.dynamicSmemBytes = (size_t)smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)cluster;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = PdlEnabled() ? 2 : 1;
+    return cudaLaunchKernelEx(&cfg, kern, args...);
+}
+
+/* makes a device current for the length of a call */
+struct XattnDevice {
+    int prev;
+    bool ok;
+    explicit XattnDevice(int dev) : prev(-1), ok(false)
+    {
+        if (cudaGetDevice(&prev) != cudaSuccess) {
+            prev = -1;
+            cudaGetLastError();
+            return;
+        }
+        ok = prev == dev || cudaSetDevice(dev) == cudaSuccess;
+        if (!ok) {
+            prev = -1;
+            cudaGetLastError();
+        }
+    }
+    ~XattnDevice()
+    {
+        int cur = -1;
+        if (prev >= 0 && cudaGetDevice(&cur) == cudaSuccess && cur != prev)
+            cudaSetDevice(prev);
+    }
+};
+
+}
+
+}
+
+#endif

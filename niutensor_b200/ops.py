@@ -225,6 +225,69 @@ def ScaledDotProductAttention(q, k, v, mask=None, scale=None, keep=None, drop_pr
     return out
 
 
+def _heads_layout(t):
+    """strides of a [batch, heads, len, dim] half tensor, as the kernels address it: dense rows, base and
+    strides on 16 bytes (the stride of an extent of one may be anything)"""
+    _check(t.stride(3) == 1 or t.shape[3] <= 1, "rows of the last dimension must be dense")
+    _check(t.data_ptr() % 16 == 0 and all(t.shape[i] <= 1 or t.stride(i) % 8 == 0 for i in range(3)),
+           "base and strides must be multiples of 16 bytes")
+    return capi.HeadsLayout(t.stride(0), t.stride(1), t.stride(2))
+
+
+def _heads_like(t):
+    """an uninitialised tensor of t's shape, with its order of dimensions where that is dense"""
+    out = torch.empty_like(t)
+    return out if out.stride(3) == 1 else torch.empty(t.shape, dtype=t.dtype, device=t.device)
+
+
+def _cross_attention_checks(q, k, v, query_lens, key_lens, scale, others=()):
+    for t in (q, k, v) + tuple(others):
+        _check(t.is_cuda, "this library has no CPU path: tensors must live on a CUDA device")
+        _check(t.dtype == torch.float16, "Unsupported data type!")
+        _check(t.device == q.device, "The code must be run on the same GPU!")
+        _check(t.dim() == 4, "Input tensors must have a order = 4!")
+    _check(k.shape == v.shape and k.shape[0] == q.shape[0] and k.shape[3] == q.shape[3], "Unmatched tensors in multiplication!")
+    _check(q.shape[1] == 0 or (k.shape[1] > 0 and q.shape[1] % k.shape[1] == 0), "the key heads must divide the query heads")
+    _check(q.shape[3] % 8 == 0 and 8 <= q.shape[3] <= 128, "the head size must be a multiple of 8 up to 128")
+    for lens in (query_lens, key_lens):
+        if lens is not None:
+            _check(lens.is_cuda and lens.device == q.device and lens.dtype == torch.int32 and lens.is_contiguous() and
+                   tuple(lens.shape) == (q.shape[0],), "lengths must be a packed int32 CUDA vector with one entry a sentence")
+    scale = 1.0 / (q.shape[3] ** 0.5) if scale is None else float(scale)
+    _check(0.0 < scale < 3.0e38, "the scale must be positive and finite")
+    return scale
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def CrossAttention(q, k, v, query_lens=None, key_lens=None, scale=None, out=None, with_lse=False):
+    """softmax(scale * q k^T) v of a decoder's positions over an encoder's states of another length
+    (the attention over the encoder's output in source/sample/transformer/submodel/Decoder.cpp).
+    q [batch, heads, lenQ, d], k and v [batch, headsKV, lenK, d] half tensors; headsKV divides heads; d a
+    multiple of 8 up to 128. Any strides on 16 bytes with dense rows, so a projection's
+    [batch, len, heads * d] is passed as .view(batch, len, heads, d).transpose(1, 2) without a copy; the
+    result has q's order of dimensions. query_lens, key_lens: int32 vectors with each sentence's
+    length in a padded batch (None: all whole); what lies past them is not looked at, rows of the result
+    past them, and rows without a key, are zeros. scale defaults to 1 / sqrt(d).
+    A decoding step is the same call with lenQ = 1, or with the hypotheses of a beam as lenQ rows of
+    their sentence. with_lse: returns (out, lse), lse fp32 [batch, heads, lenQ] = log sum exp of the
+    scaled scores (-inf in empty rows), which GradCrossAttention needs."""
+    scale = _cross_attention_checks(q, k, v, query_lens, key_lens, scale)
+    if out is None:
+        out = _heads_like(q)
+    _check(out.is_cuda and out.device == q.device and out.dtype == q.dtype and out.shape == q.shape, "Incorrect tensor sizes!")
+    batch, heads, len_q, d = q.shape
+    layouts = (capi.HeadsLayout * 4)(*[_heads_layout(t) for t in (q, k, v, out)])
+    lse = torch.empty(batch, heads, len_q, dtype=torch.float32, device=q.device) if with_lse else None
+    rc = capi.lib().ntb_cross_attention(q.device.index, _stream(q), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _ptr(lse),
+                                        X_FLOAT16, batch, heads, k.shape[1], len_q, k.shape[2], d, layouts,
+                                        _ptr(query_lens), _ptr(key_lens), scale)
+    _raise_rc(rc, "CrossAttention")
+    return (out, lse) if with_lse else out
+
+
 def RowStats(x):
     """(row maximum, sum of exp(x - maximum)) over the last dimension of a 2-D tensor, fp32."""
     _check(x.is_cuda and x.dim() == 2 and x.stride(1) == 1, "a CUDA matrix with unit column stride is required")
