@@ -174,6 +174,24 @@ int ntb_cross_attention(int devID, void * stream,
                         const ntb_heads_layout * layouts, const int * queryLens, const int * keyLens, float scale);
 
 /*
+ * Gradients of ntb_cross_attention, given its result out, its lse and dout = dE/dout (any strides):
+ * dq (as q), dk and dv (as k and v; the query heads that share a key head are summed) are written, not
+ * accumulated. layouts[0..7] are those of q, k, v, out, dout, dq, dk, dv, with the rules above; a broadcast
+ * k or v gets the gradient of every copy, so dk and dv are never broadcast. queryLens, keyLens and scale are
+ * the forward call's. Rows past a sequence's end may hold anything in q, k, v, out and dout, and get zeros in
+ * dq, dk, dv. work: device scratch of ntb_cross_attention_grad_work() bytes on a 16-byte boundary, the
+ * caller's, so that calls on several streams or in several captured graphs do not share it; its content
+ * need not survive the call. No atomics: results do not depend on timing. The reference has no such
+ * node; its backward pass runs the chain's own (source/network/XBackwardMath.cpp:714-786 for the products).
+ */
+long long ntb_cross_attention_grad_work(int batch, int headsQ, int lenQ);
+int ntb_cross_attention_grad(int devID, void * stream,
+                             const void * q, const void * k, const void * v, const void * out, const float * lse,
+                             const void * dout, void * dq, void * dk, void * dv, void * work, long long workBytes,
+                             int dtype, int batch, int headsQ, int headsKV, int lenQ, int lenK, int dim,
+                             const ntb_heads_layout * layouts, const int * queryLens, const int * keyLens, float scale);
+
+/*
  * Row-wise log-softmax over the last dimension in two halves, for logits whose rows are
  * spread over several GPUs (vocabulary shards of the output layer,
  * source/sample/transformer/submodel/Output.cpp:86-101, LogSoftmax.cpp:40-170).

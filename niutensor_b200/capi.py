@@ -39,6 +39,8 @@ PROTOTYPES = {
     "ntb_attention": (_i, [_i, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _ll, _f]),
     "ntb_attention_dropout": (_i, [_i, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _ll, _f, _f]),
     "ntb_cross_attention": (_i, [_i] + [_vp] * 6 + [_i] * 7 + [ctypes.POINTER(HeadsLayout), _vp, _vp, _f]),
+    "ntb_cross_attention_grad_work": (_ll, [_i] * 3),
+    "ntb_cross_attention_grad": (_i, [_i] + [_vp] * 11 + [_ll] + [_i] * 7 + [ctypes.POINTER(HeadsLayout), _vp, _vp, _f]),
     "ntb_row_stats": (_i, [_i, _vp, _vp, _i, _i, _i, _ll, _vp, _vp]),
     "ntb_logsoftmax_apply": (_i, [_i, _vp, _vp, _vp, _i, _i, _i, _ll, _ll, _vp, _vp]),
     "ntb_gemm_grad": (_i, [_i, _vp, _vp, _i, _vp, _i, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _f]),

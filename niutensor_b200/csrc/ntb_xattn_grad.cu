@@ -1,0 +1,899 @@
+/*
+ * Gradients of cross attention (ntb_xattn.cu), half tensors, sm_100a. With p_ij = exp(s_ij - lse_i)
+ * recomputed from the kept lse:
+ *
+ *     dv_j = sum_i p_ij do_i           dp_ij = do_i . v_j        delta_i = do_i . out_i
+ *     ds_ij = p_ij (dp_ij - delta_i)   dq_i = scale sum_j ds_ij k_j   dk_j = scale sum_i ds_ij q_i
+ *
+ * Two kernels, because the sums over j and over i run along different sides of the same score tiles and
+ * one kernel for both would have to add to dq with atomics, in an order that changes from run to run:
+ *
+ * XattnGradQKernel: a CTA owns a 128-row query tile of one head and walks the key tiles: S = q k^T,
+ * dP = do v^T, dQ += dS k (three products). It also forms delta and leaves it, with lse, for the other.
+ * XattnGradKVKernel: a CTA owns a 128-key tile of one key head and walks the query tiles of all heads
+ * that share it (so the gradients of a shared head are summed in tensor memory, in head order):
+ * S^T = k q^T, dP^T = v do^T, dV += P^T do, dK += dS^T q (four products).
+ *
+ * Both: eight warps, two threads a row (64 columns each), a TMA producer warp, an MMA warp. P and dS go
+ * back into tensor memory as halves over the tile they came from and are the A operand of the second
+ * products. The products of one step run under the exponentials of the next. Tensor memory is full
+ * (S, dP and two accumulators of 128 columns at head size 128), so tiles are not double buffered.
+ * Few tiles: the walk is split over a cluster of up to 8 CTAs, joined in rank order through
+ * distributed shared memory.
+ *
+ * Rounding: p is at most 1 and may be tiny (1 / lenK); for dv it is rounded to half as 2^12 p, exact powers
+ * of two away from half's subnormals. ds is rounded to half as it is: its scale is that of the gradients,
+ * which are halves themselves. Sums are fp32.
+ */
+#include "ntb_xattn.cuh"
+
+namespace ntb {
+
+namespace {
+
+constexpr int GR_THREADS = 320;
+constexpr int GR_PRODUCER = 8, GR_ISSUER = 9;
+constexpr float P_SCALE_LOG2 = 12.f, P_SCALE_INV = 1.f / 4096.f;
+
+struct XattnGradParams {
+    XattnShape sh;
+    HeadsAddr aQ, aK, aV, aDO;
+    const __half * out;
+    const __half * dout;
+    ntb_heads_layout lOut, lDO;
+    const float * lse;
+    float * work;              /* [batch, headsQ, tilesPerHead][2][128]: lse in the second kernel's units, delta */
+    int tilesPerHead, keyTiles;
+    int splits;
+    float scale, scaleLog2;
+    int * status;
+    /* the destinations of the split form */
+    __half * d0;               /* dq, or dk */
+    __half * d1;               /* dv */
+    ntb_heads_layout l0, l1;
+};
+
+template <int D> struct XattnGradSmem {
+    static constexpr int DC = D / 64;
+    static constexpr int TILE = DC * XBOX_BYTES;
+    /* first kernel: q, do, and a ring of k and v tiles */
+    static constexpr int SLOTS = D == 128 ? 5 : 8;
+    static constexpr int Q_TOTAL = (2 + SLOTS) * TILE + 1024;
+    /* second kernel: k, v, and a ring of (q, do, lse and delta) */
+    static constexpr int STAGE = 2 * TILE + 1024;
+    static constexpr int STAGES = D == 128 ? 2 : 4;
+    static constexpr int KV_TOTAL = 2 * TILE + STAGES * STAGE + 1024;
+    static_assert(SLOTS * TILE >= XT * D * 4 && STAGES * STAGE >= 2 * XT * D * 4, "the split's partial sums take the place of the ring");
+};
+
+__device__ __forceinline__ void GradBarrier() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
+
+/* one thread's 32 accumulator columns into its row of a split's partial sums, 16-byte chunks permuted by the row */
+__device__ __forceinline__ void StorePartial(uint32_t rowBase, int r, int chunk0, const uint32_t * o, bool have)
+{
+#pragma unroll
+    for (int jj = 0; jj < 8; jj++)
+        StoreShared16(rowBase + (((chunk0 + jj) ^ (r & 7)) << 4), have ? o[jj * 4] : 0u, have ? o[jj * 4 + 1] : 0u,
+                      have ? o[jj * 4 + 2] : 0u, have ? o[jj * 4 + 3] : 0u);
+}
+
+/* eight columns of a row summed over the cluster in rank order */
+__device__ __forceinline__ uint4 SumPartials(uint32_t rowBase, int r, int c, int splits, float factor)
+{
+    float acc[8] = { 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f };
+    for (int t = 0; t < splits; t++) {
+        const uint32_t base = MapShared(rowBase, t);
+#pragma unroll
+        for (int hf = 0; hf < 2; hf++) {
+            const float4 v = LoadRemote4(base + (((2 * c + hf) ^ (r & 7)) << 4));
+            acc[hf * 4 + 0] += v.x; acc[hf * 4 + 1] += v.y; acc[hf * 4 + 2] += v.z; acc[hf * 4 + 3] += v.w;
+        }
+    }
+    return make_uint4(PackHalf2(acc[0] * factor, acc[1] * factor), PackHalf2(acc[2] * factor, acc[3] * factor),
+                      PackHalf2(acc[4] * factor, acc[5] * factor), PackHalf2(acc[6] * factor, acc[7] * factor));
+}
+
+/* 64 columns of this thread's lane */
+__device__ __forceinline__ void TmemLoad64U(uint32_t taddr, uint32_t * x)
+{
+    TmemLoad32Async(taddr, x);
+    TmemLoad32Async(taddr + 32, x + 32);
+    TmemWaitLoad();
+}
+
+/* 32 columns of this thread's lane, scaled, into four 16-byte chunks of its row of a swizzled box */
+__device__ __forceinline__ void StageHalf32(uint32_t rowAddr, int lane, int chunk0, const uint32_t * o, float f, bool have)
+{
+#pragma unroll
+    for (int jj = 0; jj < 4; jj++) {
+        uint32_t w[4];
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+            w[e] = have ? PackHalf2(__uint_as_float(o[jj * 8 + 2 * e]) * f, __uint_as_float(o[jj * 8 + 2 * e + 1]) * f) : 0u;
+        StoreShared16(rowAddr + (((chunk0 + jj) ^ (lane & 7)) << 4), w[0], w[1], w[2], w[3]);
+    }
+}
+
+template <int D>
+__global__ void __launch_bounds__(GR_THREADS, 1)
+XattnGradQKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
+                 const __grid_constant__ CUtensorMap tmDO, const __grid_constant__ CUtensorMap tmDQ, const XattnGradParams p)
+{
+    using SM = XattnGradSmem<D>;
+    constexpr int DC = SM::DC, TILE = SM::TILE, SLOTS = SM::SLOTS;
+    constexpr int TMEM_S = 0, TMEM_DP = 128, TMEM_DQ = 256;
+    extern __shared__ uint8_t smemRaw[];
+    __shared__ __align__(8) uint64_t barFull[SLOTS], barEmpty[SLOTS], barQ, barDO, barS, barSRead, barDP, barDS, barDone, barFix;
+    __shared__ uint32_t tmemBaseSlot;
+    __shared__ int abortFlag;
+    __shared__ float sDelta[XT];
+
+    const int warp = threadIdx.x >> 5;
+    const int lane = threadIdx.x & 31;
+    const uint32_t smemBase = (SmemAddr(smemRaw) + 1023u) & ~1023u;
+    const uint32_t qS = smemBase, doS = qS + TILE, ringS = doS + TILE;
+    volatile int * abortPtr = &abortFlag;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+
+    if (warp == GR_PRODUCER && lane == 0) {
+        PrefetchTensorMap(&tmQ);
+        PrefetchTensorMap(&tmK);
+        PrefetchTensorMap(&tmV);
+        PrefetchTensorMap(&tmDO);
+        PrefetchTensorMap(&tmDQ);
+    }
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < SLOTS; i++) {
+            MbarInit(SmemAddr(&barFull[i]), 1);
+            MbarInit(SmemAddr(&barEmpty[i]), 1);
+        }
+        MbarInit(SmemAddr(&barQ), 1);
+        MbarInit(SmemAddr(&barDO), 1);
+        MbarInit(SmemAddr(&barS), 1);
+        MbarInit(SmemAddr(&barSRead), 256);
+        MbarInit(SmemAddr(&barDP), 1);
+        MbarInit(SmemAddr(&barDS), 256);
+        MbarInit(SmemAddr(&barDone), 1);
+        MbarInit(SmemAddr(&barFix), 1);
+        abortFlag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+    if (warp == GR_ISSUER) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
+                     :: "r"(SmemAddr(&tmemBaseSlot)), "r"(512u) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    TcFenceBefore();
+    __syncthreads();
+    TcFenceAfter();
+    const uint32_t tmemBase = *(volatile uint32_t *)&tmemBaseSlot;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+
+    const int rank = p.splits > 1 ? (int)ClusterRank() : 0;
+    const int item = (int)blockIdx.x / p.splits;
+    const int headItem = item / p.tilesPerHead;
+    const int q0 = (item - headItem * p.tilesPerHead) * XT;
+    const int b = headItem / p.sh.headsQ, h = headItem - b * p.sh.headsQ, kvHead = h / p.sh.group;
+    const int nq = ClampLen(p.sh.queryLens, b, p.sh.lenQ), nk = ClampLen(p.sh.keyLens, b, p.sh.lenK);
+    const int keyTiles = q0 < nq ? (nk + XT - 1) / XT : 0;
+    const int perSplit = (keyTiles + p.splits - 1) / p.splits;
+    const int tile0 = rank * perSplit < keyTiles ? rank * perSplit : keyTiles;
+    const int tile1 = tile0 + perSplit < keyTiles ? tile0 + perSplit : keyTiles;
+    const int n = tile1 - tile0;
+    /* the last tile reaches past the sequence's keys into rows that exist: those rows of k are cleared */
+    const bool fix = n > 0 && tile1 * XT > nk && nk < p.sh.lenK;
+
+    if (warp == GR_PRODUCER) {
+        if (lane == 0 && n > 0) {
+            bool ok = true;
+            MbarExpectTx(SmemAddr(&barQ), TILE);
+#pragma unroll
+            for (int dc = 0; dc < DC; dc++)
+                TmaLoad4D(qS + dc * XBOX_BYTES, &tmQ, SmemAddr(&barQ), dc * 64, q0, h * p.aQ.mulHead, b * p.aQ.mulBatch);
+            int slot = 0;
+            uint32_t phase = 0;
+            for (int t = 0; ok && t < 2 * n; t++) {
+                if (t >= SLOTS)
+                    ok = MbarWait(SmemAddr(&barEmpty[slot]), phase ^ 1u, abortPtr, p.status);
+                if (!ok)
+                    break;
+                if (t == 1) {
+                    MbarExpectTx(SmemAddr(&barDO), TILE);
+#pragma unroll
+                    for (int dc = 0; dc < DC; dc++)
+                        TmaLoad4D(doS + dc * XBOX_BYTES, &tmDO, SmemAddr(&barDO), dc * 64, q0, h * p.aDO.mulHead, b * p.aDO.mulBatch);
+                }
+                const int row = (tile0 + (t >> 1)) * XT;
+                const uint32_t dst = ringS + slot * TILE, bar = SmemAddr(&barFull[slot]);
+                MbarExpectTx(bar, TILE);
+                if ((t & 1) == 0) {
+#pragma unroll
+                    for (int dc = 0; dc < DC; dc++)
+                        TmaLoad4D(dst + dc * XBOX_BYTES, &tmK, bar, dc * 64, row, kvHead * p.aK.mulHead, b * p.aK.mulBatch);
+                }
+                else {
+#pragma unroll
+                    for (int dc = 0; dc < DC; dc++)
+                        TmaLoad4D(dst + dc * XBOX_BYTES, &tmV, bar, dc * 64, row, kvHead * p.aV.mulHead, b * p.aV.mulBatch);
+                }
+                if (++slot == SLOTS) {
+                    slot = 0;
+                    phase ^= 1u;
+                }
+            }
+        }
+        __syncwarp();
+        if (fix) {
+            /* after its load and before the products that read it as rows of the sum; the scores of these keys
+               may be taken from either state, their weights are set to 0 */
+            const int t = 2 * n - 2, slot = t % SLOTS;
+            if (MbarWaitWarp(SmemAddr(&barFull[slot]), (uint32_t)(t / SLOTS) & 1u, abortPtr, p.status, 200)) {
+                ZeroTileRows(ringS + slot * TILE, DC, nk - (tile1 - 1) * XT, lane);
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0)
+                    MbarArrive(SmemAddr(&barFix));
+            }
+        }
+    }
+    else if (warp == GR_ISSUER) {
+        if (lane == 0 && n > 0) {
+            constexpr uint32_t descS = XattnDesc(XT, 0), descQ = XattnDesc(D, 1);
+            auto product = [&](uint32_t dst, uint32_t aTile, uint32_t bTile) {
+#pragma unroll
+                for (int dc = 0; dc < DC; dc++)
+#pragma unroll
+                    for (int ks = 0; ks < 4; ks++)
+                        TcMma<0>(dst, SmemDesc(aTile + dc * XBOX_BYTES + ks * UMMA_K_BYTES, 16, 1024, 2),
+                                 SmemDesc(bTile + dc * XBOX_BYTES + ks * UMMA_K_BYTES, 16, 1024, 2), descS, (dc | ks) != 0 ? 1u : 0u);
+            };
+            auto full = [&](int t) { return MbarWait(SmemAddr(&barFull[t % SLOTS]), (uint32_t)(t / SLOTS) & 1u, abortPtr, p.status); };
+            bool ok = MbarWait(SmemAddr(&barQ), 0, abortPtr, p.status) && full(0);
+            if (ok) {
+                TcFenceAfter();
+                product(tmemBase + TMEM_S, qS, ringS);
+                TcCommit(SmemAddr(&barS));
+                ok = MbarWait(SmemAddr(&barDO), 0, abortPtr, p.status) && full(1);
+            }
+            if (ok) {
+                TcFenceAfter();
+                product(tmemBase + TMEM_DP, doS, ringS + TILE);
+                TcCommit(SmemAddr(&barDP));
+                TcCommit(SmemAddr(&barEmpty[1]));
+            }
+            for (int j = 0; ok && j < n; j++) {
+                const int tk = 2 * j;
+                const bool more = j + 1 < n;
+                if (more) {
+                    ok = full(tk + 2) && MbarWait(SmemAddr(&barSRead), (uint32_t)j & 1u, abortPtr, p.status);
+                    if (!ok)
+                        break;
+                    TcFenceAfter();
+                    product(tmemBase + TMEM_S, qS, ringS + ((tk + 2) % SLOTS) * TILE);
+                    TcCommit(SmemAddr(&barS));
+                }
+                if (!more && fix)
+                    ok = MbarWait(SmemAddr(&barFix), 0, abortPtr, p.status);
+                ok = ok && MbarWait(SmemAddr(&barDS), (uint32_t)j & 1u, abortPtr, p.status);
+                if (!ok)
+                    break;
+                TcFenceAfter();
+                const uint32_t kTile = ringS + (tk % SLOTS) * TILE;
+#pragma unroll
+                for (int ks = 0; ks < XT / 16; ks++)
+                    TcMmaTmemA(tmemBase + TMEM_DQ, tmemBase + TMEM_DP + (ks >> 2) * 64 + (ks & 3) * 8,
+                               SmemDesc(kTile + ks * 16 * ROW_BYTES, XBOX_BYTES, 1024, 2), descQ, (j | ks) != 0 ? 1u : 0u);
+                TcCommit(SmemAddr(&barEmpty[tk % SLOTS]));
+                if (more) {
+                    ok = full(tk + 3);
+                    if (!ok)
+                        break;
+                    TcFenceAfter();
+                    product(tmemBase + TMEM_DP, doS, ringS + ((tk + 3) % SLOTS) * TILE);
+                    TcCommit(SmemAddr(&barDP));
+                    TcCommit(SmemAddr(&barEmpty[(tk + 3) % SLOTS]));
+                }
+                else
+                    TcCommit(SmemAddr(&barDone));
+            }
+        }
+    }
+    else {
+        const int hf = warp >> 2, sub = warp & 3;
+        const uint32_t laneBase = (uint32_t)(sub * 32) << 16;
+        const int r = sub * 32 + lane, row = q0 + r;
+        const bool rowLive = row < nq && nk > 0;
+        /* delta, half of the row a thread, joined through shared memory */
+        float part = 0.f;
+        if (rowLive) {
+            const __half * o = p.out + b * p.lOut.batch + h * p.lOut.head + row * p.lOut.row;
+            const __half * g = p.dout + b * p.lDO.batch + h * p.lDO.head + row * p.lDO.row;
+#pragma unroll
+            for (int c = 0; c < D / 16; c++) {
+                const int col = hf * (D / 2) + c * 8;
+                if (col < p.sh.dim) {
+                    const uint4 x = *(const uint4 *)(o + col), y = *(const uint4 *)(g + col);
+                    const uint32_t xs[4] = { x.x, x.y, x.z, x.w }, ys[4] = { y.x, y.y, y.z, y.w };
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const float2 xf = __half22float2(*(const __half2 *)&xs[e]), yf = __half22float2(*(const __half2 *)&ys[e]);
+                        part = fmaf(xf.x, yf.x, part);
+                        part = fmaf(xf.y, yf.y, part);
+                    }
+                }
+            }
+        }
+        if (hf == 1)
+            sDelta[r] = part;
+        GradBarrier();
+        if (hf == 0)
+            sDelta[r] = part + sDelta[r];
+        GradBarrier();
+        const float delta = sDelta[r];
+        /* exponents of 2; plus infinity makes every weight of an empty row 0 */
+        const float lse2 = rowLive ? p.lse[((long long)b * p.sh.headsQ + h) * p.sh.lenQ + row] * LOG2E : INFINITY;
+        if (hf == 0 && rank == 0) {          /* the second kernel's exponents carry the factor of p; dP and delta its inverse */
+            float * w = p.work + (long long)item * (2 * XT);
+            w[r] = lse2 - P_SCALE_LOG2;
+            w[XT + r] = delta * P_SCALE_INV;
+        }
+        const uint32_t sT = tmemBase + laneBase + TMEM_S + hf * 64, dpT = tmemBase + laneBase + TMEM_DP + hf * 64;
+        bool ok = true;
+        for (int j = 0; j < n; j++) {
+            const uint32_t ph = (uint32_t)j & 1u;
+            ok = MbarWaitWarp(SmemAddr(&barS), ph, abortPtr, p.status, 200);
+            if (!ok)
+                break;
+            TcFenceAfter();
+            uint32_t x[64];
+            TmemLoad64U(sT, x);
+            TcFenceBefore();
+            MbarArrive(SmemAddr(&barSRead));
+#pragma unroll
+            for (int e = 0; e < 64; e++)
+                x[e] = __float_as_uint(Exp2(fmaf(__uint_as_float(x[e]), p.scaleLog2, -lse2)));
+            const int valid = nk - (tile0 + j) * XT - hf * 64;
+            ok = MbarWaitWarp(SmemAddr(&barDP), ph, abortPtr, p.status, 200);
+            if (!ok)
+                break;
+            TcFenceAfter();
+#pragma unroll
+            for (int c = 0; c < 2; c++) {
+                uint32_t y[32], w[16];
+                TmemLoad32Async(dpT + c * 32, y);
+                TmemWaitLoad();
+#pragma unroll
+                for (int e = 0; e < 32; e++) {
+                    const float ds = __uint_as_float(x[c * 32 + e]) * (__uint_as_float(y[e]) - delta);
+                    y[e] = valid >= 64 || c * 32 + e < valid ? __float_as_uint(ds) : 0u;
+                }
+#pragma unroll
+                for (int e = 0; e < 16; e++)
+                    w[e] = PackHalf2(__uint_as_float(y[2 * e]), __uint_as_float(y[2 * e + 1]));
+                TmemStore16Async(dpT + c * 16, w);
+            }
+            TmemWaitStore();
+            TcFenceBefore();
+            MbarArrive(SmemAddr(&barDS));
+        }
+        if (n > 0 && ok)
+            ok = MbarWaitWarp(SmemAddr(&barDone), 0, abortPtr, p.status, 200);
+        TcFenceAfter();
+        const bool sums = n > 0 && ok;
+        const uint32_t dqT = tmemBase + laneBase + TMEM_DQ;
+#pragma unroll
+        for (int c = hf * (D / 64); c < (hf + 1) * (D / 64); c++) {       /* 32 columns a step; this half's D / 2 */
+            uint32_t o[32];
+            if (sums) {
+                TmemLoad32Async(dqT + c * 32, o);
+                TmemWaitLoad();
+            }
+            if (p.splits == 1)
+                StageHalf32(qS + (c >> 1) * XBOX_BYTES + r * ROW_BYTES, lane, (c & 1) * 4, o, p.scale, sums && rowLive);
+            else
+                StorePartial(ringS + r * D * 4, r, c * 8, o, sums);
+        }
+        if (p.splits == 1 && ok) {
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            GradBarrier();
+            if (hf == 0 && lane == 0 && q0 + sub * 32 < p.sh.lenQ) {
+#pragma unroll
+                for (int dc = 0; dc < DC; dc++)
+                    TmaStore4D(&tmDQ, qS + dc * XBOX_BYTES + sub * 32 * ROW_BYTES, dc * 64, q0 + sub * 32, h, b);
+                asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+                asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+            }
+        }
+        __syncwarp();
+    }
+
+    __syncwarp();
+    if (*abortPtr) {
+        const long long t0 = clock64();
+        while (clock64() - t0 < 2000000LL) { }
+    }
+    if (p.splits > 1) {
+        ClusterSync();
+        if (warp < 8) {
+            const int rowsEach = XT / p.splits, chunks = D / 8;
+            for (int i = threadIdx.x; i < rowsEach * chunks; i += 256) {
+                const int c = i % chunks, r = rank * rowsEach + i / chunks, row = q0 + r;
+                if (row >= p.sh.lenQ || c * 8 >= p.sh.dim)
+                    continue;
+                uint4 w = make_uint4(0u, 0u, 0u, 0u);
+                if (row < nq && nk > 0)
+                    w = SumPartials(ringS + r * D * 4, r, c, p.splits, p.scale);
+                *(uint4 *)(p.d0 + b * p.l0.batch + h * p.l0.head + row * p.l0.row + c * 8) = w;
+            }
+        }
+        __syncwarp();
+        ClusterSync();
+    }
+    TcFenceBefore();
+    __syncthreads();
+    TcFenceAfter();
+    if (warp == GR_ISSUER)
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" :: "r"(tmemBase), "r"(512u) : "memory");
+}
+
+template <int D>
+__global__ void __launch_bounds__(GR_THREADS, 1)
+XattnGradKVKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
+                  const __grid_constant__ CUtensorMap tmDO, const __grid_constant__ CUtensorMap tmDK, const __grid_constant__ CUtensorMap tmDV,
+                  const XattnGradParams p)
+{
+    using SM = XattnGradSmem<D>;
+    constexpr int DC = SM::DC, TILE = SM::TILE, STAGES = SM::STAGES, STAGE = SM::STAGE;
+    constexpr int TMEM_S = 0, TMEM_DP = 128, TMEM_DV = 256, TMEM_DK = 256 + D;
+    extern __shared__ uint8_t smemRaw[];
+    __shared__ __align__(8) uint64_t barFull[STAGES], barEmpty[STAGES], barKV, barLoad, barS, barP, barDP, barDS, barDone;
+    __shared__ uint32_t tmemBaseSlot;
+    __shared__ int abortFlag;
+
+    const int warp = threadIdx.x >> 5;
+    const int lane = threadIdx.x & 31;
+    const uint32_t smemBase = (SmemAddr(smemRaw) + 1023u) & ~1023u;
+    const uint32_t kS = smemBase, vS = kS + TILE, ringS = vS + TILE;
+    volatile int * abortPtr = &abortFlag;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+
+    if (warp == GR_PRODUCER && lane == 0) {
+        PrefetchTensorMap(&tmQ);
+        PrefetchTensorMap(&tmK);
+        PrefetchTensorMap(&tmV);
+        PrefetchTensorMap(&tmDO);
+        PrefetchTensorMap(&tmDK);
+        PrefetchTensorMap(&tmDV);
+    }
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < STAGES; i++) {
+            MbarInit(SmemAddr(&barFull[i]), 1);
+            MbarInit(SmemAddr(&barEmpty[i]), 1);
+        }
+        MbarInit(SmemAddr(&barKV), 1);
+        MbarInit(SmemAddr(&barS), 1);
+        MbarInit(SmemAddr(&barP), 256);
+        MbarInit(SmemAddr(&barDP), 1);
+        MbarInit(SmemAddr(&barDS), 256);
+        MbarInit(SmemAddr(&barDone), 1);
+        MbarInit(SmemAddr(&barLoad), 1);
+        abortFlag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+    if (warp == GR_ISSUER) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
+                     :: "r"(SmemAddr(&tmemBaseSlot)), "r"(512u) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    TcFenceBefore();
+    __syncthreads();
+    TcFenceAfter();
+    const uint32_t tmemBase = *(volatile uint32_t *)&tmemBaseSlot;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+
+    const int rank = p.splits > 1 ? (int)ClusterRank() : 0;
+    const int item = (int)blockIdx.x / p.splits;
+    const int headItem = item / p.keyTiles;
+    const int k0 = (item - headItem * p.keyTiles) * XT;
+    const int b = headItem / p.sh.headsKV, kvHead = headItem - b * p.sh.headsKV;
+    const int nq = ClampLen(p.sh.queryLens, b, p.sh.lenQ), nk = ClampLen(p.sh.keyLens, b, p.sh.lenK);
+    const int qTiles = (nq + XT - 1) / XT;
+    const int steps = k0 < nk ? p.sh.group * qTiles : 0;
+    const int perSplit = (steps + p.splits - 1) / p.splits;
+    const int step0 = rank * perSplit < steps ? rank * perSplit : steps;
+    const int step1 = step0 + perSplit < steps ? step0 + perSplit : steps;
+    const int n = step1 - step0;
+    const bool ragged = nq < p.sh.lenQ && nq % XT != 0;       /* a head's last query tile reaches into rows past the sequence */
+
+    if (warp == GR_PRODUCER) {
+        bool ok = true;
+        uint32_t edges = 0;
+        if (n > 0 && lane == 0) {
+            MbarExpectTx(SmemAddr(&barKV), 2 * TILE);
+#pragma unroll
+            for (int dc = 0; dc < DC; dc++) {
+                TmaLoad4D(kS + dc * XBOX_BYTES, &tmK, SmemAddr(&barKV), dc * 64, k0, kvHead * p.aK.mulHead, b * p.aK.mulBatch);
+                TmaLoad4D(vS + dc * XBOX_BYTES, &tmV, SmemAddr(&barKV), dc * 64, k0, kvHead * p.aV.mulHead, b * p.aV.mulBatch);
+            }
+        }
+        for (int i = 0; ok && i < n; i++) {
+            const int st = i % STAGES, step = step0 + i;
+            const int g = step / qTiles, qt = step - g * qTiles, h = kvHead * p.sh.group + g;
+            /* a tile with rows past the sequence arrives on the producer's own barrier and is handed on by the warp */
+            const bool edge = ragged && qt == qTiles - 1;
+            const uint32_t dst = ringS + st * STAGE, bar = edge ? SmemAddr(&barLoad) : SmemAddr(&barFull[st]);
+            if (i >= STAGES)
+                ok = MbarWaitWarp(SmemAddr(&barEmpty[st]), (uint32_t)(i / STAGES + 1) & 1u, abortPtr, p.status, 200);
+            if (!ok)
+                break;
+            if (lane == 0) {
+                MbarExpectTx(bar, 2 * TILE + 2 * XT * 4);
+#pragma unroll
+                for (int dc = 0; dc < DC; dc++)
+                    TmaLoad4D(dst + dc * XBOX_BYTES, &tmQ, bar, dc * 64, qt * XT, h * p.aQ.mulHead, b * p.aQ.mulBatch);
+#pragma unroll
+                for (int dc = 0; dc < DC; dc++)
+                    TmaLoad4D(dst + TILE + dc * XBOX_BYTES, &tmDO, bar, dc * 64, qt * XT, h * p.aDO.mulHead, b * p.aDO.mulBatch);
+                const float * src = p.work + (((long long)b * p.sh.headsQ + h) * p.tilesPerHead + qt) * (2 * XT);
+                asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                             :: "r"(dst + 2 * TILE), "l"(src), "r"(2u * XT * 4u), "r"(bar) : "memory");
+            }
+            __syncwarp();
+            if (edge) {
+                /* rows of q and do past the sequence: their weights are 0, and 0 * NaN would reach the sums */
+                ok = MbarWaitWarp(bar, edges++ & 1u, abortPtr, p.status, 200);
+                if (!ok)
+                    break;
+                (void)MbarTryWait(bar, (edges - 1) & 1u, 0);
+                ZeroTileRows(dst, DC, nq - qt * XT, lane);
+                ZeroTileRows(dst + TILE, DC, nq - qt * XT, lane);
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0)
+                    MbarArrive(SmemAddr(&barFull[st]));
+            }
+        }
+    }
+    else if (warp == GR_ISSUER) {
+        if (lane == 0 && n > 0) {
+            constexpr uint32_t descS = XattnDesc(XT, 0), descD = XattnDesc(D, 1);
+            auto product = [&](uint32_t dst, uint32_t aTile, uint32_t bTile) {
+#pragma unroll
+                for (int dc = 0; dc < DC; dc++)
+#pragma unroll
+                    for (int ks = 0; ks < 4; ks++)
+                        TcMma<0>(dst, SmemDesc(aTile + dc * XBOX_BYTES + ks * UMMA_K_BYTES, 16, 1024, 2),
+                                 SmemDesc(bTile + dc * XBOX_BYTES + ks * UMMA_K_BYTES, 16, 1024, 2), descS, (dc | ks) != 0 ? 1u : 0u);
+            };
+            auto second = [&](uint32_t dst, uint32_t aTmem, uint32_t bTile, bool first) {
+#pragma unroll
+                for (int ks = 0; ks < XT / 16; ks++)
+                    TcMmaTmemA(dst, aTmem + (ks >> 2) * 64 + (ks & 3) * 8, SmemDesc(bTile + ks * 16 * ROW_BYTES, XBOX_BYTES, 1024, 2), descD,
+                               !first || ks != 0 ? 1u : 0u);
+            };
+            auto full = [&](int i) { return MbarWait(SmemAddr(&barFull[i % STAGES]), (uint32_t)(i / STAGES) & 1u, abortPtr, p.status); };
+            bool ok = MbarWait(SmemAddr(&barKV), 0, abortPtr, p.status) && full(0);
+            if (ok) {
+                TcFenceAfter();
+                product(tmemBase + TMEM_S, kS, ringS);
+                TcCommit(SmemAddr(&barS));
+                product(tmemBase + TMEM_DP, vS, ringS + TILE);
+                TcCommit(SmemAddr(&barDP));
+            }
+            for (int i = 0; ok && i < n; i++) {
+                const uint32_t ph = (uint32_t)i & 1u;
+                const uint32_t cur = ringS + (i % STAGES) * STAGE, nxt = ringS + ((i + 1) % STAGES) * STAGE;
+                const bool more = i + 1 < n;
+                ok = MbarWait(SmemAddr(&barP), ph, abortPtr, p.status);
+                if (!ok)
+                    break;
+                TcFenceAfter();
+                second(tmemBase + TMEM_DV, tmemBase + TMEM_S, cur + TILE, i == 0);
+                if (more) {
+                    ok = full(i + 1);
+                    if (!ok)
+                        break;
+                    TcFenceAfter();
+                    product(tmemBase + TMEM_S, kS, nxt);
+                    TcCommit(SmemAddr(&barS));
+                }
+                ok = MbarWait(SmemAddr(&barDS), ph, abortPtr, p.status);
+                if (!ok)
+                    break;
+                TcFenceAfter();
+                second(tmemBase + TMEM_DK, tmemBase + TMEM_DP, cur, i == 0);
+                TcCommit(SmemAddr(&barEmpty[i % STAGES]));
+                if (more) {
+                    product(tmemBase + TMEM_DP, vS, nxt + TILE);
+                    TcCommit(SmemAddr(&barDP));
+                }
+                else
+                    TcCommit(SmemAddr(&barDone));
+            }
+        }
+    }
+    else {
+        const int hf = warp >> 2, sub = warp & 3;
+        const uint32_t laneBase = (uint32_t)(sub * 32) << 16;
+        const int r = sub * 32 + lane;
+        const uint32_t sT = tmemBase + laneBase + TMEM_S + hf * 64, dpT = tmemBase + laneBase + TMEM_DP + hf * 64;
+        const float4 * statsBase = (const float4 *)(smemRaw + (ringS - SmemAddr(smemRaw)) + 2 * TILE);
+        bool ok = true;
+        for (int i = 0; i < n; i++) {
+            const uint32_t ph = (uint32_t)i & 1u;
+            const int st = i % STAGES;
+            const float4 * lse4 = statsBase + st * (STAGE / 16) + hf * 16, * delta4 = lse4 + XT / 4;
+            ok = MbarWaitWarp(SmemAddr(&barFull[st]), (uint32_t)(i / STAGES) & 1u, abortPtr, p.status, 200) &&
+                 MbarWaitWarp(SmemAddr(&barS), ph, abortPtr, p.status, 200);
+            if (!ok)
+                break;
+            /* every lane observes the copy's completion itself before it reads what was copied */
+            (void)MbarTryWait(SmemAddr(&barFull[st]), (uint32_t)(i / STAGES) & 1u, 0);
+            TcFenceAfter();
+            uint32_t x[64];
+            TmemLoad64U(sT, x);
+#pragma unroll
+            for (int c = 0; c < 2; c++) {
+                uint32_t w[16];
+#pragma unroll
+                for (int e4 = 0; e4 < 8; e4++) {
+                    const float4 ls = lse4[c * 8 + e4];
+                    const int e = c * 32 + e4 * 4;
+                    const float p0 = Exp2(fmaf(__uint_as_float(x[e]), p.scaleLog2, -ls.x)), p1 = Exp2(fmaf(__uint_as_float(x[e + 1]), p.scaleLog2, -ls.y));
+                    const float p2 = Exp2(fmaf(__uint_as_float(x[e + 2]), p.scaleLog2, -ls.z)), p3 = Exp2(fmaf(__uint_as_float(x[e + 3]), p.scaleLog2, -ls.w));
+                    x[e] = __float_as_uint(p0); x[e + 1] = __float_as_uint(p1);
+                    x[e + 2] = __float_as_uint(p2); x[e + 3] = __float_as_uint(p3);
+                    w[e4 * 2] = PackHalf2(p0, p1);
+                    w[e4 * 2 + 1] = PackHalf2(p2, p3);
+                }
+                TmemStore16Async(sT + c * 16, w);
+            }
+            TmemWaitStore();
+            TcFenceBefore();
+            MbarArrive(SmemAddr(&barP));
+            ok = MbarWaitWarp(SmemAddr(&barDP), ph, abortPtr, p.status, 200);
+            if (!ok)
+                break;
+            TcFenceAfter();
+#pragma unroll
+            for (int c = 0; c < 2; c++) {
+                uint32_t y[32], w[16];
+                TmemLoad32Async(dpT + c * 32, y);
+                TmemWaitLoad();
+#pragma unroll
+                for (int e4 = 0; e4 < 8; e4++) {
+                    const float4 de = delta4[c * 8 + e4];
+                    const int e = e4 * 4, xe = c * 32 + e;
+                    const float d0 = __uint_as_float(x[xe]) * fmaf(__uint_as_float(y[e]), P_SCALE_INV, -de.x);
+                    const float d1 = __uint_as_float(x[xe + 1]) * fmaf(__uint_as_float(y[e + 1]), P_SCALE_INV, -de.y);
+                    const float d2 = __uint_as_float(x[xe + 2]) * fmaf(__uint_as_float(y[e + 2]), P_SCALE_INV, -de.z);
+                    const float d3 = __uint_as_float(x[xe + 3]) * fmaf(__uint_as_float(y[e + 3]), P_SCALE_INV, -de.w);
+                    w[e4 * 2] = PackHalf2(d0, d1);
+                    w[e4 * 2 + 1] = PackHalf2(d2, d3);
+                }
+                TmemStore16Async(dpT + c * 16, w);
+            }
+            TmemWaitStore();
+            TcFenceBefore();
+            MbarArrive(SmemAddr(&barDS));
+        }
+        if (n > 0 && ok)
+            ok = MbarWaitWarp(SmemAddr(&barDone), 0, abortPtr, p.status, 200);
+        TcFenceAfter();
+        const bool sums = n > 0 && ok, rowLive = k0 + r < nk;
+        /* warps 0-3: dv, in the place of v; warps 4-7: dk, in the place of k */
+        const uint32_t accT = tmemBase + laneBase + (hf == 0 ? TMEM_DV : TMEM_DK);
+        const uint32_t box = (hf == 0 ? vS : kS) + sub * 32 * ROW_BYTES;
+        const float factor = hf == 0 ? P_SCALE_INV : p.scale;
+#pragma unroll
+        for (int c = 0; c < D / 32; c++) {
+            uint32_t o[32];
+            if (sums) {
+                TmemLoad32Async(accT + c * 32, o);
+                TmemWaitLoad();
+            }
+            if (p.splits == 1)
+                StageHalf32(box + (c >> 1) * XBOX_BYTES + lane * ROW_BYTES, lane, (c & 1) * 4, o, factor, sums && rowLive);
+            else
+                StorePartial(ringS + (hf * XT + r) * D * 4, r, c * 8, o, sums);
+        }
+        if (p.splits == 1 && ok) {
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0 && k0 + sub * 32 < p.sh.lenK) {
+#pragma unroll
+                for (int dc = 0; dc < DC; dc++)
+                    TmaStore4D(hf == 0 ? &tmDV : &tmDK, box + dc * XBOX_BYTES, dc * 64, k0 + sub * 32, kvHead, b);
+                asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+                asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+            }
+        }
+        __syncwarp();
+    }
+
+    __syncwarp();
+    if (*abortPtr) {
+        const long long t0 = clock64();
+        while (clock64() - t0 < 2000000LL) { }
+    }
+    if (p.splits > 1) {
+        ClusterSync();
+        if (warp < 8) {
+            const int rowsEach = XT / p.splits, chunks = D / 8;
+            for (int i = threadIdx.x; i < 2 * rowsEach * chunks; i += 256) {
+                const int c = i % chunks, rr = i / chunks, which = rr / rowsEach;
+                const int r = rank * rowsEach + (rr - which * rowsEach), row = k0 + r;
+                if (row >= p.sh.lenK || c * 8 >= p.sh.dim)
+                    continue;
+                uint4 w = make_uint4(0u, 0u, 0u, 0u);
+                if (row < nk && steps > 0)
+                    w = SumPartials(ringS + (which * XT + r) * D * 4, r, c, p.splits, which == 0 ? P_SCALE_INV : p.scale);
+                if (which == 0)
+                    *(uint4 *)(p.d1 + b * p.l1.batch + kvHead * p.l1.head + row * p.l1.row + c * 8) = w;
+                else
+                    *(uint4 *)(p.d0 + b * p.l0.batch + kvHead * p.l0.head + row * p.l0.row + c * 8) = w;
+            }
+        }
+        __syncwarp();
+        ClusterSync();
+    }
+    TcFenceBefore();
+    __syncthreads();
+    TcFenceAfter();
+    if (warp == GR_ISSUER)
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" :: "r"(tmemBase), "r"(512u) : "memory");
+}
+
+struct GradCall {
+    XattnShape sh;
+    const void * q;
+    const void * k;
+    const void * v;
+    const void * out;
+    const void * dout;
+    const float * lse;
+    void * dq;
+    void * dk;
+    void * dv;
+    float * work;
+    const ntb_heads_layout * l;      /* q, k, v, out, dout, dq, dk, dv */
+    float scale;
+};
+
+/* CTAs of a cluster that share one item's walk: until one wave is full, while a part keeps two steps; and parts
+   short enough that the tensor core's accumulator, which rounds toward zero at every instruction, stays good */
+int GradSplits(long long items, int steps, int smCount)
+{
+    int splits = 1;
+    while (splits < 8 && ((items * splits * 2 <= smCount && steps >= splits * 4) || steps / splits > 1024))
+        splits *= 2;
+    return splits;
+}
+
+template <int D>
+int LaunchGrad(const DeviceCtx & ctx, const GradCall & call, cudaStream_t stream)
+{
+    using SM = XattnGradSmem<D>;
+    const XattnShape & s = call.sh;
+    XattnGradParams p;
+    memset(&p, 0, sizeof(p));
+    p.sh = s;
+    p.out = (const __half *)call.out;
+    p.dout = (const __half *)call.dout;
+    p.lOut = call.l[3];
+    p.lDO = call.l[4];
+    p.lse = call.lse;
+    p.work = call.work;
+    p.tilesPerHead = (s.lenQ + XT - 1) / XT;
+    p.keyTiles = (s.lenK + XT - 1) / XT;
+    p.scale = call.scale;
+    p.scaleLog2 = call.scale * LOG2E;
+    p.status = ctx.status;
+    const long long itemsQ = (long long)s.batch * s.headsQ * p.tilesPerHead, itemsKV = (long long)s.batch * s.headsKV * p.keyTiles;
+    const int splitsQ = GradSplits(itemsQ, p.keyTiles, ctx.smCount);
+    const long long steps = (long long)s.group * p.tilesPerHead;
+    if (steps > 0x3fffffffLL || itemsQ * splitsQ > 0x7fffffffLL)
+        return NTB_ERR_LIMIT;
+    const int splitsKV = GradSplits(itemsKV, (int)steps, ctx.smCount);
+    if (itemsKV * splitsKV > 0x7fffffffLL)
+        return NTB_ERR_LIMIT;
+    CUtensorMap tmQ, tmK, tmV, tmDO, tmDQ, tmDK, tmDV;
+    HeadsAddr unused;
+    int rc;
+    if (s.lenQ > 0 &&
+        ((rc = EncodeHeads(&tmQ, &p.aQ, call.q, s.dim, s.lenQ, s.headsQ, s.batch, call.l[0], XT)) != NTB_OK ||
+         (rc = EncodeHeads(&tmDO, &p.aDO, call.dout, s.dim, s.lenQ, s.headsQ, s.batch, call.l[4], XT)) != NTB_OK ||
+         (rc = EncodeHeads(&tmDQ, &unused, call.dq, s.dim, s.lenQ, s.headsQ, s.batch, call.l[5], 32)) != NTB_OK))
+        return rc;
+    if (s.lenK > 0 &&
+        ((rc = EncodeHeads(&tmK, &p.aK, call.k, s.dim, s.lenK, s.headsKV, s.batch, call.l[1], XT)) != NTB_OK ||
+         (rc = EncodeHeads(&tmV, &p.aV, call.v, s.dim, s.lenK, s.headsKV, s.batch, call.l[2], XT)) != NTB_OK ||
+         (rc = EncodeHeads(&tmDK, &unused, call.dk, s.dim, s.lenK, s.headsKV, s.batch, call.l[6], 32)) != NTB_OK ||
+         (rc = EncodeHeads(&tmDV, &unused, call.dv, s.dim, s.lenK, s.headsKV, s.batch, call.l[7], 32)) != NTB_OK))
+        return rc;
+    /* an empty side's maps are never used: no step touches it */
+    if (s.lenQ == 0) {
+        tmQ = tmDO = tmK;
+        p.aQ = p.aDO = p.aK;
+    }
+    if (s.lenK == 0) {
+        tmK = tmV = tmQ;
+        p.aK = p.aV = p.aQ;
+    }
+    static SmemOptIn optQ, optKV;
+    if (!optQ.Ensure((const void *)XattnGradQKernel<D>, SM::Q_TOTAL) || !optKV.Ensure((const void *)XattnGradKVKernel<D>, SM::KV_TOTAL))
+        return NTB_ERR_CUDA;
+    cudaError_t err = cudaSuccess;
+    if (itemsQ > 0) {
+        p.splits = splitsQ;
+        p.d0 = (__half *)call.dq;
+        p.l0 = call.l[5];
+        err = LaunchClusterPdl(XattnGradQKernel<D>, (unsigned)(itemsQ * splitsQ), GR_THREADS, SM::Q_TOTAL, splitsQ, stream, tmQ, tmK, tmV, tmDO, tmDQ, p);
+        CountLaunch();
+    }
+    if (err == cudaSuccess && itemsKV > 0) {
+        p.splits = splitsKV;
+        p.d0 = (__half *)call.dk;
+        p.l0 = call.l[6];
+        p.d1 = (__half *)call.dv;
+        p.l1 = call.l[7];
+        err = LaunchClusterPdl(XattnGradKVKernel<D>, (unsigned)(itemsKV * splitsKV), GR_THREADS, SM::KV_TOTAL, splitsKV, stream, tmQ, tmK, tmV, tmDO, tmDK, tmDV, p);
+        CountLaunch();
+    }
+    return (err == cudaSuccess && cudaGetLastError() == cudaSuccess) ? NTB_OK : NTB_ERR_CUDA;
+}
+
+}
+
+}
+
+using namespace ntb;
+
+extern "C" long long ntb_cross_attention_grad_work(int batch, int headsQ, int lenQ)
+{
+    if (batch < 0 || headsQ < 0 || lenQ < 0)
+        return 0;
+    return (long long)batch * headsQ * (((long long)lenQ + XT - 1) / XT) * (2 * XT) * (long long)sizeof(float);
+}
+
+extern "C" int ntb_cross_attention_grad(int devID, void * stream, const void * q, const void * k, const void * v,
+                                        const void * out, const float * lse, const void * dout,
+                                        void * dq, void * dk, void * dv, void * work, long long workBytes,
+                                        int dtype, int batch, int headsQ, int headsKV, int lenQ, int lenK, int dim,
+                                        const ntb_heads_layout * layouts, const int * queryLens, const int * keyLens, float scale)
+{
+    GradCall call;
+    memset(&call, 0, sizeof(call));
+    int rc = XattnShapeOf(call.sh, dtype, batch, headsQ, headsKV, lenQ, lenK, dim, queryLens, keyLens, scale);
+    if (rc != NTB_OK)
+        return rc;
+    if (batch == 0 || headsKV == 0 || headsQ == 0 || (lenQ == 0 && lenK == 0))
+        return NTB_OK;
+    if (!layouts || (lenQ > 0 && (!q || !out || !lse || !dout || !dq)) || (lenK > 0 && (!k || !v || !dk || !dv)))
+        return NTB_ERR_ARG;
+    if (workBytes < ntb_cross_attention_grad_work(batch, headsQ, lenQ) || (lenQ > 0 && (!work || ((uintptr_t)work & 15))))
+        return NTB_ERR_ARG;
+    if (lenQ > 0 && (!LayoutOk(q, layouts[0], dim, lenQ, headsQ, batch, true) || !LayoutOk(out, layouts[3], dim, lenQ, headsQ, batch, true) ||
+                     !LayoutOk(dout, layouts[4], dim, lenQ, headsQ, batch, true) || !LayoutOk(dq, layouts[5], dim, lenQ, headsQ, batch, false)))
+        return NTB_ERR_ARG;
+    if (lenK > 0 && (!LayoutOk(k, layouts[1], dim, lenK, headsKV, batch, true) || !LayoutOk(v, layouts[2], dim, lenK, headsKV, batch, true) ||
+                     !LayoutOk(dk, layouts[6], dim, lenK, headsKV, batch, false) || !LayoutOk(dv, layouts[7], dim, lenK, headsKV, batch, false)))
+        return NTB_ERR_ARG;
+    call.q = q; call.k = k; call.v = v; call.out = out; call.dout = dout; call.lse = lse;
+    call.dq = dq; call.dk = dk; call.dv = dv;
+    call.work = (float *)work;
+    call.l = layouts;
+    call.scale = scale;
+    XattnDevice dev(devID);
+    if (!dev.ok)
+        return NTB_ERR_CUDA;
+    DeviceCtx * ctx = CtxFor(devID);
+    if (!ctx)
+        return NTB_ERR_CUDA;
+    rc = dim <= 64 ? LaunchGrad<64>(*ctx, call, (cudaStream_t)stream) : LaunchGrad<128>(*ctx, call, (cudaStream_t)stream);
+    if (rc == NTB_ERR_CUDA)
+        cudaGetLastError();
+    return rc;
+}

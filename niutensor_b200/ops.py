@@ -288,6 +288,29 @@ def CrossAttention(q, k, v, query_lens=None, key_lens=None, scale=None, out=None
     return (out, lse) if with_lse else out
 
 
+def GradCrossAttention(q, k, v, out, lse, dedo, query_lens=None, key_lens=None, scale=None):
+    """(dedq, dedk, dedv) of CrossAttention from its result and statistics and the gradient dedo of its
+    result; all but lse half tensors of any strides as there. Query heads that share a key head are
+    summed; a broadcast k or v gets the gradient of every copy. Lengths and scale as in the forward
+    call; rows past them get zeros."""
+    scale = _cross_attention_checks(q, k, v, query_lens, key_lens, scale, (out, dedo))
+    _check(out.shape == q.shape and dedo.shape == q.shape, "Incorrect tensor sizes!")
+    batch, heads, len_q, d = q.shape
+    _check(lse.is_cuda and lse.device == q.device and lse.dtype == torch.float32 and lse.is_contiguous() and
+           tuple(lse.shape) == (batch, heads, len_q), "lse must be the packed fp32 CUDA tensor of the forward call")
+    dedq, dedk, dedv = _heads_like(q), _heads_like(k), _heads_like(v)
+    layouts = (capi.HeadsLayout * 8)(*[_heads_layout(t) for t in (q, k, v, out, dedo, dedq, dedk, dedv)])
+    lib = capi.lib()
+    need = lib.ntb_cross_attention_grad_work(batch, heads, len_q)
+    work = torch.empty(need, dtype=torch.uint8, device=q.device)
+    rc = lib.ntb_cross_attention_grad(q.device.index, _stream(q), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(),
+                                      dedo.data_ptr(), dedq.data_ptr(), dedk.data_ptr(), dedv.data_ptr(), work.data_ptr(), need,
+                                      X_FLOAT16, batch, heads, k.shape[1], len_q, k.shape[2], d, layouts,
+                                      _ptr(query_lens), _ptr(key_lens), scale)
+    _raise_rc(rc, "GradCrossAttention")
+    return dedq, dedk, dedv
+
+
 def RowStats(x):
     """(row maximum, sum of exp(x - maximum)) over the last dimension of a 2-D tensor, fp32."""
     _check(x.is_cuda and x.dim() == 2 and x.stride(1) == 1, "a CUDA matrix with unit column stride is required")

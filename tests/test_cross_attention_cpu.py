@@ -59,3 +59,32 @@ def test_operator_refuses_host_tensors():
 
 def test_layout_structure_matches_the_header():
     assert ctypes.sizeof(capi.HeadsLayout) == 24
+
+
+def grad(q=P, k=P, v=P, out=P, lse=P, dout=P, dq=P, dk=P, dv=P, work=P, bytes_=None, dtype=capi.X_FLOAT16, batch=2, heads=4, kv=4, n=32, m=32,
+         d=64, lay=None, scale=0.125):
+    lib = capi.lib()
+    need = lib.ntb_cross_attention_grad_work(2, 4, 32) if bytes_ is None else bytes_
+    return lib.ntb_cross_attention_grad(0, None, q, k, v, out, lse, dout, dq, dk, dv, work, need, dtype, batch, heads, kv, n, m, d,
+                                        lay if lay is not None else layouts(8), None, None, scale)
+
+
+@pytest.mark.parametrize("change,code", [
+    (dict(q=None), capi.ERR_ARG), (dict(lse=None), capi.ERR_ARG), (dict(dout=None), capi.ERR_ARG), (dict(dq=None), capi.ERR_ARG),
+    (dict(dk=None), capi.ERR_ARG), (dict(dv=None), capi.ERR_ARG), (dict(work=None), capi.ERR_ARG), (dict(work=P + 4), capi.ERR_ARG),
+    (dict(bytes_=64), capi.ERR_ARG), (dict(dtype=capi.X_FLOAT), capi.ERR_DTYPE), (dict(kv=3), capi.ERR_SHAPE),
+    (dict(d=12), capi.ERR_LIMIT), (dict(scale=0.0), capi.ERR_ARG), (dict(m=-1), capi.ERR_ARG),
+    (dict(lay=layouts(8, t4=dict(row=66))), capi.ERR_ARG), (dict(lay=layouts(8, t6=dict(head=0))), capi.ERR_ARG),
+    (dict(lay=layouts(8, t7=dict(batch=0))), capi.ERR_ARG), (dict(lay=layouts(8, t5=dict(row=56))), capi.ERR_ARG),
+    (dict(dq=P + 2), capi.ERR_ARG),
+])
+def test_gradient_refuses(change, code):
+    assert grad(**change) == code
+
+
+def test_gradient_work_bytes():
+    lib = capi.lib()
+    assert lib.ntb_cross_attention_grad_work(2, 4, 1) == 2 * 4 * 1024
+    assert lib.ntb_cross_attention_grad_work(1, 1, 129) == 2048
+    assert lib.ntb_cross_attention_grad_work(3, 5, 0) == 0 and lib.ntb_cross_attention_grad_work(-1, 5, 9) == 0
+    assert lib.ntb_cross_attention_grad_work(1 << 12, 128, 1 << 16) == (1 << 19) * 512 * 1024        # beyond 32 bits
