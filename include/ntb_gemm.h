@@ -210,6 +210,53 @@ int ntb_logsoftmax_apply(int devID, void * stream, const void * x, void * y, int
                          const float * rowMax, const float * rowSumExp);
 
 /*
+ * Rows of an embedding matrix, scaled, with the rows of the positions added
+ * (source/sample/transformer/submodel/Embedding.cpp: a gather, a multiplication by sqrt(d), a sum):
+ *
+ *        out[t] = scale * w[ids[t]] + pos[t % posRows],     t < tokens
+ *
+ * ids: X_INT. w: vocab x dim with row pitch ldw; out: tokens x dim with row pitch ldo; pos: posRows x dim
+ * packed, or NULL; all of dtype X_FLOAT16 or X_FLOAT. Formed in fp32, rounded once. An id outside
+ * [0, vocab) stands for no word (padding): its row of w counts as zeros. Any alignment of the
+ * elements; rows of 16-byte bases, pitches and lengths take the wide accesses.
+ *
+ * ntb_embedding_grad is its gradient in w:
+ *
+ *        dw[v] = beta * dw[v] + scale * sum over t with ids[t] = v, in ascending t, of dout[t]
+ *
+ * beta 1: accumulated into dw as every gradient of the reference's backward pass (rows of words that
+ * do not occur are not touched). beta 0: dw is written whole and never read. Other values: NTB_ERR_ARG.
+ * (dtypeOut of dout, dtypeW of dw): (X_FLOAT16, X_FLOAT16), (X_FLOAT16, X_FLOAT), (X_FLOAT, X_FLOAT). Sums are
+ * fp32 in an order fixed by `tokens` and ids: no atomics, results do not depend on timing. Ids outside
+ * [0, vocab) add nothing. work: device scratch of ntb_embedding_grad_work(tokens, dim) bytes on a 16-byte
+ * boundary, the caller's; its content need not survive the call. dw, dout and work must not overlap.
+ */
+int ntb_embedding(int devID, void * stream, const int * ids, const void * w, const void * pos, void * out,
+                  int dtype, int tokens, int vocab, int dim, long long ldw, long long ldo, int posRows, float scale);
+long long ntb_embedding_grad_work(int tokens, int dim);
+int ntb_embedding_grad(int devID, void * stream, const int * ids, const void * dout, void * dw, int dtypeOut, int dtypeW,
+                       int tokens, int vocab, int dim, long long ldo, long long ldw, float scale, float beta,
+                       void * work, long long workBytes);
+
+/*
+ * The 2-norm of all gradients of a model together, and their clipping to maxNorm:
+ *
+ *        *norm = sqrt(sum over all tensors and elements of g^2),     out = g * min(1, maxNorm / *norm)
+ *
+ * grads, out, dtypes, counts: HOST arrays of `count` entries (device pointers, X_FLOAT16 or X_FLOAT, element
+ * counts); out[i] may be grads[i] (in place); different entries must not overlap. norm: one float on the
+ * device. A norm that is not finite leaves the gradients' values as they are (the caller reads *norm and skips
+ * the step); maxNorm infinite only takes the norm. maxNorm must not be negative or NaN. The sum is
+ * fp64 (fp32 within eight exact products of halves); its order is fixed by the sizes. work: device scratch
+ * of ntb_clip_grad_norm_work(count) bytes on an 8-byte boundary, the caller's. The arrays are read before
+ * the call returns; the addresses are part of the launch, so a captured call replays on the same tensors.
+ */
+long long ntb_clip_grad_norm_work(int count);
+int ntb_clip_grad_norm(int devID, void * stream, int count, const void * const * grads, void * const * out,
+                       const int * dtypes, const long long * counts, float maxNorm, float * norm,
+                       void * work, long long workBytes);
+
+/*
  * Both gradient products of c = alpha * op(a) * op(b) in one launch:
  *
  *        deda += alpha * (...),   dedb += alpha * (...)        (beta = 1, accumulating)

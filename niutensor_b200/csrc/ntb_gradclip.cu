@@ -1,0 +1,332 @@
+/*
+ * The norm of a whole list of gradients and their clipping to it:
+ *
+ *     norm = sqrt(sum over all elements of g^2),   out = g * min(1, maxNorm / norm)
+ *
+ * Two launches whatever the number of tensors (up to 1000; longer lists go in groups): the tensors' addresses
+ * travel in the launch parameters, so there is no table to copy to the device and the call can be captured.
+ * The list is cut into chunks of equal size that persistent CTAs walk.
+ *
+ * NormKernel: squares summed in fp64 for floats (a norm that fits a float may have squares that do not), in
+ * fp32 over eight exact products and then fp64 for halves; one partial sum a CTA. ClipKernel: every CTA adds
+ * up the partial sums in the same order (so all have the same norm; no atomics, no third launch), then scales
+ * its chunks, walking the list backwards: what the first pass read last is still in L2. Both are bound by
+ * their reads and writes: the list has to be read to the end before the first element can be written.
+ */
+#include "ntb_xattn.cuh"
+
+namespace ntb {
+
+namespace {
+
+constexpr int CL_THREADS = 512;
+constexpr int CL_CHUNK = 32768;           /* bytes */
+constexpr int CL_FEW = 64, CL_MANY = 1000;     /* tensors a launch; kernel parameters end at 32764 bytes */
+
+struct ClipTensor {
+    const void * in;
+    void * out;
+    long long n;
+    int firstChunk;
+    int half;
+};
+
+template <int MAX> struct ClipList {
+    ClipTensor t[MAX];
+    int count;
+    int chunks;
+    double * partial;
+    int partial0;             /* this launch's first partial sum */
+    int partials;             /* all of them */
+    float maxNorm;
+    float * norm;             /* written by the first CTA of the first group, or NULL */
+};
+static_assert(sizeof(ClipList<CL_MANY>) <= 32700, "kernel parameters");
+
+/* the chunk's tensor: the last one that starts at or before it and is not empty */
+template <int MAX>
+__device__ __forceinline__ int TensorOf(const ClipList<MAX> & l, int chunk)
+{
+    int lo = 0, hi = l.count - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) / 2;
+        if (l.t[mid].firstChunk <= chunk)
+            lo = mid;
+        else
+            hi = mid - 1;
+    }
+    return lo;
+}
+
+__device__ __forceinline__ double Squares(const uint4 & u, bool half)
+{
+    const uint32_t x[4] = { u.x, u.y, u.z, u.w };
+    if (half) {
+        float s = 0.f;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const float2 f = __half22float2(*(const __half2 *)&x[i]);
+            s = fmaf(f.x, f.x, s);
+            s = fmaf(f.y, f.y, s);
+        }
+        return (double)s;
+    }
+    double s = 0.0;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const double d = (double)__uint_as_float(x[i]);
+        s = fma(d, d, s);
+    }
+    return s;
+}
+
+__device__ __forceinline__ float Element(const void * p, long long i, bool half)
+{
+    return half ? __half2float(((const __half *)p)[i]) : ((const float *)p)[i];
+}
+
+__device__ __forceinline__ void SetElement(void * p, long long i, bool half, float v)
+{
+    if (half)
+        ((__half *)p)[i] = __float2half_rn(v);
+    else
+        ((float *)p)[i] = v;
+}
+
+/* the elements of a chunk: [lo, hi) of its tensor, of which [lo + head, lo + head + 16-byte packs) are aligned */
+struct ChunkRange {
+    long long lo, hi, body;
+    int packs, perPack;
+};
+__device__ __forceinline__ ChunkRange RangeOf(const ClipTensor & t, int chunk)
+{
+    const int size = t.half ? 2 : 4, per = 16 / size;
+    const long long each = CL_CHUNK / size;
+    ChunkRange r;
+    r.lo = (long long)(chunk - t.firstChunk) * each;
+    r.hi = r.lo + each < t.n ? r.lo + each : t.n;
+    const long long head = (long long)((16 - (((uintptr_t)t.in + r.lo * size) & 15)) & 15) / size;
+    r.body = r.lo + head < r.hi ? r.lo + head : r.hi;
+    r.packs = (int)((r.hi - r.body) / per);
+    r.perPack = per;
+    return r;
+}
+
+template <int MAX>
+__global__ void __launch_bounds__(CL_THREADS) NormKernel(const __grid_constant__ ClipList<MAX> l)
+{
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    double sum = 0.0;
+    for (int chunk = blockIdx.x; chunk < l.chunks; chunk += gridDim.x) {
+        const ClipTensor & t = l.t[TensorOf(l, chunk)];
+        const ChunkRange r = RangeOf(t, chunk);
+        const bool half = t.half != 0;
+        const uint4 * v = (const uint4 *)((const char *)t.in + r.body * (half ? 2 : 4));
+        constexpr int U = CL_CHUNK / 16 / CL_THREADS;
+        uint4 x[U];
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const int i = u * CL_THREADS + threadIdx.x;
+            x[u] = i < r.packs ? v[i] : make_uint4(0u, 0u, 0u, 0u);
+        }
+#pragma unroll
+        for (int u = 0; u < U; u++)
+            sum += Squares(x[u], half);
+        /* what lies before and behind the aligned packs: fewer than eight elements each */
+        const long long tail = r.body + (long long)r.packs * r.perPack;
+        if (threadIdx.x < r.body - r.lo) {
+            const double d = Element(t.in, r.lo + threadIdx.x, half);
+            sum = fma(d, d, sum);
+        }
+        if (threadIdx.x < r.hi - tail) {
+            const double d = Element(t.in, tail + threadIdx.x, half);
+            sum = fma(d, d, sum);
+        }
+    }
+    __shared__ double sums[CL_THREADS / 32];
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1)
+        sum += __shfl_down_sync(0xffffffffu, sum, off);
+    if ((threadIdx.x & 31) == 0)
+        sums[threadIdx.x >> 5] = sum;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int w = 1; w < CL_THREADS / 32; w++)
+            sum += sums[w];
+        l.partial[l.partial0 + blockIdx.x] = sum;
+    }
+}
+
+template <int MAX>
+__global__ void __launch_bounds__(CL_THREADS) ClipKernel(const __grid_constant__ ClipList<MAX> l)
+{
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    __shared__ double sums[CL_THREADS / 32];
+    double sum = 0.0;
+    for (int i = threadIdx.x; i < l.partials; i += CL_THREADS)
+        sum += l.partial[i];
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1)
+        sum += __shfl_down_sync(0xffffffffu, sum, off);
+    if ((threadIdx.x & 31) == 0)
+        sums[threadIdx.x >> 5] = sum;
+    __syncthreads();
+    double total = 0.0;
+    for (int w = 0; w < CL_THREADS / 32; w++)
+        total += sums[w];
+    const double norm = sqrt(total);
+    if (blockIdx.x == 0 && threadIdx.x == 0 && l.norm != nullptr)
+        *l.norm = (float)norm;
+    const bool clip = norm > (double)l.maxNorm && !isinf(norm);
+    const float f = clip ? (float)((double)l.maxNorm / norm) : 1.f;
+    for (int k = blockIdx.x; k < l.chunks; k += gridDim.x) {
+        const int chunk = l.chunks - 1 - k;
+        const ClipTensor & t = l.t[TensorOf(l, chunk)];
+        if (!clip && t.in == t.out)
+            continue;                             /* nothing changes */
+        const ChunkRange r = RangeOf(t, chunk);
+        const bool half = t.half != 0;
+        const int size = half ? 2 : 4;
+        if ((((uintptr_t)t.in ^ (uintptr_t)t.out) & 15) != 0) {
+            for (long long i = r.lo + threadIdx.x; i < r.hi; i += CL_THREADS)
+                SetElement(t.out, i, half, Element(t.in, i, half) * f);
+            continue;
+        }
+        const uint4 * v = (const uint4 *)((const char *)t.in + r.body * size);
+        uint4 * o = (uint4 *)((char *)t.out + r.body * size);
+        constexpr int U = CL_CHUNK / 16 / CL_THREADS;
+        uint4 x[U];
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const int i = u * CL_THREADS + threadIdx.x;
+            if (i < r.packs)
+                x[u] = __ldcs(v + i);
+        }
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const int i = u * CL_THREADS + threadIdx.x;
+            if (i < r.packs) {
+                uint32_t w[4] = { x[u].x, x[u].y, x[u].z, x[u].w };
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    if (half) {
+                        const float2 g = __half22float2(*(const __half2 *)&w[e]);
+                        w[e] = PackHalf2(g.x * f, g.y * f);
+                    }
+                    else
+                        w[e] = __float_as_uint(__uint_as_float(w[e]) * f);
+                }
+                __stcs(o + i, make_uint4(w[0], w[1], w[2], w[3]));
+            }
+        }
+        const long long tail = r.body + (long long)r.packs * r.perPack;
+        if (threadIdx.x < r.body - r.lo)
+            SetElement(t.out, r.lo + threadIdx.x, half, Element(t.in, r.lo + threadIdx.x, half) * f);
+        if (threadIdx.x < r.hi - tail)
+            SetElement(t.out, tail + threadIdx.x, half, Element(t.in, tail + threadIdx.x, half) * f);
+    }
+}
+
+int Ctas(const DeviceCtx & ctx, int chunks)
+{
+    const int most = ctx.smCount * 4;
+    return chunks < 1 ? 1 : chunks < most ? chunks : most;
+}
+
+template <int MAX>
+int ClipGroups(const DeviceCtx & ctx, int count, const void * const * grads, void * const * out, const int * dtypes, const long long * counts,
+               float maxNorm, float * norm, double * partial, cudaStream_t stream)
+{
+    for (int pass = 0; pass < 2; pass++) {
+        int partials = 0;
+        if (pass == 1)                            /* as many as the first pass wrote */
+            for (int g0 = 0; g0 < count || g0 == 0; g0 += MAX) {
+                long long chunks = 0;
+                for (int i = g0; i < count && i < g0 + MAX; i++)
+                    chunks += (counts[i] * (dtypes[i] == NTB_X_FLOAT16 ? 2 : 4) + CL_CHUNK - 1) / CL_CHUNK;
+                partials += Ctas(ctx, (int)chunks);
+            }
+        int at = 0;
+        for (int g0 = 0; g0 < count || g0 == 0; g0 += MAX) {
+            ClipList<MAX> l;
+            l.count = 0;
+            long long chunks = 0;
+            for (int i = g0; i < count && i < g0 + MAX; i++) {
+                if (counts[i] == 0)
+                    continue;
+                ClipTensor & t = l.t[l.count++];
+                t.in = grads[i];
+                t.out = out[i];
+                t.n = counts[i];
+                t.half = dtypes[i] == NTB_X_FLOAT16;
+                t.firstChunk = (int)chunks;
+                chunks += (counts[i] * (t.half ? 2 : 4) + CL_CHUNK - 1) / CL_CHUNK;
+            }
+            l.chunks = (int)chunks;
+            l.partial = partial;
+            l.partial0 = at;
+            l.partials = partials;
+            l.maxNorm = maxNorm;
+            l.norm = g0 == 0 ? norm : nullptr;
+            const int grid = Ctas(ctx, l.chunks);
+            at += grid;
+            const cudaError_t err = pass == 0 ? LaunchPdl(NormKernel<MAX>, grid, CL_THREADS, 0, stream, l)
+                                              : LaunchPdl(ClipKernel<MAX>, grid, CL_THREADS, 0, stream, l);
+            CountLaunch();
+            if (err != cudaSuccess || cudaGetLastError() != cudaSuccess) {
+                cudaGetLastError();
+                return NTB_ERR_CUDA;
+            }
+        }
+    }
+    return NTB_OK;
+}
+
+}
+
+}
+
+using namespace ntb;
+
+extern "C" long long ntb_clip_grad_norm_work(int count)
+{
+    /* partial sums: four CTAs an SM (of at most 256) a group of tensors */
+    const long long groups = count <= CL_MANY ? 1 : (count + CL_MANY - 1) / CL_MANY;
+    return groups * 256 * 4 * (long long)sizeof(double);
+}
+
+extern "C" int ntb_clip_grad_norm(int devID, void * stream, int count, const void * const * grads, void * const * out,
+                                  const int * dtypes, const long long * counts, float maxNorm, float * norm,
+                                  void * work, long long workBytes)
+{
+    if (count < 0 || !(maxNorm >= 0.f) || !norm || !work || ((uintptr_t)work & 7) || workBytes < ntb_clip_grad_norm_work(count))
+        return NTB_ERR_ARG;
+    if (count > 0 && (!grads || !out || !dtypes || !counts))
+        return NTB_ERR_ARG;
+    long long chunks = 0;
+    for (int i = 0; i < count; i++) {
+        if (dtypes[i] != NTB_X_FLOAT16 && dtypes[i] != NTB_X_FLOAT)
+            return NTB_ERR_DTYPE;
+        const int size = dtypes[i] == NTB_X_FLOAT16 ? 2 : 4;
+        if (counts[i] < 0 || (counts[i] > 0 && (!grads[i] || !out[i] || (((uintptr_t)grads[i] | (uintptr_t)out[i]) & (size - 1)))))
+            return NTB_ERR_ARG;
+        if (counts[i] > (1LL << 44))
+            return NTB_ERR_LIMIT;
+        chunks += (counts[i] * size + CL_CHUNK - 1) / CL_CHUNK;
+        if (chunks > 0x7fff0000LL)
+            return NTB_ERR_LIMIT;
+    }
+    XattnDevice dev(devID);
+    if (!dev.ok)
+        return NTB_ERR_CUDA;
+    DeviceCtx * ctx = CtxFor(devID);
+    if (!ctx)
+        return NTB_ERR_CUDA;
+    if (ctx->smCount > 256)
+        return NTB_ERR_LIMIT;
+    return count <= CL_FEW
+        ? ClipGroups<CL_FEW>(*ctx, count, grads, out, dtypes, counts, maxNorm, norm, (double *)work, (cudaStream_t)stream)
+        : ClipGroups<CL_MANY>(*ctx, count, grads, out, dtypes, counts, maxNorm, norm, (double *)work, (cudaStream_t)stream);
+}

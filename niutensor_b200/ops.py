@@ -311,6 +311,83 @@ def GradCrossAttention(q, k, v, out, lse, dedo, query_lens=None, key_lens=None, 
     return dedq, dedk, dedv
 
 
+def Embedding(w, ids, scale=1.0, pos=None):
+    """scale * w[ids], plus the rows of pos: the word and position embeddings of
+    source/sample/transformer/submodel/Embedding.cpp in one pass. w [vocab, d] fp16 or fp32 (rows may be
+    pitched), ids a packed int32 tensor of any shape, pos None or packed [len, d] of w's type, whose
+    row t % len goes to token t of the flattened ids (whole sentences of len). The result has shape
+    ids.shape + [d]. An id outside [0, vocab) is padding: no word, zeros."""
+    _check(w.is_cuda and ids.is_cuda, "this library has no CPU path: tensors must live on a CUDA device")
+    _check(w.device == ids.device, "The code must be run on the same GPU!")
+    dtype = _dtype_code(w)
+    _check(w.dim() == 2 and (w.stride(1) == 1 or w.shape[1] <= 1) and (w.shape[0] <= 1 or w.stride(0) >= w.shape[1]),
+           "a CUDA matrix with unit column stride is required")
+    _check(ids.dtype == torch.int32 and ids.is_contiguous(), "ids must be a packed int32 CUDA tensor")
+    vocab, d = w.shape
+    tokens, rows = ids.numel(), 0
+    if pos is not None:
+        _check(pos.is_cuda and pos.device == w.device and pos.dtype == w.dtype and pos.is_contiguous() and pos.dim() == 2 and pos.shape[1] == d,
+               "positions must be a packed matrix of the words' type and width")
+        rows = pos.shape[0]
+        _check(tokens == 0 or (rows > 0 and tokens % rows == 0), "Incorrect tensor sizes!")
+    out = torch.empty(tuple(ids.shape) + (d,), dtype=w.dtype, device=w.device)
+    rc = capi.lib().ntb_embedding(w.device.index, _stream(w), ids.data_ptr(), w.data_ptr(), _ptr(pos) if rows else None, out.data_ptr(), dtype,
+                                  tokens, vocab, d, w.stride(0) if vocab > 1 else d, d, rows, scale)
+    _raise_rc(rc, "Embedding")
+    return out
+
+
+def GradEmbedding(ids, dedc, dedw, scale=1.0, beta=1.0):
+    """Backward of Embedding in w: dedw = beta * dedw + scale * the sum of dedc's rows of every word, in the
+    order of the tokens; beta 1 (accumulating, as GradMatrixMul) or 0 (dedw is written whole). dedc has shape
+    ids.shape + [d], packed; dedw [vocab, d], rows may be pitched; both fp16 or both fp32, or fp16 into
+    fp32. Ids outside [0, vocab) add nothing."""
+    _check(dedc.is_cuda and ids.is_cuda and dedw.is_cuda, "this library has no CPU path: tensors must live on a CUDA device")
+    _check(dedc.device == ids.device == dedw.device, "The code must be run on the same GPU!")
+    _check(dedw.dim() == 2 and (dedw.stride(1) == 1 or dedw.shape[1] <= 1) and (dedw.shape[0] <= 1 or dedw.stride(0) >= dedw.shape[1]),
+           "a CUDA matrix with unit column stride is required")
+    _check(ids.dtype == torch.int32 and ids.is_contiguous(), "ids must be a packed int32 CUDA tensor")
+    vocab, d = dedw.shape
+    _check(dedc.is_contiguous() and tuple(dedc.shape) == tuple(ids.shape) + (d,), "Incorrect tensor sizes!")
+    _check(beta == 0.0 or beta == 1.0, "beta must be 0 or 1")
+    tokens = ids.numel()
+    lib = capi.lib()
+    need = lib.ntb_embedding_grad_work(tokens, d)
+    work = torch.empty(need, dtype=torch.uint8, device=dedw.device)
+    rc = lib.ntb_embedding_grad(dedw.device.index, _stream(dedw), ids.data_ptr(), dedc.data_ptr(), dedw.data_ptr(), _dtype_code(dedc),
+                                _dtype_code(dedw), tokens, vocab, d, d, dedw.stride(0) if vocab > 1 else d, scale, beta, work.data_ptr(), need)
+    _raise_rc(rc, "GradEmbedding")
+
+
+def ClipGradNorm(grads, max_norm, out=None):
+    """The 2-norm of a list of gradients together, as a float tensor on their device, and the gradients times
+    min(1, max_norm / norm): in place, or into the tensors of out. Packed fp16 and fp32 CUDA tensors of any
+    shapes on one device, each listed once. A norm that is not finite leaves the values as they are. Two launches,
+    no copy to the device, no synchronisation."""
+    _check(len(grads) > 0, "Empty input tensors!")
+    into = grads if out is None else out
+    _check(len(into) == len(grads), "Incorrect tensor sizes!")
+    device = grads[0].device
+    n = len(grads)
+    for g, o in zip(grads, into):
+        _check(g.is_cuda and o.is_cuda, "this library has no CPU path: tensors must live on a CUDA device")
+        _check(g.device == device and o.device == device, "The code must be run on the same GPU!")
+        _check(g.dtype == o.dtype and g.shape == o.shape, "Incorrect tensor sizes!")
+        _check(g.is_contiguous() and o.is_contiguous(), "tensors must be dense and packed")
+    _check(float(max_norm) >= 0.0, "the norm must not be negative")
+    where = [o.data_ptr() for o in into if o.numel()]
+    _check(len(set(where)) == len(where), "a tensor is listed twice")
+    norm = torch.empty((), dtype=torch.float32, device=device)
+    lib = capi.lib()
+    need = lib.ntb_clip_grad_norm_work(n)
+    work = torch.empty(need, dtype=torch.uint8, device=device)
+    rc = lib.ntb_clip_grad_norm(device.index, _stream(grads[0]), n, (ctypes.c_void_p * n)(*[g.data_ptr() for g in grads]),
+                                (ctypes.c_void_p * n)(*[o.data_ptr() for o in into]), (ctypes.c_int * n)(*[_dtype_code(g) for g in grads]),
+                                (ctypes.c_longlong * n)(*[g.numel() for g in grads]), max_norm, norm.data_ptr(), work.data_ptr(), need)
+    _raise_rc(rc, "ClipGradNorm")
+    return norm
+
+
 def RowStats(x):
     """(row maximum, sum of exp(x - maximum)) over the last dimension of a 2-D tensor, fp32."""
     _check(x.is_cuda and x.dim() == 2 and x.stride(1) == 1, "a CUDA matrix with unit column stride is required")
