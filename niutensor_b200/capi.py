@@ -38,16 +38,16 @@ PROTOTYPES = {
     "ntb_gemm_bias_act": (_i, [_i, _vp, _vp, _i, _vp, _i, _vp, _vp, _i, _i] + [_i] * 6 + [_ll] * 3 + [_f, _f, _i]),
     "ntb_attention": (_i, [_i, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _ll, _f]),
     "ntb_attention_dropout": (_i, [_i, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _ll, _f, _f]),
-    "ntb_cross_attention": (_i, [_i] + [_vp] * 6 + [_i] * 7 + [ctypes.POINTER(HeadsLayout), _vp, _vp, _f]),
+    "ntb_cross_attention": (_i, [_i] + [_vp] * 6 + [_i] * 7 + [_vp, _vp, _vp, _f]),
     "ntb_cross_attention_grad_work": (_ll, [_i] * 3),
-    "ntb_cross_attention_grad": (_i, [_i] + [_vp] * 11 + [_ll] + [_i] * 7 + [ctypes.POINTER(HeadsLayout), _vp, _vp, _f]),
+    "ntb_cross_attention_grad": (_i, [_i] + [_vp] * 11 + [_ll] + [_i] * 7 + [_vp, _vp, _vp, _f]),
     "ntb_row_stats": (_i, [_i, _vp, _vp, _i, _i, _i, _ll, _vp, _vp]),
     "ntb_logsoftmax_apply": (_i, [_i, _vp, _vp, _vp, _i, _i, _i, _ll, _ll, _vp, _vp]),
     "ntb_embedding": (_i, [_i] + [_vp] * 5 + [_i] * 4 + [_ll, _ll, _i, _f]),
     "ntb_embedding_grad_work": (_ll, [_i, _i]),
     "ntb_embedding_grad": (_i, [_i] + [_vp] * 4 + [_i] * 5 + [_ll, _ll, _f, _f, _vp, _ll]),
     "ntb_clip_grad_norm_work": (_ll, [_i]),
-    "ntb_clip_grad_norm": (_i, [_i, _vp, _i, ctypes.POINTER(_vp), ctypes.POINTER(_vp), ctypes.POINTER(_i), ctypes.POINTER(_ll), _f, _vp, _vp, _ll]),
+    "ntb_clip_grad_norm": (_i, [_i, _vp, _i, _vp, _vp, _vp, _vp, _f, _vp, _vp, _ll]),
     "ntb_gemm_grad": (_i, [_i, _vp, _vp, _i, _vp, _i, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _f]),
     "ntb_gemm_strided_batched": (_i, [_i, _vp, _vp, _i, _vp, _i, _vp, _i, _i] + [_i] * 6 + [_ll] * 6 + [_i, _f, _f]),
     "ntb_gemm_broadcast": (_i, [_i, _vp, _vp, _i, _vp, _i, _vp, _i, _i] + [_i] * 6 + [_i, _i, _f, _f]),

@@ -12,6 +12,7 @@ Names, argument meaning and shape rules follow the reference:
 Transposition flags are the reference's enum values: X_TRANS = 0, X_NOTRANS = 1.
 Where the reference prints an error and terminates, these raise NtError.
 """
+import array
 import ctypes
 
 import torch
@@ -39,6 +40,11 @@ def _dtype_code(t):
 
 def _stream(t):
     return torch.cuda.current_stream(t.device).cuda_stream
+
+
+#: the current stream of a device as an integer, without building a stream object (a call of a few microseconds
+#: would otherwise spend as long on that as on its kernel)
+_raw_stream = torch._C._cuda_getCurrentRawStream
 
 
 def _common_checks(a, b, c):
@@ -228,10 +234,19 @@ def ScaledDotProductAttention(q, k, v, mask=None, scale=None, keep=None, drop_pr
 def _heads_layout(t):
     """strides of a [batch, heads, len, dim] half tensor, as the kernels address it: dense rows, base and
     strides on 16 bytes (the stride of an extent of one may be anything)"""
-    _check(t.stride(3) == 1 or t.shape[3] <= 1, "rows of the last dimension must be dense")
-    _check(t.data_ptr() % 16 == 0 and all(t.shape[i] <= 1 or t.stride(i) % 8 == 0 for i in range(3)),
-           "base and strides must be multiples of 16 bytes")
-    return capi.HeadsLayout(t.stride(0), t.stride(1), t.stride(2))
+    s = t.stride()
+    if s[3] != 1 or (s[0] | s[1] | s[2]) & 7:
+        n = t.shape
+        _check(s[3] == 1 or n[3] <= 1, "rows of the last dimension must be dense")
+        _check(all(n[i] <= 1 or s[i] % 8 == 0 for i in range(3)), "base and strides must be multiples of 16 bytes")
+    return s[:3]
+
+
+def _aligned(*addresses):
+    """the addresses, which the kernels want on 16 bytes"""
+    for a in addresses:
+        _check(a & 15 == 0, "base and strides must be multiples of 16 bytes")
+    return addresses
 
 
 def _heads_like(t):
@@ -241,25 +256,33 @@ def _heads_like(t):
 
 
 def _cross_attention_checks(q, k, v, query_lens, key_lens, scale, others=()):
-    for t in (q, k, v) + tuple(others):
-        _check(t.is_cuda, "this library has no CPU path: tensors must live on a CUDA device")
-        _check(t.dtype == torch.float16, "Unsupported data type!")
-        _check(t.device == q.device, "The code must be run on the same GPU!")
-        _check(t.dim() == 4, "Input tensors must have a order = 4!")
-    _check(k.shape == v.shape and k.shape[0] == q.shape[0] and k.shape[3] == q.shape[3], "Unmatched tensors in multiplication!")
-    _check(q.shape[1] == 0 or (k.shape[1] > 0 and q.shape[1] % k.shape[1] == 0), "the key heads must divide the query heads")
-    _check(q.shape[3] % 8 == 0 and 8 <= q.shape[3] <= 128, "the head size must be a multiple of 8 up to 128")
+    """device index, shapes of q and k, scale"""
+    dev = q.get_device()
+    for t in (q, k, v) + others:
+        if t.dtype is not torch.float16 or t.get_device() != dev or dev < 0 or t.dim() != 4:
+            _check(t.is_cuda and q.is_cuda, "this library has no CPU path: tensors must live on a CUDA device")
+            _check(t.dtype == torch.float16, "Unsupported data type!")
+            _check(t.get_device() == dev, "The code must be run on the same GPU!")
+            _check(t.dim() == 4, "Input tensors must have a order = 4!")
+    qs, ks = q.shape, k.shape
+    d = qs[3]
+    _check(ks == v.shape and ks[0] == qs[0] and ks[3] == d, "Unmatched tensors in multiplication!")
+    _check(qs[1] == 0 or (ks[1] > 0 and qs[1] % ks[1] == 0), "the key heads must divide the query heads")
+    _check(d % 8 == 0 and 8 <= d <= 128, "the head size must be a multiple of 8 up to 128")
     for lens in (query_lens, key_lens):
         if lens is not None:
-            _check(lens.is_cuda and lens.device == q.device and lens.dtype == torch.int32 and lens.is_contiguous() and
-                   tuple(lens.shape) == (q.shape[0],), "lengths must be a packed int32 CUDA vector with one entry a sentence")
-    scale = 1.0 / (q.shape[3] ** 0.5) if scale is None else float(scale)
+            _check(lens.get_device() == dev and lens.dtype is torch.int32 and lens.is_contiguous() and lens.dim() == 1 and lens.numel() == qs[0],
+                   "lengths must be a packed int32 CUDA vector with one entry a sentence")
+    scale = 1.0 / (d ** 0.5) if scale is None else float(scale)
     _check(0.0 < scale < 3.0e38, "the scale must be positive and finite")
-    return scale
+    return dev, qs, ks, scale
 
 
 def _ptr(t):
     return None if t is None else t.data_ptr()
+
+
+_Layouts4, _Layouts8 = ctypes.c_longlong * 12, ctypes.c_longlong * 24
 
 
 def CrossAttention(q, k, v, query_lens=None, key_lens=None, scale=None, out=None, with_lse=False):
@@ -273,18 +296,20 @@ def CrossAttention(q, k, v, query_lens=None, key_lens=None, scale=None, out=None
     past them, and rows without a key, are zeros. scale defaults to 1 / sqrt(d).
     A decoding step is the same call with lenQ = 1, or with the hypotheses of a beam as lenQ rows of
     their sentence. with_lse: returns (out, lse), lse fp32 [batch, heads, lenQ] = log sum exp of the
-    scaled scores (-inf in empty rows), which GradCrossAttention needs."""
-    scale = _cross_attention_checks(q, k, v, query_lens, key_lens, scale)
+    scaled scores (-inf in empty rows), which GradCrossAttention needs. out: a tensor of q's shape to write,
+    which must not overlap the inputs."""
+    dev, qs, ks, scale = _cross_attention_checks(q, k, v, query_lens, key_lens, scale)
     if out is None:
         out = _heads_like(q)
-    _check(out.is_cuda and out.device == q.device and out.dtype == q.dtype and out.shape == q.shape, "Incorrect tensor sizes!")
-    batch, heads, len_q, d = q.shape
-    layouts = (capi.HeadsLayout * 4)(*[_heads_layout(t) for t in (q, k, v, out)])
-    lse = torch.empty(batch, heads, len_q, dtype=torch.float32, device=q.device) if with_lse else None
-    rc = capi.lib().ntb_cross_attention(q.device.index, _stream(q), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _ptr(lse),
-                                        X_FLOAT16, batch, heads, k.shape[1], len_q, k.shape[2], d, layouts,
-                                        _ptr(query_lens), _ptr(key_lens), scale)
-    _raise_rc(rc, "CrossAttention")
+    else:
+        _check(out.get_device() == dev and out.dtype is torch.float16 and out.shape == qs, "Incorrect tensor sizes!")
+    layouts = _Layouts4(*_heads_layout(q), *_heads_layout(k), *_heads_layout(v), *_heads_layout(out))
+    batch, heads, len_q, d = qs
+    lse = torch.empty(qs[:3], dtype=torch.float32, device=q.device) if with_lse else None
+    rc = capi.lib().ntb_cross_attention(dev, _raw_stream(dev), *_aligned(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr()), _ptr(lse),
+                                        X_FLOAT16, batch, heads, ks[1], len_q, ks[2], d, layouts, _ptr(query_lens), _ptr(key_lens), scale)
+    if rc:
+        _raise_rc(rc, "CrossAttention")
     return (out, lse) if with_lse else out
 
 
@@ -293,21 +318,23 @@ def GradCrossAttention(q, k, v, out, lse, dedo, query_lens=None, key_lens=None, 
     result; all but lse half tensors of any strides as there. Query heads that share a key head are
     summed; a broadcast k or v gets the gradient of every copy. Lengths and scale as in the forward
     call; rows past them get zeros."""
-    scale = _cross_attention_checks(q, k, v, query_lens, key_lens, scale, (out, dedo))
-    _check(out.shape == q.shape and dedo.shape == q.shape, "Incorrect tensor sizes!")
-    batch, heads, len_q, d = q.shape
-    _check(lse.is_cuda and lse.device == q.device and lse.dtype == torch.float32 and lse.is_contiguous() and
-           tuple(lse.shape) == (batch, heads, len_q), "lse must be the packed fp32 CUDA tensor of the forward call")
+    dev, qs, ks, scale = _cross_attention_checks(q, k, v, query_lens, key_lens, scale, (out, dedo))
+    _check(out.shape == qs and dedo.shape == qs, "Incorrect tensor sizes!")
+    batch, heads, len_q, d = qs
+    _check(lse.get_device() == dev and lse.dtype is torch.float32 and lse.is_contiguous() and lse.shape == qs[:3],
+           "lse must be the packed fp32 CUDA tensor of the forward call")
     dedq, dedk, dedv = _heads_like(q), _heads_like(k), _heads_like(v)
-    layouts = (capi.HeadsLayout * 8)(*[_heads_layout(t) for t in (q, k, v, out, dedo, dedq, dedk, dedv)])
+    layouts = _Layouts8(*_heads_layout(q), *_heads_layout(k), *_heads_layout(v), *_heads_layout(out), *_heads_layout(dedo),
+                        *_heads_layout(dedq), *_heads_layout(dedk), *_heads_layout(dedv))
     lib = capi.lib()
     need = lib.ntb_cross_attention_grad_work(batch, heads, len_q)
     work = torch.empty(need, dtype=torch.uint8, device=q.device)
-    rc = lib.ntb_cross_attention_grad(q.device.index, _stream(q), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(),
-                                      dedo.data_ptr(), dedq.data_ptr(), dedk.data_ptr(), dedv.data_ptr(), work.data_ptr(), need,
-                                      X_FLOAT16, batch, heads, k.shape[1], len_q, k.shape[2], d, layouts,
+    pq, pk, pv, po, pdo = _aligned(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), dedo.data_ptr())
+    rc = lib.ntb_cross_attention_grad(dev, _raw_stream(dev), pq, pk, pv, po, lse.data_ptr(), pdo, dedq.data_ptr(), dedk.data_ptr(), dedv.data_ptr(),
+                                      work.data_ptr(), need, X_FLOAT16, batch, heads, ks[1], len_q, ks[2], d, layouts,
                                       _ptr(query_lens), _ptr(key_lens), scale)
-    _raise_rc(rc, "GradCrossAttention")
+    if rc:
+        _raise_rc(rc, "GradCrossAttention")
     return dedq, dedk, dedv
 
 
@@ -317,23 +344,25 @@ def Embedding(w, ids, scale=1.0, pos=None):
     pitched), ids a packed int32 tensor of any shape, pos None or packed [len, d] of w's type, whose
     row t % len goes to token t of the flattened ids (whole sentences of len). The result has shape
     ids.shape + [d]. An id outside [0, vocab) is padding: no word, zeros."""
-    _check(w.is_cuda and ids.is_cuda, "this library has no CPU path: tensors must live on a CUDA device")
-    _check(w.device == ids.device, "The code must be run on the same GPU!")
+    dev = w.get_device()
+    _check(dev >= 0 and ids.is_cuda, "this library has no CPU path: tensors must live on a CUDA device")
+    _check(ids.get_device() == dev, "The code must be run on the same GPU!")
     dtype = _dtype_code(w)
-    _check(w.dim() == 2 and (w.stride(1) == 1 or w.shape[1] <= 1) and (w.shape[0] <= 1 or w.stride(0) >= w.shape[1]),
-           "a CUDA matrix with unit column stride is required")
-    _check(ids.dtype == torch.int32 and ids.is_contiguous(), "ids must be a packed int32 CUDA tensor")
-    vocab, d = w.shape
+    _check(w.dim() == 2, "a CUDA matrix with unit column stride is required")
+    (vocab, d), (pitch, unit) = w.shape, w.stride()
+    _check((unit == 1 or d <= 1) and (vocab <= 1 or pitch >= d), "a CUDA matrix with unit column stride is required")
+    _check(ids.dtype is torch.int32 and ids.is_contiguous(), "ids must be a packed int32 CUDA tensor")
     tokens, rows = ids.numel(), 0
     if pos is not None:
-        _check(pos.is_cuda and pos.device == w.device and pos.dtype == w.dtype and pos.is_contiguous() and pos.dim() == 2 and pos.shape[1] == d,
+        _check(pos.get_device() == dev and pos.dtype is w.dtype and pos.is_contiguous() and pos.dim() == 2 and pos.shape[1] == d,
                "positions must be a packed matrix of the words' type and width")
         rows = pos.shape[0]
         _check(tokens == 0 or (rows > 0 and tokens % rows == 0), "Incorrect tensor sizes!")
-    out = torch.empty(tuple(ids.shape) + (d,), dtype=w.dtype, device=w.device)
-    rc = capi.lib().ntb_embedding(w.device.index, _stream(w), ids.data_ptr(), w.data_ptr(), _ptr(pos) if rows else None, out.data_ptr(), dtype,
-                                  tokens, vocab, d, w.stride(0) if vocab > 1 else d, d, rows, scale)
-    _raise_rc(rc, "Embedding")
+    out = torch.empty(ids.shape + (d,), dtype=w.dtype, device=w.device)
+    rc = capi.lib().ntb_embedding(dev, _raw_stream(dev), ids.data_ptr(), w.data_ptr(), _ptr(pos) if rows else None, out.data_ptr(), dtype,
+                                  tokens, vocab, d, pitch if vocab > 1 else d, d, rows, scale)
+    if rc:
+        _raise_rc(rc, "Embedding")
     return out
 
 
@@ -342,21 +371,26 @@ def GradEmbedding(ids, dedc, dedw, scale=1.0, beta=1.0):
     order of the tokens; beta 1 (accumulating, as GradMatrixMul) or 0 (dedw is written whole). dedc has shape
     ids.shape + [d], packed; dedw [vocab, d], rows may be pitched; both fp16 or both fp32, or fp16 into
     fp32. Ids outside [0, vocab) add nothing."""
-    _check(dedc.is_cuda and ids.is_cuda and dedw.is_cuda, "this library has no CPU path: tensors must live on a CUDA device")
-    _check(dedc.device == ids.device == dedw.device, "The code must be run on the same GPU!")
-    _check(dedw.dim() == 2 and (dedw.stride(1) == 1 or dedw.shape[1] <= 1) and (dedw.shape[0] <= 1 or dedw.stride(0) >= dedw.shape[1]),
-           "a CUDA matrix with unit column stride is required")
-    _check(ids.dtype == torch.int32 and ids.is_contiguous(), "ids must be a packed int32 CUDA tensor")
-    vocab, d = dedw.shape
-    _check(dedc.is_contiguous() and tuple(dedc.shape) == tuple(ids.shape) + (d,), "Incorrect tensor sizes!")
+    dev = dedw.get_device()
+    _check(dev >= 0 and ids.is_cuda and dedc.is_cuda, "this library has no CPU path: tensors must live on a CUDA device")
+    _check(dedc.get_device() == dev and ids.get_device() == dev, "The code must be run on the same GPU!")
+    _check(dedw.dim() == 2, "a CUDA matrix with unit column stride is required")
+    (vocab, d), (pitch, unit) = dedw.shape, dedw.stride()
+    _check((unit == 1 or d <= 1) and (vocab <= 1 or pitch >= d), "a CUDA matrix with unit column stride is required")
+    _check(ids.dtype is torch.int32 and ids.is_contiguous(), "ids must be a packed int32 CUDA tensor")
+    _check(dedc.is_contiguous() and dedc.shape == ids.shape + (d,), "Incorrect tensor sizes!")
     _check(beta == 0.0 or beta == 1.0, "beta must be 0 or 1")
     tokens = ids.numel()
     lib = capi.lib()
     need = lib.ntb_embedding_grad_work(tokens, d)
     work = torch.empty(need, dtype=torch.uint8, device=dedw.device)
-    rc = lib.ntb_embedding_grad(dedw.device.index, _stream(dedw), ids.data_ptr(), dedc.data_ptr(), dedw.data_ptr(), _dtype_code(dedc),
-                                _dtype_code(dedw), tokens, vocab, d, d, dedw.stride(0) if vocab > 1 else d, scale, beta, work.data_ptr(), need)
-    _raise_rc(rc, "GradEmbedding")
+    rc = lib.ntb_embedding_grad(dev, _raw_stream(dev), ids.data_ptr(), dedc.data_ptr(), dedw.data_ptr(), _dtype_code(dedc),
+                                _dtype_code(dedw), tokens, vocab, d, d, pitch if vocab > 1 else d, scale, beta, work.data_ptr(), need)
+    if rc:
+        _raise_rc(rc, "GradEmbedding")
+
+
+_CLIP_TYPES = {torch.float32, torch.float16}
 
 
 def ClipGradNorm(grads, max_norm, out=None):
@@ -364,27 +398,42 @@ def ClipGradNorm(grads, max_norm, out=None):
     min(1, max_norm / norm): in place, or into the tensors of out. Packed fp16 and fp32 CUDA tensors of any
     shapes on one device, each listed once. A norm that is not finite leaves the values as they are. Two launches,
     no copy to the device, no synchronisation."""
-    _check(len(grads) > 0, "Empty input tensors!")
-    into = grads if out is None else out
-    _check(len(into) == len(grads), "Incorrect tensor sizes!")
-    device = grads[0].device
     n = len(grads)
-    for g, o in zip(grads, into):
-        _check(g.is_cuda and o.is_cuda, "this library has no CPU path: tensors must live on a CUDA device")
-        _check(g.device == device and o.device == device, "The code must be run on the same GPU!")
-        _check(g.dtype == o.dtype and g.shape == o.shape, "Incorrect tensor sizes!")
-        _check(g.is_contiguous() and o.is_contiguous(), "tensors must be dense and packed")
-    _check(float(max_norm) >= 0.0, "the norm must not be negative")
-    where = [o.data_ptr() for o in into if o.numel()]
-    _check(len(set(where)) == len(where), "a tensor is listed twice")
-    norm = torch.empty((), dtype=torch.float32, device=device)
+    _check(n > 0, "Empty input tensors!")
+    into = grads if out is None else out
+    _check(len(into) == n, "Incorrect tensor sizes!")
+    max_norm = float(max_norm)
+    _check(max_norm >= 0.0, "the norm must not be negative")
+    # one pass of each question over the list: a model has hundreds of tensors
+    T = torch.Tensor
+    dev = grads[0].get_device()
+    types, counts, sources = [g.dtype for g in grads], list(map(T.numel, grads)), list(map(T.data_ptr, grads))
+    _check(dev >= 0 and all(map(T.is_contiguous, grads)), "tensors must be dense and packed, on a CUDA device: this library has no CPU path")
+    _check(set(map(T.get_device, grads)) == {dev}, "The code must be run on the same GPU!")
+    targets = sources
+    if into is not grads:
+        targets = list(map(T.data_ptr, into))
+        _check(all(map(T.is_contiguous, into)), "tensors must be dense and packed")
+        _check(set(map(T.get_device, into)) == {dev}, "The code must be run on the same GPU!")
+        _check([o.dtype for o in into] == types and list(map(T.numel, into)) == counts, "Incorrect tensor sizes!")
+    if 0 in counts:
+        where = [a for a, c in zip(targets, counts) if c]
+        _check(len(set(where)) == len(where), "a tensor is listed twice")
+    else:
+        _check(len(set(targets)) == n, "a tensor is listed twice")
+    kinds = set(types)
+    _check(kinds <= _CLIP_TYPES, "Unsupported data type!")
+    codes = array.array("i", [_dtype_code(grads[0])]) * n if len(kinds) == 1 else array.array("i", [X_FLOAT if x is torch.float32 else X_FLOAT16 for x in types])
+    a, c = array.array("Q", sources), array.array("q", counts)
+    b = a if targets is sources else array.array("Q", targets)
+    norm = torch.empty((), dtype=torch.float32, device=grads[0].device)
     lib = capi.lib()
     need = lib.ntb_clip_grad_norm_work(n)
-    work = torch.empty(need, dtype=torch.uint8, device=device)
-    rc = lib.ntb_clip_grad_norm(device.index, _stream(grads[0]), n, (ctypes.c_void_p * n)(*[g.data_ptr() for g in grads]),
-                                (ctypes.c_void_p * n)(*[o.data_ptr() for o in into]), (ctypes.c_int * n)(*[_dtype_code(g) for g in grads]),
-                                (ctypes.c_longlong * n)(*[g.numel() for g in grads]), max_norm, norm.data_ptr(), work.data_ptr(), need)
-    _raise_rc(rc, "ClipGradNorm")
+    work = torch.empty(need, dtype=torch.uint8, device=grads[0].device)
+    rc = lib.ntb_clip_grad_norm(dev, _raw_stream(dev), n, a.buffer_info()[0], b.buffer_info()[0], codes.buffer_info()[0], c.buffer_info()[0],
+                                max_norm, norm.data_ptr(), work.data_ptr(), need)
+    if rc:
+        _raise_rc(rc, "ClipGradNorm")
     return norm
 
 
