@@ -30,7 +30,11 @@ namespace {
 
 constexpr int EM_THREADS = 256;
 constexpr int SORT_THREADS = 1024, SORT_WARPS = SORT_THREADS / 32;
-constexpr int SORT_MAX_BITS = 9;
+constexpr int SORT_MAX_BITS = 9, SORT_RADIX = 1 << SORT_MAX_BITS;
+constexpr int SORT_AHEAD = 8;             /* tokens a thread holds at once */
+constexpr int SORT_TILE = SORT_THREADS * SORT_AHEAD;
+constexpr int SORT_CTAS = 16;             /* largest cluster */
+static_assert(SORT_RADIX <= SORT_THREADS, "a thread a digit");
 
 template <typename T> struct EmVec;
 template <> struct EmVec<__half> { static constexpr int N = 8; };
@@ -150,9 +154,42 @@ __device__ __forceinline__ void ClearWarp(unsigned char * p, long long n, int la
         p[done + lane] = 0;
 }
 
+/* the lanes whose digit equals this lane's: one ballot a bit (a 32-bit match instruction took several times as long) */
+__device__ __forceinline__ unsigned SameDigit(int d, int bits, bool in)
+{
+    unsigned same = __ballot_sync(0xffffffffu, in);
+#pragma unroll
+    for (int b = 0; b < SORT_MAX_BITS; b++) {
+        if (b < bits) {
+            const bool set = ((d >> b) & 1) != 0;
+            const unsigned vote = __ballot_sync(0xffffffffu, set);
+            same &= set ? vote : ~vote;
+        }
+    }
+    return same;
+}
+
+/* exclusive sum over the block's first R threads' values; every thread calls */
+__device__ __forceinline__ int BlockScan(int value, int * warpSums, int warp, int lane)
+{
+    int scan = value;
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+        const int o = __shfl_up_sync(0xffffffffu, scan, off);
+        if (lane >= off)
+            scan += o;
+    }
+    if (lane == 31)
+        warpSums[warp] = scan;
+    __syncthreads();
+    const int lower = __reduce_add_sync(0xffffffffu, lane < warp ? warpSums[lane] : 0);
+    return lower + scan - value;
+}
+
 __global__ void __launch_bounds__(SORT_THREADS) TokenSortKernel(const SortParams p)
 {
-    extern __shared__ int counters[];                          /* [warp][digit], then [digit] totals, [digit] bases */
+    extern __shared__ __align__(16) unsigned char sortSmem[];
+    __shared__ int totals[SORT_RADIX], bases[SORT_RADIX], localBases[SORT_RADIX], warpSums[2][SORT_WARPS];
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -160,7 +197,6 @@ __global__ void __launch_bounds__(SORT_THREADS) TokenSortKernel(const SortParams
         const long long warps = (long long)(gridDim.x - p.ctas) * SORT_WARPS;
         const long long first = (long long)(blockIdx.x - p.ctas) * SORT_WARPS + warp;
         if (p.clearPitch == p.clearBytes) {
-            /* rows back to back: equal pieces of a multiple of 512 bytes */
             const long long all = p.clearPitch * p.clearRows;
             const long long piece = 4096;
             for (long long o = first * piece; o < all; o += warps * piece)
@@ -173,20 +209,21 @@ __global__ void __launch_bounds__(SORT_THREADS) TokenSortKernel(const SortParams
         return;
     }
     const int R = 1 << p.bits;
-    int * totals = counters + SORT_WARPS * R, * bases = totals + R;
-    __shared__ int warpSums[SORT_WARPS];
-    const int rank = (int)blockIdx.x;
-    /* this warp's piece of the list, a multiple of 32 tokens long but for the last */
-    const long long pieces = (long long)p.ctas * SORT_WARPS;
-    const long long per = ((p.tokens + pieces - 1) / pieces + 31) / 32 * 32;
-    const long long begin = ((long long)rank * SORT_WARPS + warp) * per;
-    const long long lo = begin < p.tokens ? begin : p.tokens;
-    const long long hi = lo + per < p.tokens ? lo + per : p.tokens;
+    int2 * stage = (int2 *)sortSmem;                              /* a tile in its new order */
+    int * counters = (int *)(stage + SORT_TILE);                  /* [warp][digit] */
     int * mine = counters + warp * R;
+    const int rank = (int)blockIdx.x;
+    /* this CTA's part of the list */
+    const long long per = (p.tokens + p.ctas - 1) / p.ctas;
+    const long long lo = rank * per < p.tokens ? rank * per : p.tokens;
+    const long long hi = lo + per < p.tokens ? lo + per : p.tokens;
     const unsigned before = (1u << lane) - 1u;
+    /* a list of one tile stays in shared memory between the passes; a part of one tile is loaded once a pass */
+    const bool resident = p.ctas == 1 && p.tokens <= SORT_TILE, once = hi - lo <= SORT_TILE;
 
     for (int pass = 0; pass < p.passes; pass++) {
         const int shift = pass * p.bits;
+        const bool last = pass == p.passes - 1;
         /* the last pass writes a */
         int2 * dst = ((p.passes - 1 - pass) & 1) == 0 ? p.a : p.b;
         const int2 * src = dst == p.a ? p.b : p.a;
@@ -195,84 +232,131 @@ __global__ void __launch_bounds__(SORT_THREADS) TokenSortKernel(const SortParams
                 const int id = p.ids[i];
                 return make_int2(id >= 0 && id < p.vocab ? id : p.vocab, (int)i);
             }
-            return __ldcg(src + i);
+            return resident ? stage[i] : __ldcg(src + i);
         };
-        for (int d = threadIdx.x; d < SORT_WARPS * R; d += SORT_THREADS)
-            counters[d] = 0;
-        __syncthreads();
-        for (long long i0 = lo; i0 < hi; i0 += 32) {
-            const long long i = i0 + lane;
-            const bool in = i < hi;
-            const int d = in ? (load(i).x >> shift) & (R - 1) : R;
-            const unsigned same = __match_any_sync(0xffffffffu, d);
-            if (in && (same & before) == 0)
-                mine[d] += __popc(same);
-            __syncwarp();
-        }
-        __syncthreads();
-        if ((int)threadIdx.x < R) {
-            int run = 0;
-            for (int w = 0; w < SORT_WARPS; w++) {
-                const int c = counters[w * R + threadIdx.x];
-                counters[w * R + threadIdx.x] = run;
-                run += c;
-            }
-            totals[threadIdx.x] = run;
-        }
-        if (p.ctas > 1)
-            ClusterSync();
-        else
-            __syncthreads();
-        /* where a digit's tokens start: all smaller digits, then the same digit in the CTAs before this one */
-        int all = 0, ahead = 0;
-        if ((int)threadIdx.x < R) {
-            for (int c = 0; c < p.ctas; c++) {
-                int n;
-                if (p.ctas > 1)
-                    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(n) : "r"(MapShared(SmemAddr(totals + threadIdx.x), c)) : "memory");
-                else
-                    n = totals[threadIdx.x];
-                all += n;
-                ahead += c < rank ? n : 0;
-            }
-        }
-        int scan = all;
+        auto digit = [&](const int2 & x) { return (x.x >> shift) & (R - 1); };
+        /* a warp's tokens lie one behind the other: ranks within a digit follow the list's order */
+        int2 x[SORT_AHEAD];
+        int count = 0, each = 0;                                  /* of a tile; steps of 32 a warp */
+        auto loadTile = [&](long long tile) {
+            count = hi - tile < SORT_TILE ? (int)(hi - tile) : SORT_TILE;
+            each = (count + SORT_WARPS * 32 - 1) / (SORT_WARPS * 32);
 #pragma unroll
-        for (int off = 1; off < 32; off <<= 1) {
-            const int o = __shfl_up_sync(0xffffffffu, scan, off);
-            if (lane >= off)
-                scan += o;
-        }
-        if (lane == 31)
-            warpSums[warp] = scan;
-        __syncthreads();
-        int lower = 0;
-        for (int w = 0; w < warp; w++)
-            lower += warpSums[w];
-        if ((int)threadIdx.x < R)
-            bases[threadIdx.x] = lower + scan - all + ahead;
-        __syncthreads();
-        for (long long i0 = lo; i0 < hi; i0 += 32) {
-            const long long i = i0 + lane;
-            const bool in = i < hi;
-            const int2 x = in ? load(i) : make_int2(0, 0);
-            const int d = in ? (x.x >> shift) & (R - 1) : R;
-            const unsigned same = __match_any_sync(0xffffffffu, d);
-            int at = 0;
-            if (in)
-                at = bases[d] + mine[d] + __popc(same & before);
-            __syncwarp();
-            if (in && (same & before) == 0)
-                mine[d] += __popc(same);
-            __syncwarp();
-            if (in)
-                __stcg(dst + at, x);
-        }
-        /* the scattered list is complete, and the totals have been read, before the next pass */
-        if (p.ctas > 1)
-            ClusterSync();
-        else
+            for (int u = 0; u < SORT_AHEAD; u++) {
+                const int i = (warp * each + u) * 32 + lane;
+                x[u] = u < each && i < count ? load(tile + i) : make_int2(0, 0);
+            }
+        };
+        if (once)
+            loadTile(lo);
+        if (!resident) {
+            if ((int)threadIdx.x < R)
+                totals[threadIdx.x] = 0;
             __syncthreads();
+            if (once) {
+#pragma unroll
+                for (int u = 0; u < SORT_AHEAD; u++)
+                    if (u < each && (warp * each + u) * 32 + lane < count)
+                        atomicAdd(totals + digit(x[u]), 1);
+            }
+            else {
+                for (long long i0 = lo + threadIdx.x; i0 < hi; i0 += SORT_TILE) {
+                    int d[SORT_AHEAD];
+#pragma unroll
+                    for (int u = 0; u < SORT_AHEAD; u++)
+                        d[u] = i0 + u * SORT_THREADS < hi ? digit(load(i0 + u * SORT_THREADS)) : -1;
+#pragma unroll
+                    for (int u = 0; u < SORT_AHEAD; u++)
+                        if (d[u] >= 0)
+                            atomicAdd(totals + d[u], 1);
+                }
+            }
+            ClusterSync();
+            /* where a digit's tokens start: all smaller digits, then the same digit in the CTAs before this one */
+            int all = 0, ahead = 0;
+            if ((int)threadIdx.x < R) {
+                int n[SORT_CTAS];
+#pragma unroll
+                for (int c = 0; c < SORT_CTAS; c++) {
+                    n[c] = 0;
+                    if (c < p.ctas)
+                        asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(n[c]) : "r"(MapShared(SmemAddr(totals + threadIdx.x), c)) : "memory");
+                }
+#pragma unroll
+                for (int c = 0; c < SORT_CTAS; c++) {
+                    all += n[c];
+                    ahead += c < rank ? n[c] : 0;
+                }
+            }
+            const int start = BlockScan(all, warpSums[0], warp, lane) + ahead;
+            if ((int)threadIdx.x < R)
+                bases[threadIdx.x] = start;
+        }
+
+        for (long long tile = lo; tile < hi; tile += SORT_TILE) {
+            if (!once)
+                loadTile(tile);
+            int place[SORT_AHEAD];
+            for (int i = threadIdx.x; i < SORT_WARPS * R / 4; i += SORT_THREADS)
+                ((int4 *)counters)[i] = make_int4(0, 0, 0, 0);
+            __syncthreads();
+#pragma unroll
+            for (int u = 0; u < SORT_AHEAD; u++) {
+                if (u < each) {
+                    const bool in = (warp * each + u) * 32 + lane < count;
+                    const int d = digit(x[u]);
+                    const unsigned same = SameDigit(d, p.bits, in);
+                    place[u] = mine[d] + __popc(same & before);
+                    __syncwarp();
+                    if (in && (same & before) == 0)
+                        mine[d] += __popc(same);
+                    __syncwarp();
+                }
+            }
+            __syncthreads();
+            int run = 0;
+            if ((int)threadIdx.x < R) {
+                int c[SORT_WARPS];
+#pragma unroll
+                for (int w = 0; w < SORT_WARPS; w++)
+                    c[w] = counters[w * R + threadIdx.x];
+#pragma unroll
+                for (int w = 0; w < SORT_WARPS; w++) {
+                    counters[w * R + threadIdx.x] = run;
+                    run += c[w];
+                }
+            }
+            const int local = BlockScan(run, warpSums[1], warp, lane);
+            if ((int)threadIdx.x < R)
+                localBases[threadIdx.x] = local;
+            __syncthreads();
+#pragma unroll
+            for (int u = 0; u < SORT_AHEAD; u++)
+                if (u < each && (warp * each + u) * 32 + lane < count) {
+                    const int d = digit(x[u]);
+                    stage[localBases[d] + mine[d] + place[u]] = x[u];
+                }
+            __syncthreads();
+            if (resident) {
+                if (last)
+                    for (int i = threadIdx.x; i < count; i += SORT_THREADS)
+                        dst[i] = stage[i];
+            }
+            else {
+                /* in the new order neighbours go to neighbouring places: whole lines instead of one store a token */
+                for (int i = threadIdx.x; i < count; i += SORT_THREADS) {
+                    const int2 y = stage[i];
+                    const int d = digit(y);
+                    __stcg(dst + bases[d] + i - localBases[d], y);
+                }
+                __syncthreads();
+                if ((int)threadIdx.x < R)
+                    bases[threadIdx.x] += run;
+            }
+        }
+        /* the list in its new order is complete, and the totals have been read, before the next pass */
+        if (!resident)
+            ClusterSync();
     }
 }
 
@@ -290,44 +374,25 @@ struct RunParams {
     int accumulate;
 };
 
-/* N columns of a run's sum into dw */
-template <typename TW, int N>
-__device__ __forceinline__ void WriteRow(const RunParams & p, int id, int col, const float * acc)
+/* one column of a run's sum into dw */
+template <typename TW>
+__device__ __forceinline__ void WriteColumn(const RunParams & p, int id, int col, float acc)
 {
     TW * dst = (TW *)p.dw + id * p.ldw + col;
-    float v[N];
-#pragma unroll
-    for (int e = 0; e < N; e++)
-        v[e] = fmaf(acc[e], p.scale, p.accumulate ? Get(dst + e) : 0.f);
-#pragma unroll
-    for (int e = 0; e < N; e++)
-        Put(dst + e, v[e]);
-}
-template <typename TW, int N>
-__device__ __forceinline__ void WriteRowVec(const RunParams & p, int id, int col, const float * acc)
-{
-    TW * dst = (TW *)p.dw + id * p.ldw + col;
-    constexpr int PN = EmVec<TW>::N;
-#pragma unroll
-    for (int k = 0; k < N; k += PN) {
-        float v[PN];
-#pragma unroll
-        for (int e = 0; e < PN; e++)
-            v[e] = 0.f;
-        if (p.accumulate)
-            UnpackRow(*(const uint4 *)(dst + k), v, (const TW *)nullptr);
-#pragma unroll
-        for (int e = 0; e < PN; e++)
-            v[e] = fmaf(acc[k + e], p.scale, v[e]);
-        *(uint4 *)(dst + k) = PackRow(v, (const TW *)nullptr);
-    }
+    Put(dst, fmaf(acc, p.scale, p.accumulate ? Get(dst) : 0.f));
 }
 
-/* VEC: 16-byte loads of dout, 16-byte accesses to dw; else one column a thread */
-template <typename TO, typename TW, bool VEC>
+/*
+ * VEC: 16-byte loads of dout, 16-byte accesses to dw; else one column a thread. ACC: the old rows of dw are added.
+ * A thread walks its block's tokens with the loads of U of them in flight together (with ACC those of the old
+ * rows where a word ends, too: loaded at the point of use, 100000 tokens of 512 halves took 140 us instead of 85);
+ * the adds stay in order.
+ */
+template <typename TO, typename TW, bool VEC, bool ACC>
 __global__ void RunSumKernel(const RunParams p)
 {
     constexpr int N = VEC ? EmVec<TO>::N : 1;
+    constexpr int WN = VEC ? N / EmVec<TW>::N : 1;            /* 16-byte pieces of dw a thread owns */
     extern __shared__ int2 items[];                           /* the block's tokens, with the words before and behind it */
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -349,9 +414,8 @@ __global__ void RunSumKernel(const RunParams p)
     const int2 * it = items + 1;
     constexpr int U = VEC ? 8 : 4;
     for (int i0 = 0; i0 < n; i0 += U) {
-        /* the loads of U rows in flight together; the adds stay in order */
-        uint4 raw[VEC ? U : 1];
-        float one[VEC ? 1 : U];
+        uint4 raw[VEC ? U : 1], oldRaw[VEC && ACC ? U * WN : 1];
+        float one[VEC ? 1 : U], oldOne[!VEC && ACC ? U : 1];
 #pragma unroll
         for (int u = 0; u < U; u++) {
             const int i = i0 + u < n ? i0 + u : n - 1;
@@ -360,6 +424,19 @@ __global__ void RunSumKernel(const RunParams p)
                 raw[u] = __ldcs((const uint4 *)src);
             else
                 one[u] = Get(src);
+            if (ACC) {
+                const int id = it[i].x;
+                const bool ends = id != it[i + 1].x && id != p.vocab;
+                const TW * dst = (const TW *)p.dw + (ends ? id : 0) * p.ldw + col;
+                if (VEC) {
+#pragma unroll
+                    for (int k = 0; k < WN; k++)
+                        if (ends)
+                            oldRaw[u * WN + k] = ((const uint4 *)dst)[k];
+                }
+                else
+                    oldOne[u] = ends ? Get(dst) : 0.f;
+            }
         }
 #pragma unroll
         for (int u = 0; u < U; u++) {
@@ -384,10 +461,22 @@ __global__ void RunSumKernel(const RunParams p)
                             for (int e = 0; e < N; e++)
                                 dst[e] = acc[e];
                         }
-                        else if (VEC)
-                            WriteRowVec<TW, N>(p, id, col, acc);
+                        else if (VEC) {
+                            TW * dst = (TW *)p.dw + id * p.ldw + col;
+                            constexpr int PN = EmVec<TW>::N;
+#pragma unroll
+                            for (int k = 0; k < WN; k++) {
+                                float v[PN];
+                                if (ACC)
+                                    UnpackRow(oldRaw[u * WN + k], v, (const TW *)nullptr);
+#pragma unroll
+                                for (int e = 0; e < PN; e++)
+                                    v[e] = fmaf(acc[(k * PN + e) % N], p.scale, ACC ? v[e] : 0.f);
+                                ((uint4 *)dst)[k] = PackRow(v, (const TW *)nullptr);
+                            }
+                        }
                         else
-                            WriteRow<TW, N>(p, id, col, acc);
+                            Put((TW *)p.dw + id * p.ldw + col, fmaf(acc[0], p.scale, ACC ? oldOne[u] : 0.f));
                     }
 #pragma unroll
                     for (int e = 0; e < N; e++)
@@ -413,15 +502,21 @@ __global__ void RunJoinKernel(const RunParams p)
     const long long begin = (long long)i * p.block;
     if (i > 0 && p.sorted[begin - 1].x == id)
         return;                                                /* it began in an earlier block */
-    /* the last block the run reaches: the first of the following ones whose last token is another word (lists are sorted) */
+    /* the first of the following blocks whose last token is another word (the list is sorted), or the last block:
+       32 probes at a time, so that a long list takes two rounds of memory latency and not ten */
     int lo = i + 1, hi = p.blocks - 1;
+    const int lane = threadIdx.x & 31;
     while (lo < hi) {
-        const int mid = (lo + hi) / 2;
-        const long long last = (long long)(mid + 1) * p.block - 1;
-        if (p.sorted[last < p.tokens ? last : p.tokens - 1].x == id)
-            lo = mid + 1;
-        else
-            hi = mid;
+        const int step = (hi - lo + 31) / 32;
+        const int probe = lo + lane * step;
+        bool goesOn = false;
+        if (probe < hi)
+            goesOn = p.sorted[(long long)(probe + 1) * p.block - 1].x == id;
+        const int n = __popc(__ballot_sync(0xffffffffu, goesOn));         /* probes 0 .. n - 1 go on */
+        const int from = n == 0 ? lo : lo + (n - 1) * step + 1;
+        const int to = lo + n * step < hi ? lo + n * step : hi;
+        lo = from;
+        hi = n == 0 ? lo : to;
     }
     /* block lo begins with the run, or is behind a run that ended with block lo - 1 */
     const int stop = p.sorted[(long long)lo * p.block].x == id ? lo : lo - 1;
@@ -439,7 +534,7 @@ __global__ void RunJoinKernel(const RunParams p)
         }
         for (; j <= stop; j++)
             acc += p.head[(long long)j * p.dim + col];
-        WriteRow<TW, 1>(p, id, col, &acc);
+        WriteColumn<TW>(p, id, col, acc);
     }
 }
 
@@ -450,6 +545,14 @@ int RunBlock(int tokens)
     while (block < 256 && (long long)block * 592 < tokens)
         block *= 2;
     return block;
+}
+
+/* CTAs that sort. Whole call on a B200 with 512 halves a row, us in graph replay with 1 / 8 / 16 CTAs: 2048 tokens
+   17.9 / 18.0 / 18.8, 4096 22.5 / 19.8 / 20.2, 8192 32 / 22 / 22, 20000 96 / 33 / 32, 100000 391 / 109 / 85. One CTA keeps
+   its passes in shared memory and needs no barriers of the cluster; more rank fewer tokens each. */
+int SortCtas(int tokens)
+{
+    return tokens <= 2048 ? 1 : tokens <= 16384 ? 8 : SORT_CTAS;
 }
 
 bool RowsAligned(const void * p, long long pitch, int dim, int size)
@@ -474,7 +577,9 @@ cudaError_t LaunchRuns(const RunParams & p, cudaStream_t stream)
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = PdlEnabled() ? 1 : 0;
-    cudaError_t err = vec ? cudaLaunchKernelEx(&cfg, RunSumKernel<TO, TW, true>, p) : cudaLaunchKernelEx(&cfg, RunSumKernel<TO, TW, false>, p);
+    cudaError_t err = p.accumulate
+        ? (vec ? cudaLaunchKernelEx(&cfg, RunSumKernel<TO, TW, true, true>, p) : cudaLaunchKernelEx(&cfg, RunSumKernel<TO, TW, false, true>, p))
+        : (vec ? cudaLaunchKernelEx(&cfg, RunSumKernel<TO, TW, true, false>, p) : cudaLaunchKernelEx(&cfg, RunSumKernel<TO, TW, false, false>, p));
     CountLaunch();
     if (err != cudaSuccess || p.blocks == 1)
         return err;
@@ -566,8 +671,8 @@ extern "C" int ntb_embedding_grad(int devID, void * stream, const int * ids, con
         keyBits++;
     s.passes = (keyBits + SORT_MAX_BITS - 1) / SORT_MAX_BITS;
     s.bits = (keyBits + s.passes - 1) / s.passes;
-    /* one CTA sorts a thousand tokens a pass in about the time of a cluster barrier */
-    s.ctas = tokens <= 2048 ? 1 : tokens <= 8192 ? 4 : 8;
+    s.bits = s.bits < 2 ? 2 : s.bits;                       /* counters are cleared four at a time */
+    s.ctas = SortCtas(tokens);
     int grid = tokens > 0 ? s.ctas : 0;
     if (tokens == 0)
         s.ctas = 0;
@@ -582,9 +687,13 @@ extern "C" int ntb_embedding_grad(int devID, void * stream, const int * ids, con
         const int extra = (ctx->smCount - grid) / unit * unit;
         grid += extra > unit ? extra : unit;
     }
-    const int smem = (SORT_WARPS + 2) * (1 << s.bits) * (int)sizeof(int);
+    const int smem = SORT_TILE * (int)sizeof(int2) + SORT_WARPS * (1 << s.bits) * (int)sizeof(int);
     static SmemOptIn optIn;
-    if (!optIn.Ensure((const void *)TokenSortKernel, (SORT_WARPS + 2) * (1 << SORT_MAX_BITS) * (int)sizeof(int)))
+    if (!optIn.Ensure((const void *)TokenSortKernel, SORT_TILE * (int)sizeof(int2) + SORT_WARPS * SORT_RADIX * (int)sizeof(int)))
+        return NTB_ERR_CUDA;
+    /* clusters of more than 8 CTAs are an opt-in of the kernel's on the device */
+    static ClusterOptIn wide;
+    if (s.ctas > 8 && !wide.Ensure((const void *)TokenSortKernel))
         return NTB_ERR_CUDA;
     cudaError_t err = LaunchClusterPdl(TokenSortKernel, (unsigned)grid, SORT_THREADS, smem, s.ctas > 0 ? s.ctas : 1, st, s);
     CountLaunch();

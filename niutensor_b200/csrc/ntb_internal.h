@@ -165,6 +165,26 @@ struct SmemOptIn {
     }
 };
 
+/* the same for clusters of more than eight CTAs */
+struct ClusterOptIn {
+    std::atomic<int> done[64];
+    ClusterOptIn() { for (int i = 0; i < 64; i++) done[i].store(0); }
+    bool Ensure(const void * kern)
+    {
+        int dev = 0;
+        if (cudaGetDevice(&dev) != cudaSuccess)
+            return false;
+        const bool tracked = dev >= 0 && dev < 64;
+        if (tracked && done[dev].load(std::memory_order_acquire))
+            return true;
+        if (cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess)
+            return false;
+        if (tracked)
+            done[dev].store(1, std::memory_order_release);
+        return true;
+    }
+};
+
 static inline size_t ElemSize(int dt) { return dt == NTB_X_FLOAT16 ? 2 : 4; }
 
 }
