@@ -11,7 +11,7 @@
  * on the key side); the sample pads the sentences of a batch, which the two length vectors describe.
  *
  * XattnKernel (many query rows): a CTA holds one or two 128-row query tiles ("streams") of one key
- * head and walks the key tiles. Warps 0-3 (4-7): softmax of stream 0 (1), a thread per row;
+ * head and walks the key tiles. Warps 0-7 (8-15): softmax of stream 0 (1), two threads a row;
  * then the TMA producer warp and the MMA warp. Scores S = q k^T go to tensor memory, the softmax
  * writes the weights back over them as halves, and the second product takes them from there as its A
  * operand, so neither ever touches shared memory. While one stream is in its softmax the tensor
@@ -55,10 +55,37 @@ template <int D, int STREAMS> struct XattnSmem {
     static constexpr int Q_BYTES = STREAMS * TILE;
     static constexpr int RING_BYTES = SLOTS * TILE;
     static constexpr int TOTAL = Q_BYTES + RING_BYTES + 1024;
-    static constexpr int THREADS = STREAMS * 128 + 64;
+    static constexpr int THREADS = STREAMS * 256 + 64;
     static constexpr int TMEM_COLS = STREAMS == 2 ? 512 : 256;
     static_assert(RING_BYTES >= STREAMS * XT * D * 4, "the split's partial sums take the place of the ring");
 };
+
+/* the 256 threads of a stream: whether any of them says so; and a plain barrier */
+__device__ __forceinline__ bool StreamAny(int id, bool say)
+{
+    uint32_t any;
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 q, %1, 0;\n\tbarrier.cta.red.or.aligned.pred p, %2, 256, q;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                 : "=r"(any) : "r"((uint32_t)say), "r"(id) : "memory");
+    return any != 0;
+}
+__device__ __forceinline__ void StreamBarrier(int id) { asm volatile("barrier.cta.sync.aligned %0, 256;" :: "r"(id) : "memory"); }
+
+/* one value from the two threads of every row of a stream, through one word a row */
+template <typename Op>
+__device__ __forceinline__ float Joint(int s, int hf, volatile float * word, float mine, Op op)
+{
+    if (hf == 1)
+        *word = mine;
+    StreamBarrier(1 + s);
+    if (hf == 0) {
+        mine = op(mine, *word);
+        *word = mine;
+    }
+    StreamBarrier(1 + s);
+    if (hf == 1)
+        mine = *word;
+    return mine;
+}
 
 template <int D, int STREAMS>
 __global__ void __launch_bounds__(XattnSmem<D, STREAMS>::THREADS, STREAMS == 2 ? 1 : 2)
@@ -72,6 +99,7 @@ XattnKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
     __shared__ __align__(8) uint64_t barFull[SLOTS], barEmpty[SLOTS], barQ[STREAMS], barS[STREAMS], barP[STREAMS], barO[STREAMS], barFix;
     __shared__ uint32_t tmemBaseSlot;
     __shared__ int abortFlag;
+    __shared__ float sHalf[STREAMS][XT];                 /* what the two threads of a row tell each other */
     const int warp = threadIdx.x >> 5;
     const int lane = threadIdx.x & 31;
     const uint32_t smemBase = (SmemAddr(smemRaw) + 1023u) & ~1023u;
@@ -79,7 +107,7 @@ XattnKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
     /* a split item's references and sums, in the place of its queries once those have been read */
     float * sM = (float *)(smemRaw + (smemBase - SmemAddr(smemRaw))), * sL = sM + STREAMS * XT;
     volatile int * abortPtr = &abortFlag;
-    constexpr int PRODUCER = STREAMS * 4, ISSUER = STREAMS * 4 + 1;
+    constexpr int PRODUCER = STREAMS * 8, ISSUER = STREAMS * 8 + 1;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
     if (warp == PRODUCER && lane == 0) {
@@ -96,7 +124,7 @@ XattnKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
         for (int s = 0; s < STREAMS; s++) {
             MbarInit(SmemAddr(&barQ[s]), 1);
             MbarInit(SmemAddr(&barS[s]), 1);
-            MbarInit(SmemAddr(&barP[s]), 128);
+            MbarInit(SmemAddr(&barP[s]), 256);
             MbarInit(SmemAddr(&barO[s]), 1);
         }
         MbarInit(SmemAddr(&barFix), 1);
@@ -156,17 +184,16 @@ XattnKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
                     TmaLoad4D(qS + s * TILE + dc * XBOX_BYTES, &tmQ, SmemAddr(&barQ[s]), dc * 64, q0[s],
                               head[s] * p.aQ.mulHead, b * p.aQ.mulBatch);
             }
-            int slot = 0;
-            uint32_t phase = 0;
-            for (int t = 0; ok && t < 2 * n; t++) {
-                if (t >= SLOTS)
-                    ok = MbarWait(SmemAddr(&barEmpty[slot]), phase ^ 1u, abortPtr, p.status);
+            /* tiles in the order of their use: k 0, v 0, k 1, v 1, ... */
+            for (int i = 0; ok && i < 2 * n; i++) {
+                if (i >= SLOTS)
+                    ok = MbarWait(SmemAddr(&barEmpty[i % SLOTS]), (uint32_t)(i / SLOTS + 1) & 1u, abortPtr, p.status);
                 if (!ok)
                     break;
-                const int row = (tile0 + (t >> 1)) * XT;
-                const uint32_t dst = ringS + slot * TILE, bar = SmemAddr(&barFull[slot]);
+                const int row = (tile0 + (i >> 1)) * XT;
+                const uint32_t dst = ringS + (i % SLOTS) * TILE, bar = SmemAddr(&barFull[i % SLOTS]);
                 MbarExpectTx(bar, TILE);
-                if ((t & 1) == 0) {
+                if ((i & 1) == 0) {
 #pragma unroll
                     for (int dc = 0; dc < DC; dc++)
                         TmaLoad4D(dst + dc * XBOX_BYTES, &tmK, bar, dc * 64, row, kvHead * p.aK.mulHead, b * p.aK.mulBatch);
@@ -176,17 +203,13 @@ XattnKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
                     for (int dc = 0; dc < DC; dc++)
                         TmaLoad4D(dst + dc * XBOX_BYTES, &tmV, bar, dc * 64, row, kvHead * p.aV.mulHead, b * p.aV.mulBatch);
                 }
-                if (++slot == SLOTS) {
-                    slot = 0;
-                    phase ^= 1u;
-                }
             }
         }
         __syncwarp();
         if (fix) {
-            const int t = 2 * n - 1, slot = t % SLOTS;
-            if (MbarWaitWarp(SmemAddr(&barFull[slot]), (uint32_t)(t / SLOTS) & 1u, abortPtr, p.status, 200)) {
-                ZeroTileRows(ringS + slot * TILE, DC, nk - (tile1 - 1) * XT, lane);
+            const int i = 2 * n - 1;
+            if (WaitNowWarp(SmemAddr(&barFull[i % SLOTS]), (uint32_t)(i / SLOTS) & 1u, abortPtr, p.status)) {
+                ZeroTileRows(ringS + (i % SLOTS) * TILE, DC, nk - (tile1 - 1) * XT, lane);
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
                 if (lane == 0)
@@ -197,7 +220,6 @@ XattnKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
     else if (warp == ISSUER) {
         if (lane == 0 && n > 0) {
             constexpr uint32_t descS = XattnDesc(XT, 0), descO = XattnDesc(D, 1);
-            bool ok = true;
             auto scores = [&](int s, uint32_t kTile) {
 #pragma unroll
                 for (int dc = 0; dc < DC; dc++)
@@ -208,12 +230,13 @@ XattnKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
                                  SmemDesc(kTile + dc * XBOX_BYTES + ks * UMMA_K_BYTES, 16, 1024, 2), descS, (dc | ks) != 0 ? 1u : 0u);
                 TcCommit(SmemAddr(&barS[s]));
             };
-            ok = MbarWait(SmemAddr(&barFull[0]), 0, abortPtr, p.status);
+            auto full = [&](int i) { return WaitNow(SmemAddr(&barFull[i % SLOTS]), (uint32_t)(i / SLOTS) & 1u, abortPtr, p.status); };
+            bool ok = full(0);
 #pragma unroll
             for (int s = 0; s < STREAMS; s++) {
                 if (!live[s])
                     continue;
-                ok = ok && MbarWait(SmemAddr(&barQ[s]), 0, abortPtr, p.status);
+                ok = ok && WaitNow(SmemAddr(&barQ[s]), 0, abortPtr, p.status);
                 if (ok) {
                     TcFenceAfter();
                     scores(s, ringS);
@@ -222,173 +245,176 @@ XattnKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
             if (ok)
                 TcCommit(SmemAddr(&barEmpty[0]));
             for (int j = 0; ok && j < n; j++) {
-                const int tv = 2 * j + 1, sv = tv % SLOTS, tk = tv + 1, sk = tk % SLOTS;
-                ok = MbarWait(SmemAddr(&barFull[sv]), (uint32_t)(tv / SLOTS) & 1u, abortPtr, p.status);
+                const int iv = 2 * j + 1, ik = iv + 1;
+                const uint32_t vTile = ringS + (iv % SLOTS) * TILE, kTile = ringS + (ik % SLOTS) * TILE;
+                ok = full(iv) && (j + 1 == n || full(ik));
                 if (ok && fix && j == n - 1)
-                    ok = MbarWait(SmemAddr(&barFix), 0, abortPtr, p.status);
-                if (ok && j + 1 < n)
-                    ok = MbarWait(SmemAddr(&barFull[sk]), (uint32_t)(tk / SLOTS) & 1u, abortPtr, p.status);
-                const uint32_t vTile = ringS + sv * TILE;
+                    ok = WaitNow(SmemAddr(&barFix), 0, abortPtr, p.status);
 #pragma unroll
                 for (int s = 0; s < STREAMS; s++) {
                     if (!ok || !live[s])
                         continue;
-                    ok = MbarWait(SmemAddr(&barP[s]), (uint32_t)j & 1u, abortPtr, p.status);
+                    ok = WaitNow(SmemAddr(&barP[s]), (uint32_t)j & 1u, abortPtr, p.status);
                     if (!ok)
                         continue;
                     TcFenceAfter();
+                    /* the weights of keys 0-63 and 64-127 lie over the two halves of the scores */
 #pragma unroll
                     for (int ks = 0; ks < XT / 16; ks++)
-                        TcMmaTmemA(tmemBase + TMEM_O + s * D, tmemBase + TMEM_S + s * XT + ks * 8,
+                        TcMmaTmemA(tmemBase + TMEM_O + s * D, tmemBase + TMEM_S + s * XT + (ks >> 2) * 64 + (ks & 3) * 8,
                                    SmemDesc(vTile + ks * 16 * ROW_BYTES, XBOX_BYTES, 1024, 2), descO, (j | ks) != 0 ? 1u : 0u);
                     if (j + 1 < n)
-                        scores(s, ringS + sk * TILE);
+                        scores(s, kTile);
                     else
                         TcCommit(SmemAddr(&barO[s]));
                 }
                 if (ok) {
-                    TcCommit(SmemAddr(&barEmpty[sv]));
+                    TcCommit(SmemAddr(&barEmpty[iv % SLOTS]));
                     if (j + 1 < n)
-                        TcCommit(SmemAddr(&barEmpty[sk]));
+                        TcCommit(SmemAddr(&barEmpty[ik % SLOTS]));
                 }
             }
         }
     }
     else {
-        const int s = STREAMS == 2 ? warp >> 2 : 0;
-        const int sub = warp & 3;
+        const int s = STREAMS == 2 ? warp >> 3 : 0, hf = (warp >> 2) & 1, sub = warp & 3;
         const uint32_t laneBase = (uint32_t)(sub * 32) << 16;
-        const uint32_t sT = tmemBase + laneBase + TMEM_S + s * XT, oT = tmemBase + laneBase + TMEM_O + s * D;
-        const int r = sub * 32 + lane;                      /* this thread's row of the tile */
+        const uint32_t sT = tmemBase + laneBase + TMEM_S + s * XT + hf * 64;
+        const uint32_t oT = tmemBase + laneBase + TMEM_O + s * D + hf * (D / 2);
+        const int r = sub * 32 + lane;                      /* this thread's row of the tile; its half: keys and columns hf */
         const bool mine = STREAMS == 2 && s == 1 ? live[STREAMS - 1] : live[0];
         const bool there = STREAMS == 2 && s == 1 ? exists[STREAMS - 1] : exists[0];
         const int myHead = STREAMS == 2 && s == 1 ? head[STREAMS - 1] : head[0];
         const int myQ0 = STREAMS == 2 && s == 1 ? q0[STREAMS - 1] : q0[0];
-        float m = -INFINITY, l = 0.f;                        /* reference of the exponents (times log2 e), sum */
+        float m = -INFINITY, l = 0.f;                        /* reference of the exponents (times log2 e), this half's sum */
+        const uint64_t scale2 = Pair(p.scaleLog2, p.scaleLog2);
+        /* After a wait that ran out the loop goes on with what is there (the next waits return at once): the
+           warps of a stream meet at a barrier in every step, which none of them may leave out. */
         bool ok = true;
         if (mine) {
             for (int j = 0; j < n; j++) {
-                ok = MbarWaitWarp(SmemAddr(&barS[s]), (uint32_t)j & 1u, abortPtr, p.status, 200);
-                if (!ok)
-                    break;
+                ok = WaitNowWarp(SmemAddr(&barS[s]), (uint32_t)j & 1u, abortPtr, p.status) && ok;
                 TcFenceAfter();
-                uint32_t x[XT];
-#pragma unroll
-                for (int c = 0; c < 4; c++)
-                    TmemLoad32Async(sT + c * 32, x + c * 32);
+                uint32_t x[64];
+                TmemLoad32Async(sT, x);
+                TmemLoad32Async(sT + 32, x + 32);
                 TmemWaitLoad();
-                const int valid = nk - (tile0 + j) * XT;
-                if (valid < XT) {
+                const int valid = nk - (tile0 + j) * XT - hf * 64;
+                if (valid < 64) {
 #pragma unroll
-                    for (int e = 0; e < XT; e++)
+                    for (int e = 0; e < 64; e++)
                         x[e] = e < valid ? x[e] : 0xff800000u;
                 }
                 float m4[4] = { -INFINITY, -INFINITY, -INFINITY, -INFINITY };
 #pragma unroll
-                for (int e = 0; e < XT; e += 2)
+                for (int e = 0; e < 64; e += 2)
                     m4[(e >> 1) & 3] = fmaxf(fmaxf(m4[(e >> 1) & 3], __uint_as_float(x[e])), __uint_as_float(x[e + 1]));
                 const float top = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * p.scaleLog2;
-                if (j == 0)
-                    m = top;
-                else if (__any_sync(0xffffffffu, top > m + 8.f)) {
-                    /* the scores' commit covers the second product before it: the accumulator is current */
-                    const float mNew = fmaxf(m, top);
+                /* Both threads of a row use one reference. It follows the maximum once that is 8 ahead in some row of
+                   the stream (weights up to 2^8 are as exact in half as weights up to 1), which the first tile
+                   settles and later ones rarely need. */
+                if (StreamAny(1 + s, j == 0 || top > m + 8.f)) {
+                    const float mNew = fmaxf(m, Joint(s, hf, &sHalf[s][r], top, [](float a, float b) { return fmaxf(a, b); }));
                     const float f = mNew > m ? Exp2(m - mNew) : 1.f;
                     m = mNew;
                     l *= f;
+                    if (j > 0) {
+                        /* the scores' commit covers the second product before it: the accumulator is current */
+#pragma unroll 1
+                        for (int c = 0; c < D / 2; c += 8) {      /* few registers: the scores are in the others */
+                            uint32_t o[8];
+                            TmemLoad8Async(oT + c, o);
+                            TmemWaitLoad();
 #pragma unroll
-                    for (int c = 0; c < D / 32; c++) {
-                        uint32_t o[32];
-                        TmemLoad32Async(oT + c * 32, o);
-                        TmemWaitLoad();
-#pragma unroll
-                        for (int e = 0; e < 32; e++)
-                            o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-                        TmemStore16Async(oT + c * 32, o);
-                        TmemStore16Async(oT + c * 32 + 16, o + 16);
+                            for (int e = 0; e < 8; e++)
+                                o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+                            TmemStore4Async(oT + c, o);
+                            TmemStore4Async(oT + c + 4, o + 4);
+                        }
                     }
                 }
                 const float ref = m == -INFINITY ? 0.f : m;
-                float l4[4] = { 0.f, 0.f, 0.f, 0.f };
+                const uint64_t ref2 = Pair(-ref, -ref);
+                uint64_t sum[2] = { 0, 0 };
 #pragma unroll
-                for (int c = 0; c < 4; c++) {
-                    uint32_t w[16];
+                for (int c = 0; c < 8; c++) {
+                    uint32_t w[4];
 #pragma unroll
-                    for (int e = 0; e < 16; e++) {
-                        const float p0 = Exp2(fmaf(__uint_as_float(x[c * 32 + 2 * e]), p.scaleLog2, -ref));
-                        const float p1 = Exp2(fmaf(__uint_as_float(x[c * 32 + 2 * e + 1]), p.scaleLog2, -ref));
-                        l4[e & 3] += p0 + p1;
+                    for (int e = 0; e < 4; e++) {
+                        const uint64_t y = Fma2(Pair(__uint_as_float(x[c * 8 + 2 * e]), __uint_as_float(x[c * 8 + 2 * e + 1])), scale2, ref2);
+                        float p0, p1;
+                        Unpair(y, p0, p1);
+                        p0 = Exp2(p0);
+                        p1 = Exp2(p1);
+                        sum[e & 1] = Add2(sum[e & 1], Pair(p0, p1));
                         w[e] = PackHalf2(p0, p1);
                     }
-                    TmemStore16Async(sT + c * 16, w);
+                    TmemStore4Async(sT + c * 4, w);
                 }
-                l += (l4[0] + l4[1]) + (l4[2] + l4[3]);
+                float la, lb;
+                Unpair(Add2(sum[0], sum[1]), la, lb);
+                l += la + lb;
                 TmemWaitStore();
                 TcFenceBefore();
                 MbarArrive(SmemAddr(&barP[s]));
             }
+            /* the row's sum from its two halves */
+            l = Joint(s, hf, &sHalf[s][r], l, [](float a, float b) { return a + b; });
         }
         /* every stream's last product is done: its inputs in shared memory are free again */
 #pragma unroll
         for (int t = 0; t < STREAMS; t++)
-            if (n > 0 && live[t] && ok)
-                ok = MbarWaitWarp(SmemAddr(&barO[t]), 0, abortPtr, p.status, 200);
+            if (n > 0 && live[t])
+                ok = WaitNowWarp(SmemAddr(&barO[t]), 0, abortPtr, p.status) && ok;
         TcFenceAfter();
         const bool sums = mine && n > 0 && ok;
-        if (p.splits == 1) {
-            const int row = myQ0 + r;
-            const bool rowLive = mine && row < nq && n > 0;
-            const float inv = rowLive && l > 0.f ? 1.f / l : 0.f;
-            if (there && ok) {
-                const uint32_t box = qS + s * TILE + sub * 32 * ROW_BYTES;
-#pragma unroll
-                for (int c = 0; c < D / 32; c++) {
-                    uint32_t o[32];
-                    if (sums) {
-                        TmemLoad32Async(oT + c * 32, o);
-                        TmemWaitLoad();
-                    }
-#pragma unroll
-                    for (int jj = 0; jj < 4; jj++) {
-                        uint32_t w[4];
-#pragma unroll
-                        for (int e = 0; e < 4; e++)
-                            w[e] = rowLive ? PackHalf2(__uint_as_float(o[jj * 8 + 2 * e]) * inv, __uint_as_float(o[jj * 8 + 2 * e + 1]) * inv) : 0u;
-                        const int chunk = (c & 1) * 4 + jj;
-                        StoreShared16(box + (c >> 1) * XBOX_BYTES + lane * ROW_BYTES + ((chunk ^ (lane & 7)) << 4), w[0], w[1], w[2], w[3]);
-                    }
-                }
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                __syncwarp();
-                if (lane == 0 && myQ0 + sub * 32 < p.sh.lenQ) {
-#pragma unroll
-                    for (int dc = 0; dc < DC; dc++)
-                        TmaStore4D(&tmO, box + dc * XBOX_BYTES, dc * 64, myQ0 + sub * 32, myHead, b);
-                    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
-                    asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
-                }
-                if (p.lse != nullptr && row < p.sh.lenQ)
-                    p.lse[((long long)b * p.sh.headsQ + myHead) * p.sh.lenQ + row] =
-                        rowLive ? (m + log2f(l)) * LN2 : -INFINITY;
-            }
-        }
-        else {
-            /* the partial sums of this CTA's keys, 16-byte chunks of a row permuted by the row's low bits */
+        const int row = myQ0 + r;
+        const bool rowLive = mine && row < nq && n > 0;
+        const float inv = rowLive && l > 0.f ? 1.f / l : 0.f;
+        if (p.splits > 1 && hf == 0) {
             sM[s * XT + r] = sums ? m : -INFINITY;
             sL[s * XT + r] = sums ? l : 0.f;
-            const uint32_t base = ringS + (s * XT + r) * D * 4;
+        }
+        const uint32_t box = qS + s * TILE + sub * 32 * ROW_BYTES, part = ringS + (s * XT + r) * D * 4;
 #pragma unroll
-            for (int c = 0; c < D / 32; c++) {
-                uint32_t o[32];
-                if (sums) {
-                    TmemLoad32Async(oT + c * 32, o);
-                    TmemWaitLoad();
+        for (int cc = 0; cc < D / 64; cc++) {
+            const int c = hf * (D / 64) + cc;                /* of the row's 32-column pieces */
+            uint32_t o[32];
+            if (sums) {
+                TmemLoad32Async(oT + cc * 32, o);
+                TmemWaitLoad();
+            }
+            if (p.splits == 1) {
+#pragma unroll
+                for (int jj = 0; jj < 4; jj++) {
+                    uint32_t w[4];
+#pragma unroll
+                    for (int e = 0; e < 4; e++)
+                        w[e] = sums && rowLive ? PackHalf2(__uint_as_float(o[jj * 8 + 2 * e]) * inv, __uint_as_float(o[jj * 8 + 2 * e + 1]) * inv) : 0u;
+                    const int chunk = (c & 1) * 4 + jj;
+                    StoreShared16(box + (c >> 1) * XBOX_BYTES + lane * ROW_BYTES + ((chunk ^ (lane & 7)) << 4), w[0], w[1], w[2], w[3]);
                 }
+            }
+            else {
+                /* the partial sums of this CTA's keys, 16-byte chunks of a row permuted by the row's low bits */
 #pragma unroll
                 for (int jj = 0; jj < 8; jj++)
-                    StoreShared16(base + (((c * 8 + jj) ^ (r & 7)) << 4), sums ? o[jj * 4] : 0u, sums ? o[jj * 4 + 1] : 0u,
+                    StoreShared16(part + (((c * 8 + jj) ^ (r & 7)) << 4), sums ? o[jj * 4] : 0u, sums ? o[jj * 4 + 1] : 0u,
                                   sums ? o[jj * 4 + 2] : 0u, sums ? o[jj * 4 + 3] : 0u);
             }
+        }
+        if (p.splits == 1) {
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            StreamBarrier(1 + s);
+            if (there && ok && hf == 0 && lane == 0 && myQ0 + sub * 32 < p.sh.lenQ) {
+#pragma unroll
+                for (int dc = 0; dc < DC; dc++)
+                    TmaStore4D(&tmO, box + dc * XBOX_BYTES, dc * 64, myQ0 + sub * 32, myHead, b);
+                asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+                asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+            }
+            if (there && ok && hf == 0 && p.lse != nullptr && row < p.sh.lenQ)
+                p.lse[((long long)b * p.sh.headsQ + myHead) * p.sh.lenQ + row] = rowLive ? (m + log2f(l)) * LN2 : -INFINITY;
         }
         __syncwarp();
     }
@@ -400,10 +426,10 @@ XattnKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
     }
     if (p.splits > 1) {
         ClusterSync();
-        if (warp < STREAMS * 4) {
+        if (warp < STREAMS * 8) {
             const int rowsEach = XT / p.splits;
             const int chunks = D / 8;
-            for (int i = threadIdx.x; i < STREAMS * rowsEach * chunks; i += STREAMS * 128) {
+            for (int i = threadIdx.x; i < STREAMS * rowsEach * chunks; i += STREAMS * 256) {
                 const int c = i % chunks, rr = i / chunks;
                 const int s = rr / rowsEach, r = rank * rowsEach + (rr - s * rowsEach);
                 const bool second = STREAMS == 2 && s == 1;

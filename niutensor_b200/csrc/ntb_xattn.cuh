@@ -54,6 +54,35 @@ __device__ __forceinline__ int ClampLen(const int * lens, int b, int longest)
     return n < 0 ? 0 : n > longest ? longest : n;
 }
 
+/*
+ * The waits on the critical path between the softmax warps and the MMA thread: without a suspend hint (a
+ * parked thread sees the barrier several hundred clocks late, as much as half a tile's products take), all lanes
+ * polling; bounded as MbarWait.
+ */
+__device__ __forceinline__ bool WaitNow(uint32_t bar, uint32_t parity, volatile int * abortFlag, int * status)
+{
+    return MbarWait(bar, parity, abortFlag, status, 0);
+}
+__device__ __forceinline__ bool WaitNowWarp(uint32_t bar, uint32_t parity, volatile int * abortFlag, int * status)
+{
+    if (__all_sync(0xffffffffu, MbarTryWait(bar, parity, 0) != 0))
+        return true;
+    const long long t0 = clock64();
+    for (uint32_t it = 1; ; ++it) {
+        if (__all_sync(0xffffffffu, MbarTryWait(bar, parity, 0) != 0))
+            return true;
+        if ((it & 63u) == 0) {
+            const bool late = clock64() - t0 > WaitLimit(status);
+            if (late) {
+                *abortFlag = 1;
+                atomicExch(status, NTB_ERR_DEVICE_WAIT);
+            }
+            if (__any_sync(0xffffffffu, late || *abortFlag != 0))
+                return false;
+        }
+    }
+}
+
 __device__ __forceinline__ void TmaLoad4D(uint32_t dst, const CUtensorMap * map, uint32_t bar, int c0, int c1, int c2, int c3)
 {
     asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes"
@@ -87,6 +116,11 @@ __device__ __forceinline__ void TmemLoad32Async(uint32_t taddr, uint32_t * r)
                    "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
                  : "r"(taddr) : "memory");
 }
+__device__ __forceinline__ void TmemLoad8Async(uint32_t taddr, uint32_t * r)
+{
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]) : "r"(taddr) : "memory");
+}
 __device__ __forceinline__ void TmemWaitLoad() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void TmemWaitStore() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
@@ -100,11 +134,47 @@ __device__ __forceinline__ void TmemStore16Async(uint32_t taddr, const uint32_t 
                  : "memory");
 }
 
+__device__ __forceinline__ void TmemStore4Async(uint32_t taddr, const uint32_t * v)
+{
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1, %2, %3, %4};"
+                 :: "r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]) : "memory");
+}
+
 __device__ __forceinline__ float Exp2(float x)
 {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+
+/* pairs of floats in one 64-bit register: sm_100 adds and multiplies both in one instruction */
+__device__ __forceinline__ uint64_t Pair(float lo, float hi)
+{
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+    return r;
+}
+__device__ __forceinline__ void Unpair(uint64_t v, float & lo, float & hi)
+{
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
+}
+__device__ __forceinline__ uint64_t Fma2(uint64_t a, uint64_t b, uint64_t c)
+{
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t Add2(uint64_t a, uint64_t b)
+{
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t Mul2(uint64_t a, uint64_t b)
+{
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
 }
 
 __device__ __forceinline__ uint32_t PackHalf2(float lo, float hi)

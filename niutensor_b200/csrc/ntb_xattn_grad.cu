@@ -31,8 +31,8 @@ namespace ntb {
 
 namespace {
 
-constexpr int GR_THREADS = 320;
-constexpr int GR_PRODUCER = 8, GR_ISSUER = 9;
+constexpr int GR_THREADS = 352;
+constexpr int GR_PRODUCER = 8, GR_ISSUER = 9;      /* and a second issuing warp, 10 */
 constexpr float P_SCALE_LOG2 = 12.f, P_SCALE_INV = 1.f / 4096.f;
 
 struct XattnGradParams {
@@ -56,14 +56,14 @@ struct XattnGradParams {
 template <int D> struct XattnGradSmem {
     static constexpr int DC = D / 64;
     static constexpr int TILE = DC * XBOX_BYTES;
-    /* first kernel: q, do, and a ring of k and v tiles */
-    static constexpr int SLOTS = D == 128 ? 5 : 8;
-    static constexpr int Q_TOTAL = (2 + SLOTS) * TILE + 1024;
+    /* first kernel: q, do, and a ring of (k, v) */
+    static constexpr int QSTAGES = D == 128 ? 2 : 4;
+    static constexpr int Q_TOTAL = (2 + 2 * QSTAGES) * TILE + 1024;
     /* second kernel: k, v, and a ring of (q, do, lse and delta) */
     static constexpr int STAGE = 2 * TILE + 1024;
     static constexpr int STAGES = D == 128 ? 2 : 4;
     static constexpr int KV_TOTAL = 2 * TILE + STAGES * STAGE + 1024;
-    static_assert(SLOTS * TILE >= XT * D * 4 && STAGES * STAGE >= 2 * XT * D * 4, "the split's partial sums take the place of the ring");
+    static_assert(QSTAGES * 2 * TILE >= XT * D * 4 && STAGES * STAGE >= 2 * XT * D * 4, "the split's partial sums take the place of the ring");
 };
 
 __device__ __forceinline__ void GradBarrier() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
@@ -120,10 +120,10 @@ XattnGradQKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                  const __grid_constant__ CUtensorMap tmDO, const __grid_constant__ CUtensorMap tmDQ, const XattnGradParams p)
 {
     using SM = XattnGradSmem<D>;
-    constexpr int DC = SM::DC, TILE = SM::TILE, SLOTS = SM::SLOTS;
+    constexpr int DC = SM::DC, TILE = SM::TILE, STAGES = SM::QSTAGES;
     constexpr int TMEM_S = 0, TMEM_DP = 128, TMEM_DQ = 256;
     extern __shared__ uint8_t smemRaw[];
-    __shared__ __align__(8) uint64_t barFull[SLOTS], barEmpty[SLOTS], barQ, barDO, barS, barSRead, barDP, barDS, barDone, barFix;
+    __shared__ __align__(8) uint64_t barFull[STAGES], barEmpty[STAGES], barQ, barDO, barS, barSRead, barDP, barDS, barDone, barFix;
     __shared__ uint32_t tmemBaseSlot;
     __shared__ int abortFlag;
     __shared__ float sDelta[XT];
@@ -143,9 +143,9 @@ XattnGradQKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         PrefetchTensorMap(&tmDQ);
     }
     if (threadIdx.x == 0) {
-        for (int i = 0; i < SLOTS; i++) {
+        for (int i = 0; i < STAGES; i++) {
             MbarInit(SmemAddr(&barFull[i]), 1);
-            MbarInit(SmemAddr(&barEmpty[i]), 1);
+            MbarInit(SmemAddr(&barEmpty[i]), 2);
         }
         MbarInit(SmemAddr(&barQ), 1);
         MbarInit(SmemAddr(&barDO), 1);
@@ -191,45 +191,35 @@ XattnGradQKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
 #pragma unroll
             for (int dc = 0; dc < DC; dc++)
                 TmaLoad4D(qS + dc * XBOX_BYTES, &tmQ, SmemAddr(&barQ), dc * 64, q0, h * p.aQ.mulHead, b * p.aQ.mulBatch);
-            int slot = 0;
-            uint32_t phase = 0;
-            for (int t = 0; ok && t < 2 * n; t++) {
-                if (t >= SLOTS)
-                    ok = MbarWait(SmemAddr(&barEmpty[slot]), phase ^ 1u, abortPtr, p.status);
+            for (int s = 0; ok && s < n; s++) {
+                if (s >= STAGES)
+                    ok = MbarWait(SmemAddr(&barEmpty[s % STAGES]), (uint32_t)(s / STAGES + 1) & 1u, abortPtr, p.status);
                 if (!ok)
                     break;
-                if (t == 1) {
+                const int row = (tile0 + s) * XT;
+                const uint32_t dst = ringS + (s % STAGES) * 2 * TILE, bar = SmemAddr(&barFull[s % STAGES]);
+                MbarExpectTx(bar, 2 * TILE);
+#pragma unroll
+                for (int dc = 0; dc < DC; dc++)
+                    TmaLoad4D(dst + dc * XBOX_BYTES, &tmK, bar, dc * 64, row, kvHead * p.aK.mulHead, b * p.aK.mulBatch);
+                if (s == 0) {
                     MbarExpectTx(SmemAddr(&barDO), TILE);
 #pragma unroll
                     for (int dc = 0; dc < DC; dc++)
                         TmaLoad4D(doS + dc * XBOX_BYTES, &tmDO, SmemAddr(&barDO), dc * 64, q0, h * p.aDO.mulHead, b * p.aDO.mulBatch);
                 }
-                const int row = (tile0 + (t >> 1)) * XT;
-                const uint32_t dst = ringS + slot * TILE, bar = SmemAddr(&barFull[slot]);
-                MbarExpectTx(bar, TILE);
-                if ((t & 1) == 0) {
 #pragma unroll
-                    for (int dc = 0; dc < DC; dc++)
-                        TmaLoad4D(dst + dc * XBOX_BYTES, &tmK, bar, dc * 64, row, kvHead * p.aK.mulHead, b * p.aK.mulBatch);
-                }
-                else {
-#pragma unroll
-                    for (int dc = 0; dc < DC; dc++)
-                        TmaLoad4D(dst + dc * XBOX_BYTES, &tmV, bar, dc * 64, row, kvHead * p.aV.mulHead, b * p.aV.mulBatch);
-                }
-                if (++slot == SLOTS) {
-                    slot = 0;
-                    phase ^= 1u;
-                }
+                for (int dc = 0; dc < DC; dc++)
+                    TmaLoad4D(dst + TILE + dc * XBOX_BYTES, &tmV, bar, dc * 64, row, kvHead * p.aV.mulHead, b * p.aV.mulBatch);
             }
         }
         __syncwarp();
         if (fix) {
             /* after its load and before the products that read it as rows of the sum; the scores of these keys
                may be taken from either state, their weights are set to 0 */
-            const int t = 2 * n - 2, slot = t % SLOTS;
-            if (MbarWaitWarp(SmemAddr(&barFull[slot]), (uint32_t)(t / SLOTS) & 1u, abortPtr, p.status, 200)) {
-                ZeroTileRows(ringS + slot * TILE, DC, nk - (tile1 - 1) * XT, lane);
+            const int s = n - 1;
+            if (WaitNowWarp(SmemAddr(&barFull[s % STAGES]), (uint32_t)(s / STAGES) & 1u, abortPtr, p.status)) {
+                ZeroTileRows(ringS + (s % STAGES) * 2 * TILE, DC, nk - (tile1 - 1) * XT, lane);
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
                 if (lane == 0)
@@ -237,7 +227,9 @@ XattnGradQKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
             }
         }
     }
-    else if (warp == GR_ISSUER) {
+    else if (warp >= GR_ISSUER) {
+        /* two issuing threads: the scores, and what hangs on the gradients. Behind its own tensor-core instructions a
+           thread sees a barrier only some 300 clocks late; one thread would add up the waits of both chains */
         if (lane == 0 && n > 0) {
             constexpr uint32_t descS = XattnDesc(XT, 0), descQ = XattnDesc(D, 1);
             auto product = [&](uint32_t dst, uint32_t aTile, uint32_t bTile) {
@@ -248,54 +240,49 @@ XattnGradQKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                         TcMma<0>(dst, SmemDesc(aTile + dc * XBOX_BYTES + ks * UMMA_K_BYTES, 16, 1024, 2),
                                  SmemDesc(bTile + dc * XBOX_BYTES + ks * UMMA_K_BYTES, 16, 1024, 2), descS, (dc | ks) != 0 ? 1u : 0u);
             };
-            auto full = [&](int t) { return MbarWait(SmemAddr(&barFull[t % SLOTS]), (uint32_t)(t / SLOTS) & 1u, abortPtr, p.status); };
-            bool ok = MbarWait(SmemAddr(&barQ), 0, abortPtr, p.status) && full(0);
-            if (ok) {
-                TcFenceAfter();
-                product(tmemBase + TMEM_S, qS, ringS);
-                TcCommit(SmemAddr(&barS));
-                ok = MbarWait(SmemAddr(&barDO), 0, abortPtr, p.status) && full(1);
-            }
-            if (ok) {
-                TcFenceAfter();
-                product(tmemBase + TMEM_DP, doS, ringS + TILE);
-                TcCommit(SmemAddr(&barDP));
-                TcCommit(SmemAddr(&barEmpty[1]));
-            }
-            for (int j = 0; ok && j < n; j++) {
-                const int tk = 2 * j;
-                const bool more = j + 1 < n;
-                if (more) {
-                    ok = full(tk + 2) && MbarWait(SmemAddr(&barSRead), (uint32_t)j & 1u, abortPtr, p.status);
+            auto full = [&](int s) { return WaitNow(SmemAddr(&barFull[s % STAGES]), (uint32_t)(s / STAGES) & 1u, abortPtr, p.status); };
+            if (warp == GR_ISSUER) {
+                bool ok = WaitNow(SmemAddr(&barQ), 0, abortPtr, p.status);
+                for (int j = 0; ok && j < n; j++) {
+                    ok = full(j) && (j == 0 || WaitNow(SmemAddr(&barSRead), (uint32_t)(j - 1) & 1u, abortPtr, p.status));
                     if (!ok)
                         break;
                     TcFenceAfter();
-                    product(tmemBase + TMEM_S, qS, ringS + ((tk + 2) % SLOTS) * TILE);
+                    product(tmemBase + TMEM_S, qS, ringS + (j % STAGES) * 2 * TILE);
                     TcCommit(SmemAddr(&barS));
+                    TcCommit(SmemAddr(&barEmpty[j % STAGES]));
                 }
-                if (!more && fix)
-                    ok = MbarWait(SmemAddr(&barFix), 0, abortPtr, p.status);
-                ok = ok && MbarWait(SmemAddr(&barDS), (uint32_t)j & 1u, abortPtr, p.status);
-                if (!ok)
-                    break;
-                TcFenceAfter();
-                const uint32_t kTile = ringS + (tk % SLOTS) * TILE;
-#pragma unroll
-                for (int ks = 0; ks < XT / 16; ks++)
-                    TcMmaTmemA(tmemBase + TMEM_DQ, tmemBase + TMEM_DP + (ks >> 2) * 64 + (ks & 3) * 8,
-                               SmemDesc(kTile + ks * 16 * ROW_BYTES, XBOX_BYTES, 1024, 2), descQ, (j | ks) != 0 ? 1u : 0u);
-                TcCommit(SmemAddr(&barEmpty[tk % SLOTS]));
-                if (more) {
-                    ok = full(tk + 3);
+            }
+            else {
+                bool ok = WaitNow(SmemAddr(&barDO), 0, abortPtr, p.status) && full(0);
+                if (ok) {
+                    TcFenceAfter();
+                    product(tmemBase + TMEM_DP, doS, ringS + TILE);
+                    TcCommit(SmemAddr(&barDP));
+                }
+                for (int j = 0; ok && j < n; j++) {
+                    const bool more = j + 1 < n;
+                    const uint32_t kTile = ringS + (j % STAGES) * 2 * TILE;
+                    if (more)
+                        ok = full(j + 1);
+                    else if (fix)
+                        ok = WaitNow(SmemAddr(&barFix), 0, abortPtr, p.status);
+                    ok = ok && WaitNow(SmemAddr(&barDS), (uint32_t)j & 1u, abortPtr, p.status);
                     if (!ok)
                         break;
                     TcFenceAfter();
-                    product(tmemBase + TMEM_DP, doS, ringS + ((tk + 3) % SLOTS) * TILE);
-                    TcCommit(SmemAddr(&barDP));
-                    TcCommit(SmemAddr(&barEmpty[(tk + 3) % SLOTS]));
+#pragma unroll
+                    for (int ks = 0; ks < XT / 16; ks++)
+                        TcMmaTmemA(tmemBase + TMEM_DQ, tmemBase + TMEM_DP + (ks >> 2) * 64 + (ks & 3) * 8,
+                                   SmemDesc(kTile + ks * 16 * ROW_BYTES, XBOX_BYTES, 1024, 2), descQ, (j | ks) != 0 ? 1u : 0u);
+                    TcCommit(SmemAddr(&barEmpty[j % STAGES]));
+                    if (more) {
+                        product(tmemBase + TMEM_DP, doS, ringS + ((j + 1) % STAGES) * 2 * TILE + TILE);
+                        TcCommit(SmemAddr(&barDP));
+                    }
+                    else
+                        TcCommit(SmemAddr(&barDone));
                 }
-                else
-                    TcCommit(SmemAddr(&barDone));
             }
         }
     }
@@ -342,7 +329,7 @@ XattnGradQKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         bool ok = true;
         for (int j = 0; j < n; j++) {
             const uint32_t ph = (uint32_t)j & 1u;
-            ok = MbarWaitWarp(SmemAddr(&barS), ph, abortPtr, p.status, 200);
+            ok = WaitNowWarp(SmemAddr(&barS), ph, abortPtr, p.status);
             if (!ok)
                 break;
             TcFenceAfter();
@@ -354,7 +341,7 @@ XattnGradQKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
             for (int e = 0; e < 64; e++)
                 x[e] = __float_as_uint(Exp2(fmaf(__uint_as_float(x[e]), p.scaleLog2, -lse2)));
             const int valid = nk - (tile0 + j) * XT - hf * 64;
-            ok = MbarWaitWarp(SmemAddr(&barDP), ph, abortPtr, p.status, 200);
+            ok = WaitNowWarp(SmemAddr(&barDP), ph, abortPtr, p.status);
             if (!ok)
                 break;
             TcFenceAfter();
@@ -378,7 +365,7 @@ XattnGradQKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
             MbarArrive(SmemAddr(&barDS));
         }
         if (n > 0 && ok)
-            ok = MbarWaitWarp(SmemAddr(&barDone), 0, abortPtr, p.status, 200);
+            ok = WaitNowWarp(SmemAddr(&barDone), 0, abortPtr, p.status);
         TcFenceAfter();
         const bool sums = n > 0 && ok;
         const uint32_t dqT = tmemBase + laneBase + TMEM_DQ;
@@ -394,10 +381,10 @@ XattnGradQKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
             else
                 StorePartial(ringS + r * D * 4, r, c * 8, o, sums);
         }
-        if (p.splits == 1 && ok) {
+        if (p.splits == 1) {
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            GradBarrier();
-            if (hf == 0 && lane == 0 && q0 + sub * 32 < p.sh.lenQ) {
+            GradBarrier();                       /* all eight warps come here, whatever became of their waits */
+            if (ok && hf == 0 && lane == 0 && q0 + sub * 32 < p.sh.lenQ) {
 #pragma unroll
                 for (int dc = 0; dc < DC; dc++)
                     TmaStore4D(&tmDQ, qS + dc * XBOX_BYTES + sub * 32 * ROW_BYTES, dc * 64, q0 + sub * 32, h, b);
@@ -469,14 +456,14 @@ XattnGradKVKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     if (threadIdx.x == 0) {
         for (int i = 0; i < STAGES; i++) {
             MbarInit(SmemAddr(&barFull[i]), 1);
-            MbarInit(SmemAddr(&barEmpty[i]), 1);
+            MbarInit(SmemAddr(&barEmpty[i]), 2);
         }
         MbarInit(SmemAddr(&barKV), 1);
         MbarInit(SmemAddr(&barS), 1);
         MbarInit(SmemAddr(&barP), 256);
         MbarInit(SmemAddr(&barDP), 1);
         MbarInit(SmemAddr(&barDS), 256);
-        MbarInit(SmemAddr(&barDone), 1);
+        MbarInit(SmemAddr(&barDone), 2);
         MbarInit(SmemAddr(&barLoad), 1);
         abortFlag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -556,7 +543,8 @@ XattnGradKVKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
             }
         }
     }
-    else if (warp == GR_ISSUER) {
+    else if (warp >= GR_ISSUER) {
+        /* two issuing threads, as above: the scores and dv, the gradients of the weights and dk */
         if (lane == 0 && n > 0) {
             constexpr uint32_t descS = XattnDesc(XT, 0), descD = XattnDesc(D, 1);
             auto product = [&](uint32_t dst, uint32_t aTile, uint32_t bTile) {
@@ -573,41 +561,30 @@ XattnGradKVKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
                     TcMmaTmemA(dst, aTmem + (ks >> 2) * 64 + (ks & 3) * 8, SmemDesc(bTile + ks * 16 * ROW_BYTES, XBOX_BYTES, 1024, 2), descD,
                                !first || ks != 0 ? 1u : 0u);
             };
-            auto full = [&](int i) { return MbarWait(SmemAddr(&barFull[i % STAGES]), (uint32_t)(i / STAGES) & 1u, abortPtr, p.status); };
-            bool ok = MbarWait(SmemAddr(&barKV), 0, abortPtr, p.status) && full(0);
+            auto full = [&](int i) { return WaitNow(SmemAddr(&barFull[i % STAGES]), (uint32_t)(i / STAGES) & 1u, abortPtr, p.status); };
+            const bool first = warp == GR_ISSUER;
+            /* (S, k, q, do) or (dP, v, do, q): the tile of the first product, its operands, the second product's */
+            const uint32_t tileT = tmemBase + (first ? TMEM_S : TMEM_DP), accT = tmemBase + (first ? TMEM_DV : TMEM_DK);
+            const uint32_t aTile = first ? kS : vS, bOff = first ? 0 : TILE, cOff = first ? TILE : 0;
+            const uint32_t barOut = first ? SmemAddr(&barS) : SmemAddr(&barDP), barIn = first ? SmemAddr(&barP) : SmemAddr(&barDS);
+            bool ok = WaitNow(SmemAddr(&barKV), 0, abortPtr, p.status) && full(0);
             if (ok) {
                 TcFenceAfter();
-                product(tmemBase + TMEM_S, kS, ringS);
-                TcCommit(SmemAddr(&barS));
-                product(tmemBase + TMEM_DP, vS, ringS + TILE);
-                TcCommit(SmemAddr(&barDP));
+                product(tileT, aTile, ringS + bOff);
+                TcCommit(barOut);
             }
             for (int i = 0; ok && i < n; i++) {
-                const uint32_t ph = (uint32_t)i & 1u;
                 const uint32_t cur = ringS + (i % STAGES) * STAGE, nxt = ringS + ((i + 1) % STAGES) * STAGE;
                 const bool more = i + 1 < n;
-                ok = MbarWait(SmemAddr(&barP), ph, abortPtr, p.status);
+                ok = (!more || full(i + 1)) && WaitNow(barIn, (uint32_t)i & 1u, abortPtr, p.status);
                 if (!ok)
                     break;
                 TcFenceAfter();
-                second(tmemBase + TMEM_DV, tmemBase + TMEM_S, cur + TILE, i == 0);
-                if (more) {
-                    ok = full(i + 1);
-                    if (!ok)
-                        break;
-                    TcFenceAfter();
-                    product(tmemBase + TMEM_S, kS, nxt);
-                    TcCommit(SmemAddr(&barS));
-                }
-                ok = MbarWait(SmemAddr(&barDS), ph, abortPtr, p.status);
-                if (!ok)
-                    break;
-                TcFenceAfter();
-                second(tmemBase + TMEM_DK, tmemBase + TMEM_DP, cur, i == 0);
+                second(accT, tileT, cur + cOff, i == 0);
                 TcCommit(SmemAddr(&barEmpty[i % STAGES]));
                 if (more) {
-                    product(tmemBase + TMEM_DP, vS, nxt + TILE);
-                    TcCommit(SmemAddr(&barDP));
+                    product(tileT, aTile, nxt + bOff);
+                    TcCommit(barOut);
                 }
                 else
                     TcCommit(SmemAddr(&barDone));
@@ -625,12 +602,11 @@ XattnGradKVKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
             const uint32_t ph = (uint32_t)i & 1u;
             const int st = i % STAGES;
             const float4 * lse4 = statsBase + st * (STAGE / 16) + hf * 16, * delta4 = lse4 + XT / 4;
-            ok = MbarWaitWarp(SmemAddr(&barFull[st]), (uint32_t)(i / STAGES) & 1u, abortPtr, p.status, 200) &&
-                 MbarWaitWarp(SmemAddr(&barS), ph, abortPtr, p.status, 200);
+            /* every lane observes the copy's completion itself before it reads what was copied */
+            ok = WaitNowWarp(SmemAddr(&barFull[st]), (uint32_t)(i / STAGES) & 1u, abortPtr, p.status) &&
+                 WaitNowWarp(SmemAddr(&barS), ph, abortPtr, p.status);
             if (!ok)
                 break;
-            /* every lane observes the copy's completion itself before it reads what was copied */
-            (void)MbarTryWait(SmemAddr(&barFull[st]), (uint32_t)(i / STAGES) & 1u, 0);
             TcFenceAfter();
             uint32_t x[64];
             TmemLoad64U(sT, x);
@@ -653,7 +629,7 @@ XattnGradKVKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
             TmemWaitStore();
             TcFenceBefore();
             MbarArrive(SmemAddr(&barP));
-            ok = MbarWaitWarp(SmemAddr(&barDP), ph, abortPtr, p.status, 200);
+            ok = WaitNowWarp(SmemAddr(&barDP), ph, abortPtr, p.status);
             if (!ok)
                 break;
             TcFenceAfter();
@@ -680,7 +656,7 @@ XattnGradKVKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
             MbarArrive(SmemAddr(&barDS));
         }
         if (n > 0 && ok)
-            ok = MbarWaitWarp(SmemAddr(&barDone), 0, abortPtr, p.status, 200);
+            ok = WaitNowWarp(SmemAddr(&barDone), 0, abortPtr, p.status);
         TcFenceAfter();
         const bool sums = n > 0 && ok, rowLive = k0 + r < nk;
         /* warps 0-3: dv, in the place of v; warps 4-7: dk, in the place of k */
