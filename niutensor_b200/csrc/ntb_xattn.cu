@@ -43,9 +43,12 @@ struct XattnParams {
     int units;                 /* query tiles of one key head: group * tilesPerHead */
     int unitsPerItem;          /* items of one key head: ceil(units / STREAMS) */
     int splits;                /* CTAs of a cluster that share an item's keys */
+    int item0;                 /* first item of this launch */
     float scaleLog2;
     int * status;
 };
+
+constexpr int EVENTS = 4;         /* barriers of a stream's steps, used in turn: more than the ring's tiles run ahead */
 
 template <int D, int STREAMS> struct XattnSmem {
     static constexpr int DC = D / 64;
@@ -55,7 +58,7 @@ template <int D, int STREAMS> struct XattnSmem {
     static constexpr int Q_BYTES = STREAMS * TILE;
     static constexpr int RING_BYTES = SLOTS * TILE;
     static constexpr int TOTAL = Q_BYTES + RING_BYTES + 1024;
-    static constexpr int THREADS = STREAMS * 256 + 64;
+    static constexpr int THREADS = STREAMS == 2 ? 608 : 320;     /* softmax, producer, issuer; relay with two streams */
     static constexpr int TMEM_COLS = STREAMS == 2 ? 512 : 256;
     static_assert(RING_BYTES >= STREAMS * XT * D * 4, "the split's partial sums take the place of the ring");
 };
@@ -96,7 +99,7 @@ XattnKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
     constexpr int DC = SM::DC, TILE = SM::TILE, SLOTS = SM::SLOTS;
     constexpr int TMEM_S = 0, TMEM_O = STREAMS * 128;
     extern __shared__ uint8_t smemRaw[];
-    __shared__ __align__(8) uint64_t barFull[SLOTS], barEmpty[SLOTS], barQ[STREAMS], barS[STREAMS], barP[STREAMS], barO[STREAMS], barFix;
+    __shared__ __align__(8) uint64_t barFull[SLOTS], barDone[STREAMS][EVENTS], barQ[STREAMS], barS[STREAMS], barP[STREAMS], barO[STREAMS], barFix;
     __shared__ uint32_t tmemBaseSlot;
     __shared__ int abortFlag;
     __shared__ float sHalf[STREAMS][XT];                 /* what the two threads of a row tell each other */
@@ -107,7 +110,7 @@ XattnKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
     /* a split item's references and sums, in the place of its queries once those have been read */
     float * sM = (float *)(smemRaw + (smemBase - SmemAddr(smemRaw))), * sL = sM + STREAMS * XT;
     volatile int * abortPtr = &abortFlag;
-    constexpr int PRODUCER = STREAMS * 8, ISSUER = STREAMS * 8 + 1;
+    constexpr int PRODUCER = STREAMS * 8, ISSUER = STREAMS * 8 + 1, RELAY = STREAMS * 8 + 2;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
     if (warp == PRODUCER && lane == 0) {
@@ -119,12 +122,13 @@ XattnKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
     if (threadIdx.x == 0) {
         for (int i = 0; i < SLOTS; i++) {
             MbarInit(SmemAddr(&barFull[i]), 1);
-            MbarInit(SmemAddr(&barEmpty[i]), 1);
         }
         for (int s = 0; s < STREAMS; s++) {
+            for (int i = 0; i < EVENTS; i++)
+                MbarInit(SmemAddr(&barDone[s][i]), 1);
             MbarInit(SmemAddr(&barQ[s]), 1);
             MbarInit(SmemAddr(&barS[s]), 1);
-            MbarInit(SmemAddr(&barP[s]), 256);
+            MbarInit(SmemAddr(&barP[s]), STREAMS == 2 ? 257 : 256);            /* the softmax threads and the relay */
             MbarInit(SmemAddr(&barO[s]), 1);
         }
         MbarInit(SmemAddr(&barFix), 1);
@@ -145,7 +149,7 @@ XattnKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
 
     /* this CTA's item, and its part of the item's keys */
     const int rank = p.splits > 1 ? (int)ClusterRank() : 0;
-    const int item = (int)blockIdx.x / p.splits;
+    const int item = p.item0 + (int)blockIdx.x / p.splits;
     const int headItem = item / p.unitsPerItem;
     const int unit0 = (item - headItem * p.unitsPerItem) * STREAMS;
     const int b = headItem / p.sh.headsKV, kvHead = headItem - b * p.sh.headsKV;
@@ -171,6 +175,13 @@ XattnKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
     /* the last tile reaches past the sequence's keys into rows that exist: their values of v are cleared */
     const bool fix = n > 0 && tile1 * XT > nk && nk < p.sh.lenK;
 
+    /* v of tile j and k of the next have arrived, and the rows of v past the sequence's end are cleared */
+    auto CopiesThere = [&](int j) {
+        const int iv = 2 * j + 1, ik = iv + 1;
+        return MbarWait(SmemAddr(&barFull[iv % SLOTS]), (uint32_t)(iv / SLOTS) & 1u, abortPtr, p.status, 0) &&
+               (j + 1 == n || MbarWait(SmemAddr(&barFull[ik % SLOTS]), (uint32_t)(ik / SLOTS) & 1u, abortPtr, p.status, 0)) &&
+               (!fix || j + 1 < n || MbarWait(SmemAddr(&barFix), 0, abortPtr, p.status, 0));
+    };
     if (warp == PRODUCER) {
         bool ok = true;
         if (lane == 0 && n > 0) {
@@ -186,8 +197,15 @@ XattnKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
             }
             /* tiles in the order of their use: k 0, v 0, k 1, v 1, ... */
             for (int i = 0; ok && i < 2 * n; i++) {
-                if (i >= SLOTS)
-                    ok = MbarWait(SmemAddr(&barEmpty[i % SLOTS]), (uint32_t)(i / SLOTS + 1) & 1u, abortPtr, p.status);
+                /* the slot's last tile, number i - SLOTS (k of tile t or v of tile t - 1), was done with when every stream
+                   had its scores of tile t */
+                if (i >= SLOTS) {
+                    const int t = (i - SLOTS + 1) / 2;
+#pragma unroll
+                    for (int s = 0; s < STREAMS; s++)
+                        if (live[s])
+                            ok = ok && MbarWait(SmemAddr(&barDone[s][t % EVENTS]), (uint32_t)(t / EVENTS) & 1u, abortPtr, p.status);
+                }
                 if (!ok)
                     break;
                 const int row = (tile0 + (i >> 1)) * XT;
@@ -230,8 +248,7 @@ XattnKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
                                  SmemDesc(kTile + dc * XBOX_BYTES + ks * UMMA_K_BYTES, 16, 1024, 2), descS, (dc | ks) != 0 ? 1u : 0u);
                 TcCommit(SmemAddr(&barS[s]));
             };
-            auto full = [&](int i) { return WaitNow(SmemAddr(&barFull[i % SLOTS]), (uint32_t)(i / SLOTS) & 1u, abortPtr, p.status); };
-            bool ok = full(0);
+            bool ok = WaitNow(SmemAddr(&barFull[0]), 0, abortPtr, p.status);
 #pragma unroll
             for (int s = 0; s < STREAMS; s++) {
                 if (!live[s])
@@ -242,14 +259,12 @@ XattnKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
                     scores(s, ringS);
                 }
             }
-            if (ok)
-                TcCommit(SmemAddr(&barEmpty[0]));
             for (int j = 0; ok && j < n; j++) {
                 const int iv = 2 * j + 1, ik = iv + 1;
                 const uint32_t vTile = ringS + (iv % SLOTS) * TILE, kTile = ringS + (ik % SLOTS) * TILE;
-                ok = full(iv) && (j + 1 == n || full(ik));
-                if (ok && fix && j == n - 1)
-                    ok = WaitNow(SmemAddr(&barFix), 0, abortPtr, p.status);
+                /* with a second CTA on the SM the issuing thread has time for these waits (see the relay) */
+                if (STREAMS == 1)
+                    ok = CopiesThere(j);
 #pragma unroll
                 for (int s = 0; s < STREAMS; s++) {
                     if (!ok || !live[s])
@@ -268,10 +283,28 @@ XattnKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
                     else
                         TcCommit(SmemAddr(&barO[s]));
                 }
-                if (ok) {
-                    TcCommit(SmemAddr(&barEmpty[iv % SLOTS]));
-                    if (j + 1 < n)
-                        TcCommit(SmemAddr(&barEmpty[ik % SLOTS]));
+            }
+        }
+    }
+    else if (STREAMS == 2 && warp == RELAY) {
+        /* The issuing thread sets the pace of two long streams: behind its own tensor-core instructions it sees a
+           barrier only some 300 clocks late, and a second commit behind its instructions takes it 400. So it waits for one
+           barrier and commits to one a tile: this thread's arrival says that v of the tile and k of the next are there,
+           and a softmax thread tells the producer what has been read. With the issuing thread doing both itself, a step of
+           both streams at head size 128 took 3770 clocks, 1200 of them in that. */
+        if (lane == 0 && n > 0) {
+            bool ok = true;
+            for (int j = 0; ok && j < n; j++) {
+                ok = CopiesThere(j);
+#pragma unroll
+                for (int s = 0; s < STREAMS; s++) {
+                    if (!live[s])
+                        continue;
+                    /* not before the tile before has been handed over: its arrival would count there */
+                    if (j > 0)
+                        ok = ok && MbarWait(SmemAddr(&barP[s]), (uint32_t)(j - 1) & 1u, abortPtr, p.status, 20);
+                    if (ok)
+                        MbarArrive(SmemAddr(&barP[s]));
                 }
             }
         }
@@ -294,6 +327,9 @@ XattnKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
         if (mine) {
             for (int j = 0; j < n; j++) {
                 ok = WaitNowWarp(SmemAddr(&barS[s]), (uint32_t)j & 1u, abortPtr, p.status) && ok;
+                /* with these scores the products before them are done, too */
+                if ((warp & 7) == 0 && lane == 0)
+                    MbarArrive(SmemAddr(&barDone[s][j % EVENTS]));
                 TcFenceAfter();
                 uint32_t x[64];
                 TmemLoad32Async(sT, x);
@@ -479,13 +515,12 @@ XattnKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
 }
 
 template <int D, int STREAMS>
-int LaunchXattn(const XattnCall & call, const XattnParams & base, int splits, cudaStream_t stream)
+int LaunchXattn(const DeviceCtx & ctx, const XattnCall & call, const XattnParams & base, int splits, cudaStream_t stream)
 {
     XattnParams p = base;
     p.unitsPerItem = (p.units + STREAMS - 1) / STREAMS;
-    p.splits = splits;
-    const long long grid = (long long)p.sh.batch * p.sh.headsKV * p.unitsPerItem * splits;
-    if (grid > 0x7fffffffLL)
+    const long long items = (long long)p.sh.batch * p.sh.headsKV * p.unitsPerItem;
+    if (items * splits > 0x7fffffffLL)
         return NTB_ERR_LIMIT;
     CUtensorMap tmQ, tmK, tmV, tmO;
     HeadsAddr unused;
@@ -503,9 +538,30 @@ int LaunchXattn(const XattnCall & call, const XattnParams & base, int splits, cu
     static SmemOptIn optIn;
     if (!optIn.Ensure((const void *)XattnKernel<D, STREAMS>, SM::TOTAL))
         return NTB_ERR_CUDA;
-    const cudaError_t err = LaunchClusterPdl(XattnKernel<D, STREAMS>, (unsigned)grid, SM::THREADS, SM::TOTAL, splits, stream, tmQ, tmK, tmV, tmO, p);
-    CountLaunch();
-    return (err == cudaSuccess && cudaGetLastError() == cudaSuccess) ? NTB_OK : NTB_ERR_CUDA;
+    /* The items of a last wave that fills at most half of the GPU are split over it, in a launch of their own, when
+       they are long: 512 items of 64 key tiles are 3.46 waves and take 3.5 instead of 4. */
+    const int slots = STREAMS == 2 ? ctx.smCount : 2 * ctx.smCount;
+    const int keyTiles = (p.sh.lenK + XT - 1) / XT;
+    long long rest = items % slots;
+    int restSplits = splits;
+    if (items > slots && splits == 1 && keyTiles >= 24)
+        while (restSplits < 8 && rest * restSplits * 2 <= slots && keyTiles >= restSplits * 8)
+            restSplits *= 2;
+    if (restSplits == splits)
+        rest = 0;
+    for (int part = 0; part < 2; part++) {
+        const long long n = part == 0 ? items - rest : rest;
+        if (n == 0)
+            continue;
+        p.item0 = part == 0 ? 0 : (int)(items - rest);
+        p.splits = part == 0 ? splits : restSplits;
+        const cudaError_t err = LaunchClusterPdl(XattnKernel<D, STREAMS>, (unsigned)(n * p.splits), SM::THREADS, SM::TOTAL, p.splits, stream,
+                                                 tmQ, tmK, tmV, tmO, p);
+        CountLaunch();
+        if (err != cudaSuccess || cudaGetLastError() != cudaSuccess)
+            return NTB_ERR_CUDA;
+    }
+    return NTB_OK;
 }
 
 int DispatchXattn(const DeviceCtx & ctx, const XattnCall & call, cudaStream_t stream)
@@ -538,8 +594,8 @@ int DispatchXattn(const DeviceCtx & ctx, const XattnCall & call, cudaStream_t st
     while (splits < 8 && ((items * splits * 2 <= 2LL * ctx.smCount && keyTiles >= splits * 4) || keyTiles / splits > 1024))
         splits *= 2;
     if (s.dim <= 64)
-        return two ? LaunchXattn<64, 2>(call, p, splits, stream) : LaunchXattn<64, 1>(call, p, splits, stream);
-    return two ? LaunchXattn<128, 2>(call, p, splits, stream) : LaunchXattn<128, 1>(call, p, splits, stream);
+        return two ? LaunchXattn<64, 2>(ctx, call, p, splits, stream) : LaunchXattn<64, 1>(ctx, call, p, splits, stream);
+    return two ? LaunchXattn<128, 2>(ctx, call, p, splits, stream) : LaunchXattn<128, 1>(ctx, call, p, splits, stream);
 }
 
 }
