@@ -128,7 +128,7 @@ XattnKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
                 MbarInit(SmemAddr(&barDone[s][i]), 1);
             MbarInit(SmemAddr(&barQ[s]), 1);
             MbarInit(SmemAddr(&barS[s]), 1);
-            MbarInit(SmemAddr(&barP[s]), STREAMS == 2 ? 257 : 256);            /* the softmax threads and the relay */
+            MbarInit(SmemAddr(&barP[s]), STREAMS == 2 ? 9 : 8);            /* the softmax warps and the relay */
             MbarInit(SmemAddr(&barO[s]), 1);
         }
         MbarInit(SmemAddr(&barFix), 1);
@@ -392,7 +392,7 @@ XattnKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
                 l += la + lb;
                 TmemWaitStore();
                 TcFenceBefore();
-                MbarArrive(SmemAddr(&barP[s]));
+                ArriveWarp(SmemAddr(&barP[s]), lane);
             }
             /* the row's sum from its two halves */
             l = Joint(s, hf, &sHalf[s][r], l, [](float a, float b) { return a + b; });

@@ -83,6 +83,15 @@ __device__ __forceinline__ bool WaitNowWarp(uint32_t bar, uint32_t parity, volat
     }
 }
 
+/* One arrival for a warp whose lanes have ordered what they did to tensor memory (TcFenceBefore): one for every
+   thread would be hundreds of shared-memory operations a tile, against the tensor core's operand reads. */
+__device__ __forceinline__ void ArriveWarp(uint32_t bar, int lane)
+{
+    __syncwarp();
+    if (lane == 0)
+        MbarArrive(bar);
+}
+
 __device__ __forceinline__ void TmaLoad4D(uint32_t dst, const CUtensorMap * map, uint32_t bar, int c0, int c1, int c2, int c3)
 {
     asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes"
@@ -181,6 +190,11 @@ __device__ __forceinline__ uint32_t PackHalf2(float lo, float hi)
 {
     const __half2 h = __floats2half2_rn(lo, hi);
     return *(const uint32_t *)&h;
+}
+
+__device__ __forceinline__ void LoadShared16(uint32_t addr, uint32_t * v)
+{
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(addr) : "memory");
 }
 
 __device__ __forceinline__ void StoreShared16(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d)

@@ -32,19 +32,17 @@ namespace ntb {
 namespace {
 
 constexpr int GR_THREADS = 352;
-constexpr int GR_PRODUCER = 8, GR_ISSUER = 9;      /* and a second issuing warp, 10 */
+constexpr int GR_PRODUCER = 8, GR_ISSUER = 9, GR_RELAY = 10;
+constexpr int GR_EVENTS = 8;       /* barriers of the first kernel's steps, used in turn: more than the ring runs ahead */
 constexpr float P_SCALE_LOG2 = 12.f, P_SCALE_INV = 1.f / 4096.f;
 
 struct XattnGradParams {
     XattnShape sh;
-    HeadsAddr aQ, aK, aV, aDO;
-    const __half * out;
-    const __half * dout;
-    ntb_heads_layout lOut, lDO;
+    HeadsAddr aQ, aK, aV, aO, aDO;
     const float * lse;
     float * work;              /* [batch, headsQ, tilesPerHead][2][128]: lse in the second kernel's units, delta */
     int tilesPerHead, keyTiles;
-    int splits;
+    int splits, item0;         /* of this launch */
     float scale, scaleLog2;
     int * status;
     /* the destinations of the split form */
@@ -56,14 +54,15 @@ struct XattnGradParams {
 template <int D> struct XattnGradSmem {
     static constexpr int DC = D / 64;
     static constexpr int TILE = DC * XBOX_BYTES;
-    /* first kernel: q, do, and a ring of (k, v) */
-    static constexpr int QSTAGES = D == 128 ? 2 : 4;
-    static constexpr int Q_TOTAL = (2 + 2 * QSTAGES) * TILE + 1024;
-    /* second kernel: k, v, and a ring of (q, do, lse and delta) */
-    static constexpr int STAGE = 2 * TILE + 1024;
-    static constexpr int STAGES = D == 128 ? 2 : 4;
-    static constexpr int KV_TOTAL = 2 * TILE + STAGES * STAGE + 1024;
-    static_assert(QSTAGES * 2 * TILE >= XT * D * 4 && STAGES * STAGE >= 2 * XT * D * 4, "the split's partial sums take the place of the ring");
+    /* first kernel: a ring of k and v tiles (q and do are in tensor memory) */
+    static constexpr int SLOTS = 7;
+    static constexpr int Q_TOTAL = SLOTS * TILE + 1024;
+    /* second kernel: k, v, rings of q, of do, and of the query rows' (lse, delta); barriers */
+    static constexpr int QSLOTS = 3, DOSLOTS = 2, STATSLOTS = 2, STAT = 2 * XT * 4;
+    static constexpr int KV_RING = 2 * TILE, KV_STATS = KV_RING + (QSLOTS + DOSLOTS) * TILE, KV_BARS = KV_STATS + STATSLOTS * STAT;
+    static constexpr int KV_TOTAL = KV_BARS + 256;
+    static_assert(SLOTS * TILE >= XT * D * 4 && (QSLOTS + DOSLOTS) * TILE >= 2 * XT * D * 4, "the split's partial sums take the place of the rings");
+    static_assert(KV_TOTAL <= 232448, "shared memory of a CTA");
 };
 
 __device__ __forceinline__ void GradBarrier() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
@@ -117,13 +116,15 @@ __device__ __forceinline__ void StageHalf32(uint32_t rowAddr, int lane, int chun
 template <int D>
 __global__ void __launch_bounds__(GR_THREADS, 1)
 XattnGradQKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
-                 const __grid_constant__ CUtensorMap tmDO, const __grid_constant__ CUtensorMap tmDQ, const XattnGradParams p)
+                 const __grid_constant__ CUtensorMap tmO, const __grid_constant__ CUtensorMap tmDO, const __grid_constant__ CUtensorMap tmDQ,
+                 const XattnGradParams p)
 {
     using SM = XattnGradSmem<D>;
-    constexpr int DC = SM::DC, TILE = SM::TILE, STAGES = SM::QSTAGES;
-    constexpr int TMEM_S = 0, TMEM_DP = 128, TMEM_DQ = 256;
+    constexpr int DC = SM::DC, TILE = SM::TILE, SLOTS = SM::SLOTS;
+    constexpr int TMEM_S = 0, TMEM_DP = 128, TMEM_DQ = 256, TMEM_Q = 256 + D, TMEM_DO = TMEM_Q + D / 2;
+    constexpr int ROWS0 = SLOTS - 3;                         /* slots of the rows of q, do and out before the ring needs them */
     extern __shared__ uint8_t smemRaw[];
-    __shared__ __align__(8) uint64_t barFull[STAGES], barEmpty[STAGES], barQ, barDO, barS, barSRead, barDP, barDS, barDone, barFix;
+    __shared__ __align__(8) uint64_t barFull[SLOTS], barEvent[GR_EVENTS], barRows, barQ, barS, barSRead, barDP, barDS, barDone, barFix;
     __shared__ uint32_t tmemBaseSlot;
     __shared__ int abortFlag;
     __shared__ float sDelta[XT];
@@ -131,28 +132,29 @@ XattnGradQKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
     const int warp = threadIdx.x >> 5;
     const int lane = threadIdx.x & 31;
     const uint32_t smemBase = (SmemAddr(smemRaw) + 1023u) & ~1023u;
-    const uint32_t qS = smemBase, doS = qS + TILE, ringS = doS + TILE;
+    const uint32_t ringS = smemBase, outS = ringS;          /* dq is staged where the ring was */
     volatile int * abortPtr = &abortFlag;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
     if (warp == GR_PRODUCER && lane == 0) {
         PrefetchTensorMap(&tmQ);
+        PrefetchTensorMap(&tmO);
+        PrefetchTensorMap(&tmDO);
         PrefetchTensorMap(&tmK);
         PrefetchTensorMap(&tmV);
-        PrefetchTensorMap(&tmDO);
         PrefetchTensorMap(&tmDQ);
     }
     if (threadIdx.x == 0) {
-        for (int i = 0; i < STAGES; i++) {
+        for (int i = 0; i < SLOTS; i++)
             MbarInit(SmemAddr(&barFull[i]), 1);
-            MbarInit(SmemAddr(&barEmpty[i]), 2);
-        }
-        MbarInit(SmemAddr(&barQ), 1);
-        MbarInit(SmemAddr(&barDO), 1);
+        for (int i = 0; i < GR_EVENTS; i++)
+            MbarInit(SmemAddr(&barEvent[i]), 1);
+        MbarInit(SmemAddr(&barRows), 1);
+        MbarInit(SmemAddr(&barQ), 8);
         MbarInit(SmemAddr(&barS), 1);
-        MbarInit(SmemAddr(&barSRead), 256);
+        MbarInit(SmemAddr(&barSRead), 9);                  /* the softmax warps and the relay */
         MbarInit(SmemAddr(&barDP), 1);
-        MbarInit(SmemAddr(&barDS), 256);
+        MbarInit(SmemAddr(&barDS), 9);
         MbarInit(SmemAddr(&barDone), 1);
         MbarInit(SmemAddr(&barFix), 1);
         abortFlag = 0;
@@ -171,7 +173,7 @@ XattnGradQKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
     asm volatile("griddepcontrol.wait;" ::: "memory");
 
     const int rank = p.splits > 1 ? (int)ClusterRank() : 0;
-    const int item = (int)blockIdx.x / p.splits;
+    const int item = p.item0 + (int)blockIdx.x / p.splits;
     const int headItem = item / p.tilesPerHead;
     const int q0 = (item - headItem * p.tilesPerHead) * XT;
     const int b = headItem / p.sh.headsQ, h = headItem - b * p.sh.headsQ, kvHead = h / p.sh.group;
@@ -187,39 +189,47 @@ XattnGradQKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
     if (warp == GR_PRODUCER) {
         if (lane == 0 && n > 0) {
             bool ok = true;
-            MbarExpectTx(SmemAddr(&barQ), TILE);
+            /* tiles in the order of their use: k 0, v 0, k 1, v 1, ... The last three slots first hold this item's rows of
+               q, do and out, on their way to tensor memory. */
+            MbarExpectTx(SmemAddr(&barRows), 3 * TILE);
 #pragma unroll
-            for (int dc = 0; dc < DC; dc++)
-                TmaLoad4D(qS + dc * XBOX_BYTES, &tmQ, SmemAddr(&barQ), dc * 64, q0, h * p.aQ.mulHead, b * p.aQ.mulBatch);
-            for (int s = 0; ok && s < n; s++) {
-                if (s >= STAGES)
-                    ok = MbarWait(SmemAddr(&barEmpty[s % STAGES]), (uint32_t)(s / STAGES + 1) & 1u, abortPtr, p.status);
+            for (int dc = 0; dc < DC; dc++) {
+                TmaLoad4D(ringS + ROWS0 * TILE + dc * XBOX_BYTES, &tmQ, SmemAddr(&barRows), dc * 64, q0, h * p.aQ.mulHead, b * p.aQ.mulBatch);
+                TmaLoad4D(ringS + (ROWS0 + 1) * TILE + dc * XBOX_BYTES, &tmDO, SmemAddr(&barRows), dc * 64, q0, h * p.aDO.mulHead, b * p.aDO.mulBatch);
+                TmaLoad4D(ringS + (ROWS0 + 2) * TILE + dc * XBOX_BYTES, &tmO, SmemAddr(&barRows), dc * 64, q0, h * p.aO.mulHead, b * p.aO.mulBatch);
+            }
+            for (int i = 0; ok && i < 2 * n; i++) {
+                if (i == ROWS0)
+                    ok = MbarWait(SmemAddr(&barQ), 0, abortPtr, p.status);
+                if (i >= SLOTS) {
+                    /* v t was done with when its product was, k t when the next tile's was */
+                    const int old = i - SLOTS, event = (old & 1) ? old / 2 : old / 2 + 1;
+                    ok = MbarWait(SmemAddr(&barEvent[event % GR_EVENTS]), (uint32_t)(event / GR_EVENTS) & 1u, abortPtr, p.status);
+                }
                 if (!ok)
                     break;
-                const int row = (tile0 + s) * XT;
-                const uint32_t dst = ringS + (s % STAGES) * 2 * TILE, bar = SmemAddr(&barFull[s % STAGES]);
-                MbarExpectTx(bar, 2 * TILE);
-#pragma unroll
-                for (int dc = 0; dc < DC; dc++)
-                    TmaLoad4D(dst + dc * XBOX_BYTES, &tmK, bar, dc * 64, row, kvHead * p.aK.mulHead, b * p.aK.mulBatch);
-                if (s == 0) {
-                    MbarExpectTx(SmemAddr(&barDO), TILE);
+                const int row = (tile0 + (i >> 1)) * XT;
+                const uint32_t dst = ringS + (i % SLOTS) * TILE, bar = SmemAddr(&barFull[i % SLOTS]);
+                MbarExpectTx(bar, TILE);
+                if ((i & 1) == 0) {
 #pragma unroll
                     for (int dc = 0; dc < DC; dc++)
-                        TmaLoad4D(doS + dc * XBOX_BYTES, &tmDO, SmemAddr(&barDO), dc * 64, q0, h * p.aDO.mulHead, b * p.aDO.mulBatch);
+                        TmaLoad4D(dst + dc * XBOX_BYTES, &tmK, bar, dc * 64, row, kvHead * p.aK.mulHead, b * p.aK.mulBatch);
                 }
+                else {
 #pragma unroll
-                for (int dc = 0; dc < DC; dc++)
-                    TmaLoad4D(dst + TILE + dc * XBOX_BYTES, &tmV, bar, dc * 64, row, kvHead * p.aV.mulHead, b * p.aV.mulBatch);
+                    for (int dc = 0; dc < DC; dc++)
+                        TmaLoad4D(dst + dc * XBOX_BYTES, &tmV, bar, dc * 64, row, kvHead * p.aV.mulHead, b * p.aV.mulBatch);
+                }
             }
         }
         __syncwarp();
         if (fix) {
             /* after its load and before the products that read it as rows of the sum; the scores of these keys
                may be taken from either state, their weights are set to 0 */
-            const int s = n - 1;
-            if (WaitNowWarp(SmemAddr(&barFull[s % STAGES]), (uint32_t)(s / STAGES) & 1u, abortPtr, p.status)) {
-                ZeroTileRows(ringS + (s % STAGES) * 2 * TILE, DC, nk - (tile1 - 1) * XT, lane);
+            const int i = 2 * n - 2;
+            if (WaitNowWarp(SmemAddr(&barFull[i % SLOTS]), (uint32_t)(i / SLOTS) & 1u, abortPtr, p.status)) {
+                ZeroTileRows(ringS + (i % SLOTS) * TILE, DC, nk - (tile1 - 1) * XT, lane);
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
                 if (lane == 0)
@@ -227,62 +237,77 @@ XattnGradQKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
             }
         }
     }
-    else if (warp >= GR_ISSUER) {
-        /* two issuing threads: the scores, and what hangs on the gradients. Behind its own tensor-core instructions a
-           thread sees a barrier only some 300 clocks late; one thread would add up the waits of both chains */
+    else if (warp == GR_ISSUER) {
         if (lane == 0 && n > 0) {
             constexpr uint32_t descS = XattnDesc(XT, 0), descQ = XattnDesc(D, 1);
-            auto product = [&](uint32_t dst, uint32_t aTile, uint32_t bTile) {
+            auto product = [&](uint32_t dst, uint32_t aTmem, uint32_t bTile) {
 #pragma unroll
-                for (int dc = 0; dc < DC; dc++)
-#pragma unroll
-                    for (int ks = 0; ks < 4; ks++)
-                        TcMma<0>(dst, SmemDesc(aTile + dc * XBOX_BYTES + ks * UMMA_K_BYTES, 16, 1024, 2),
-                                 SmemDesc(bTile + dc * XBOX_BYTES + ks * UMMA_K_BYTES, 16, 1024, 2), descS, (dc | ks) != 0 ? 1u : 0u);
+                for (int ks = 0; ks < D / 16; ks++)
+                    TcMmaTmemA(dst, aTmem + ks * 8, SmemDesc(bTile + (ks >> 2) * XBOX_BYTES + (ks & 3) * UMMA_K_BYTES, 16, 1024, 2), descS,
+                               ks != 0 ? 1u : 0u);
             };
-            auto full = [&](int s) { return WaitNow(SmemAddr(&barFull[s % STAGES]), (uint32_t)(s / STAGES) & 1u, abortPtr, p.status); };
-            if (warp == GR_ISSUER) {
-                bool ok = WaitNow(SmemAddr(&barQ), 0, abortPtr, p.status);
-                for (int j = 0; ok && j < n; j++) {
-                    ok = full(j) && (j == 0 || WaitNow(SmemAddr(&barSRead), (uint32_t)(j - 1) & 1u, abortPtr, p.status));
+            bool ok = WaitNow(SmemAddr(&barQ), 0, abortPtr, p.status) && WaitNow(SmemAddr(&barFull[0]), 0, abortPtr, p.status);
+            if (ok) {
+                TcFenceAfter();
+                product(tmemBase + TMEM_S, tmemBase + TMEM_Q, ringS);
+                TcCommit(SmemAddr(&barS));
+                ok = WaitNow(SmemAddr(&barFull[1]), 0, abortPtr, p.status);
+            }
+            if (ok) {
+                TcFenceAfter();
+                product(tmemBase + TMEM_DP, tmemBase + TMEM_DO, ringS + TILE);
+                TcCommit(SmemAddr(&barDP));
+            }
+            for (int j = 0; ok && j < n; j++) {
+                const bool more = j + 1 < n;
+                if (more) {
+                    /* the scores are in registers: the next ones, under the exponentials of these */
+                    ok = WaitNow(SmemAddr(&barSRead), (uint32_t)j & 1u, abortPtr, p.status);
                     if (!ok)
                         break;
                     TcFenceAfter();
-                    product(tmemBase + TMEM_S, qS, ringS + (j % STAGES) * 2 * TILE);
+                    product(tmemBase + TMEM_S, tmemBase + TMEM_Q, ringS + ((2 * j + 2) % SLOTS) * TILE);
                     TcCommit(SmemAddr(&barS));
-                    TcCommit(SmemAddr(&barEmpty[j % STAGES]));
                 }
-            }
-            else {
-                bool ok = WaitNow(SmemAddr(&barDO), 0, abortPtr, p.status) && full(0);
-                if (ok) {
-                    TcFenceAfter();
-                    product(tmemBase + TMEM_DP, doS, ringS + TILE);
+                ok = WaitNow(SmemAddr(&barDS), (uint32_t)j & 1u, abortPtr, p.status);
+                if (!ok)
+                    break;
+                TcFenceAfter();
+#pragma unroll
+                for (int ks = 0; ks < XT / 16; ks++)
+                    TcMmaTmemA(tmemBase + TMEM_DQ, tmemBase + TMEM_DP + (ks >> 2) * 64 + (ks & 3) * 8,
+                               SmemDesc(ringS + ((2 * j) % SLOTS) * TILE + ks * 16 * ROW_BYTES, XBOX_BYTES, 1024, 2), descQ, (j | ks) != 0 ? 1u : 0u);
+                if (more) {
+                    product(tmemBase + TMEM_DP, tmemBase + TMEM_DO, ringS + ((2 * j + 3) % SLOTS) * TILE);
                     TcCommit(SmemAddr(&barDP));
                 }
-                for (int j = 0; ok && j < n; j++) {
-                    const bool more = j + 1 < n;
-                    const uint32_t kTile = ringS + (j % STAGES) * 2 * TILE;
-                    if (more)
-                        ok = full(j + 1);
-                    else if (fix)
-                        ok = WaitNow(SmemAddr(&barFix), 0, abortPtr, p.status);
-                    ok = ok && WaitNow(SmemAddr(&barDS), (uint32_t)j & 1u, abortPtr, p.status);
-                    if (!ok)
-                        break;
-                    TcFenceAfter();
-#pragma unroll
-                    for (int ks = 0; ks < XT / 16; ks++)
-                        TcMmaTmemA(tmemBase + TMEM_DQ, tmemBase + TMEM_DP + (ks >> 2) * 64 + (ks & 3) * 8,
-                                   SmemDesc(kTile + ks * 16 * ROW_BYTES, XBOX_BYTES, 1024, 2), descQ, (j | ks) != 0 ? 1u : 0u);
-                    TcCommit(SmemAddr(&barEmpty[j % STAGES]));
-                    if (more) {
-                        product(tmemBase + TMEM_DP, doS, ringS + ((j + 1) % STAGES) * 2 * TILE + TILE);
-                        TcCommit(SmemAddr(&barDP));
-                    }
-                    else
-                        TcCommit(SmemAddr(&barDone));
+                else
+                    TcCommit(SmemAddr(&barDone));
+            }
+        }
+    }
+    else if (warp == GR_RELAY) {
+        /* Behind its own tensor-core instructions a thread sees a barrier only some 300 clocks late, so the issuing
+           thread waits for the softmax threads alone: this thread's arrivals among theirs say that the copies for the
+           products that follow are there (and, at the end, that the rows of k past the sequence are cleared). */
+        if (lane == 0 && n > 0) {
+            bool ok = true;
+            for (int j = 0; ok && j < n; j++) {
+                const int ik = 2 * j + 2, iv = 2 * j + 3;
+                if (j + 1 < n) {
+                    /* not before the phase before is complete: the arrival would count there */
+                    ok = WaitNow(SmemAddr(&barFull[ik % SLOTS]), (uint32_t)(ik / SLOTS) & 1u, abortPtr, p.status) &&
+                         (j == 0 || WaitNow(SmemAddr(&barSRead), (uint32_t)(j - 1) & 1u, abortPtr, p.status));
+                    if (ok)
+                        MbarArrive(SmemAddr(&barSRead));
+                    ok = ok && WaitNow(SmemAddr(&barFull[iv % SLOTS]), (uint32_t)(iv / SLOTS) & 1u, abortPtr, p.status);
                 }
+                else if (fix)
+                    ok = WaitNow(SmemAddr(&barFix), 0, abortPtr, p.status);
+                if (ok && j > 0)
+                    ok = WaitNow(SmemAddr(&barDS), (uint32_t)(j - 1) & 1u, abortPtr, p.status);
+                if (ok)
+                    MbarArrive(SmemAddr(&barDS));
             }
         }
     }
@@ -291,26 +316,37 @@ XattnGradQKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         const uint32_t laneBase = (uint32_t)(sub * 32) << 16;
         const int r = sub * 32 + lane, row = q0 + r;
         const bool rowLive = row < nq && nk > 0;
-        /* delta, half of the row a thread, joined through shared memory */
+        /* q and do go to tensor memory as the A operands of the first products (from shared memory those would
+           read two operands, at the rate all of shared memory has), half of a row a thread; delta on the way,
+           joined through shared memory */
         float part = 0.f;
-        if (rowLive) {
-            const __half * o = p.out + b * p.lOut.batch + h * p.lOut.head + row * p.lOut.row;
-            const __half * g = p.dout + b * p.lDO.batch + h * p.lDO.head + row * p.lDO.row;
+        bool ok = true;
+        if (n > 0) {
+            ok = WaitNowWarp(SmemAddr(&barRows), 0, abortPtr, p.status);
 #pragma unroll
             for (int c = 0; c < D / 16; c++) {
                 const int col = hf * (D / 2) + c * 8;
-                if (col < p.sh.dim) {
-                    const uint4 x = *(const uint4 *)(o + col), y = *(const uint4 *)(g + col);
-                    const uint32_t xs[4] = { x.x, x.y, x.z, x.w }, ys[4] = { y.x, y.y, y.z, y.w };
+                const uint32_t at = ringS + ROWS0 * TILE + (col >> 6) * XBOX_BYTES + r * ROW_BYTES + ((((col >> 3) & 7) ^ (r & 7)) << 4);
+                uint32_t xs[4], ys[4], zs[4];
+                LoadShared16(at, zs);
+                LoadShared16(at + TILE, ys);
+                LoadShared16(at + 2 * TILE, xs);
 #pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        const float2 xf = __half22float2(*(const __half2 *)&xs[e]), yf = __half22float2(*(const __half2 *)&ys[e]);
-                        part = fmaf(xf.x, yf.x, part);
-                        part = fmaf(xf.y, yf.y, part);
-                    }
+                for (int e = 0; e < 4; e++) {
+                    const float2 xf = __half22float2(*(const __half2 *)&xs[e]), yf = __half22float2(*(const __half2 *)&ys[e]);
+                    part = fmaf(xf.x, yf.x, part);
+                    part = fmaf(xf.y, yf.y, part);
                 }
+                TmemStore4Async(tmemBase + laneBase + TMEM_DO + col / 2, ys);
+                TmemStore4Async(tmemBase + laneBase + TMEM_Q + col / 2, zs);
             }
+            TmemWaitStore();
+            TcFenceBefore();
+            ArriveWarp(SmemAddr(&barQ), lane);
         }
+        /* rows past the sequence hold anything; they are no part of any other row's sums here */
+        if (!rowLive)
+            part = 0.f;
         if (hf == 1)
             sDelta[r] = part;
         GradBarrier();
@@ -326,8 +362,7 @@ XattnGradQKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
             w[XT + r] = delta * P_SCALE_INV;
         }
         const uint32_t sT = tmemBase + laneBase + TMEM_S + hf * 64, dpT = tmemBase + laneBase + TMEM_DP + hf * 64;
-        bool ok = true;
-        for (int j = 0; j < n; j++) {
+        for (int j = 0; ok && j < n; j++) {
             const uint32_t ph = (uint32_t)j & 1u;
             ok = WaitNowWarp(SmemAddr(&barS), ph, abortPtr, p.status);
             if (!ok)
@@ -336,7 +371,7 @@ XattnGradQKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
             uint32_t x[64];
             TmemLoad64U(sT, x);
             TcFenceBefore();
-            MbarArrive(SmemAddr(&barSRead));
+            ArriveWarp(SmemAddr(&barSRead), lane);
 #pragma unroll
             for (int e = 0; e < 64; e++)
                 x[e] = __float_as_uint(Exp2(fmaf(__uint_as_float(x[e]), p.scaleLog2, -lse2)));
@@ -344,6 +379,9 @@ XattnGradQKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
             ok = WaitNowWarp(SmemAddr(&barDP), ph, abortPtr, p.status);
             if (!ok)
                 break;
+            /* v of this tile and k of the one before have been read */
+            if (threadIdx.x == 0)
+                MbarArrive(SmemAddr(&barEvent[j % GR_EVENTS]));
             TcFenceAfter();
 #pragma unroll
             for (int c = 0; c < 2; c++) {
@@ -362,7 +400,7 @@ XattnGradQKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
             }
             TmemWaitStore();
             TcFenceBefore();
-            MbarArrive(SmemAddr(&barDS));
+            ArriveWarp(SmemAddr(&barDS), lane);
         }
         if (n > 0 && ok)
             ok = WaitNowWarp(SmemAddr(&barDone), 0, abortPtr, p.status);
@@ -377,7 +415,7 @@ XattnGradQKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                 TmemWaitLoad();
             }
             if (p.splits == 1)
-                StageHalf32(qS + (c >> 1) * XBOX_BYTES + r * ROW_BYTES, lane, (c & 1) * 4, o, p.scale, sums && rowLive);
+                StageHalf32(outS + (c >> 1) * XBOX_BYTES + r * ROW_BYTES, lane, (c & 1) * 4, o, p.scale, sums && rowLive);
             else
                 StorePartial(ringS + r * D * 4, r, c * 8, o, sums);
         }
@@ -387,7 +425,7 @@ XattnGradQKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
             if (ok && hf == 0 && lane == 0 && q0 + sub * 32 < p.sh.lenQ) {
 #pragma unroll
                 for (int dc = 0; dc < DC; dc++)
-                    TmaStore4D(&tmDQ, qS + dc * XBOX_BYTES + sub * 32 * ROW_BYTES, dc * 64, q0 + sub * 32, h, b);
+                    TmaStore4D(&tmDQ, outS + dc * XBOX_BYTES + sub * 32 * ROW_BYTES, dc * 64, q0 + sub * 32, h, b);
                 asm volatile("cp.async.bulk.commit_group;" ::: "memory");
                 asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
             }
@@ -431,18 +469,24 @@ XattnGradKVKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
                   const XattnGradParams p)
 {
     using SM = XattnGradSmem<D>;
-    constexpr int DC = SM::DC, TILE = SM::TILE, STAGES = SM::STAGES, STAGE = SM::STAGE;
+    constexpr int DC = SM::DC, TILE = SM::TILE, QSLOTS = SM::QSLOTS, DOSLOTS = SM::DOSLOTS, STATSLOTS = SM::STATSLOTS;
     constexpr int TMEM_S = 0, TMEM_DP = 128, TMEM_DV = 256, TMEM_DK = 256 + D;
-    extern __shared__ uint8_t smemRaw[];
-    __shared__ __align__(8) uint64_t barFull[STAGES], barEmpty[STAGES], barKV, barLoad, barS, barP, barDP, barDS, barDone;
-    __shared__ uint32_t tmemBaseSlot;
-    __shared__ int abortFlag;
+    /* everything in one region, on a swizzle boundary by its alignment: there is no room to move it up */
+    extern __shared__ __align__(1024) uint8_t kvSmem[];
+    struct Bars {
+        uint64_t qFull[QSLOTS], qEmpty[QSLOTS], doFull[DOSLOTS], doEmpty[DOSLOTS], statFull[STATSLOTS], statEmpty[STATSLOTS];
+        uint64_t kv, load, s, p, dp, ds, done;
+        uint32_t tmem;
+        int abort;
+    };
+    static_assert(sizeof(Bars) <= 256, "place of the barriers");
+    Bars & bars = *(Bars *)(kvSmem + SM::KV_BARS);
 
     const int warp = threadIdx.x >> 5;
     const int lane = threadIdx.x & 31;
-    const uint32_t smemBase = (SmemAddr(smemRaw) + 1023u) & ~1023u;
-    const uint32_t kS = smemBase, vS = kS + TILE, ringS = vS + TILE;
-    volatile int * abortPtr = &abortFlag;
+    const uint32_t smemBase = SmemAddr(kvSmem);
+    const uint32_t kS = smemBase, vS = kS + TILE, ringS = vS + TILE, doRing = ringS + QSLOTS * TILE, statRing = smemBase + SM::KV_STATS;
+    volatile int * abortPtr = &bars.abort;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
     if (warp == GR_PRODUCER && lane == 0) {
@@ -454,34 +498,42 @@ XattnGradKVKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         PrefetchTensorMap(&tmDV);
     }
     if (threadIdx.x == 0) {
-        for (int i = 0; i < STAGES; i++) {
-            MbarInit(SmemAddr(&barFull[i]), 1);
-            MbarInit(SmemAddr(&barEmpty[i]), 2);
+        for (int i = 0; i < QSLOTS; i++) {
+            MbarInit(SmemAddr(&bars.qFull[i]), 1);
+            MbarInit(SmemAddr(&bars.qEmpty[i]), 1);
         }
-        MbarInit(SmemAddr(&barKV), 1);
-        MbarInit(SmemAddr(&barS), 1);
-        MbarInit(SmemAddr(&barP), 256);
-        MbarInit(SmemAddr(&barDP), 1);
-        MbarInit(SmemAddr(&barDS), 256);
-        MbarInit(SmemAddr(&barDone), 2);
-        MbarInit(SmemAddr(&barLoad), 1);
-        abortFlag = 0;
+        for (int i = 0; i < DOSLOTS; i++) {
+            MbarInit(SmemAddr(&bars.doFull[i]), 1);
+            MbarInit(SmemAddr(&bars.doEmpty[i]), 1);
+        }
+        for (int i = 0; i < STATSLOTS; i++) {
+            MbarInit(SmemAddr(&bars.statFull[i]), 1);
+            MbarInit(SmemAddr(&bars.statEmpty[i]), 1);
+        }
+        MbarInit(SmemAddr(&bars.kv), 1);
+        MbarInit(SmemAddr(&bars.load), 1);
+        MbarInit(SmemAddr(&bars.s), 1);
+        MbarInit(SmemAddr(&bars.p), 9);                    /* the softmax warps and the relay */
+        MbarInit(SmemAddr(&bars.dp), 1);
+        MbarInit(SmemAddr(&bars.ds), 9);
+        MbarInit(SmemAddr(&bars.done), 1);
+        bars.abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
     if (warp == GR_ISSUER) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
-                     :: "r"(SmemAddr(&tmemBaseSlot)), "r"(512u) : "memory");
+                     :: "r"(SmemAddr(&bars.tmem)), "r"(512u) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
     TcFenceBefore();
     __syncthreads();
     TcFenceAfter();
-    const uint32_t tmemBase = *(volatile uint32_t *)&tmemBaseSlot;
+    const uint32_t tmemBase = *(volatile uint32_t *)&bars.tmem;
     asm volatile("griddepcontrol.wait;" ::: "memory");
 
     const int rank = p.splits > 1 ? (int)ClusterRank() : 0;
-    const int item = (int)blockIdx.x / p.splits;
+    const int item = p.item0 + (int)blockIdx.x / p.splits;
     const int headItem = item / p.keyTiles;
     const int k0 = (item - headItem * p.keyTiles) * XT;
     const int b = headItem / p.sh.headsKV, kvHead = headItem - b * p.sh.headsKV;
@@ -498,53 +550,78 @@ XattnGradKVKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         bool ok = true;
         uint32_t edges = 0;
         if (n > 0 && lane == 0) {
-            MbarExpectTx(SmemAddr(&barKV), 2 * TILE);
+            MbarExpectTx(SmemAddr(&bars.kv), 2 * TILE);
 #pragma unroll
             for (int dc = 0; dc < DC; dc++) {
-                TmaLoad4D(kS + dc * XBOX_BYTES, &tmK, SmemAddr(&barKV), dc * 64, k0, kvHead * p.aK.mulHead, b * p.aK.mulBatch);
-                TmaLoad4D(vS + dc * XBOX_BYTES, &tmV, SmemAddr(&barKV), dc * 64, k0, kvHead * p.aV.mulHead, b * p.aV.mulBatch);
+                TmaLoad4D(kS + dc * XBOX_BYTES, &tmK, SmemAddr(&bars.kv), dc * 64, k0, kvHead * p.aK.mulHead, b * p.aK.mulBatch);
+                TmaLoad4D(vS + dc * XBOX_BYTES, &tmV, SmemAddr(&bars.kv), dc * 64, k0, kvHead * p.aV.mulHead, b * p.aV.mulBatch);
             }
         }
-        for (int i = 0; ok && i < n; i++) {
-            const int st = i % STAGES, step = step0 + i;
-            const int g = step / qTiles, qt = step - g * qTiles, h = kvHead * p.sh.group + g;
-            /* a tile with rows past the sequence arrives on the producer's own barrier and is handed on by the warp */
+        /* one tile of q or do into its ring; a tile with rows past the sequence arrives on the producer's own barrier,
+           has them cleared (their weights are 0, and 0 * NaN would reach the sums), and is handed on by the warp */
+        auto load = [&](const CUtensorMap * map, const HeadsAddr & a, int i, uint32_t dst, uint32_t full) {
+            const int step = step0 + i, g = step / qTiles, qt = step - g * qTiles, h = kvHead * p.sh.group + g;
             const bool edge = ragged && qt == qTiles - 1;
-            const uint32_t dst = ringS + st * STAGE, bar = edge ? SmemAddr(&barLoad) : SmemAddr(&barFull[st]);
-            if (i >= STAGES)
-                ok = MbarWaitWarp(SmemAddr(&barEmpty[st]), (uint32_t)(i / STAGES + 1) & 1u, abortPtr, p.status, 200);
-            if (!ok)
-                break;
+            const uint32_t bar = edge ? SmemAddr(&bars.load) : full;
             if (lane == 0) {
-                MbarExpectTx(bar, 2 * TILE + 2 * XT * 4);
+                MbarExpectTx(bar, TILE);
 #pragma unroll
                 for (int dc = 0; dc < DC; dc++)
-                    TmaLoad4D(dst + dc * XBOX_BYTES, &tmQ, bar, dc * 64, qt * XT, h * p.aQ.mulHead, b * p.aQ.mulBatch);
-#pragma unroll
-                for (int dc = 0; dc < DC; dc++)
-                    TmaLoad4D(dst + TILE + dc * XBOX_BYTES, &tmDO, bar, dc * 64, qt * XT, h * p.aDO.mulHead, b * p.aDO.mulBatch);
-                const float * src = p.work + (((long long)b * p.sh.headsQ + h) * p.tilesPerHead + qt) * (2 * XT);
-                asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
-                             :: "r"(dst + 2 * TILE), "l"(src), "r"(2u * XT * 4u), "r"(bar) : "memory");
+                    TmaLoad4D(dst + dc * XBOX_BYTES, map, bar, dc * 64, qt * XT, h * a.mulHead, b * a.mulBatch);
             }
             __syncwarp();
             if (edge) {
-                /* rows of q and do past the sequence: their weights are 0, and 0 * NaN would reach the sums */
-                ok = MbarWaitWarp(bar, edges++ & 1u, abortPtr, p.status, 200);
+                ok = WaitNowWarp(bar, edges++ & 1u, abortPtr, p.status);
                 if (!ok)
-                    break;
-                (void)MbarTryWait(bar, (edges - 1) & 1u, 0);
+                    return;
                 ZeroTileRows(dst, DC, nq - qt * XT, lane);
-                ZeroTileRows(dst + TILE, DC, nq - qt * XT, lane);
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
                 if (lane == 0)
-                    MbarArrive(SmemAddr(&barFull[st]));
+                    MbarArrive(full);
             }
+        };
+        auto loadQ = [&](int i) {
+            if (i >= QSLOTS)
+                ok = ok && MbarWaitWarp(SmemAddr(&bars.qEmpty[i % QSLOTS]), (uint32_t)(i / QSLOTS + 1) & 1u, abortPtr, p.status, 200);
+            if (ok)
+                load(&tmQ, p.aQ, i, ringS + (i % QSLOTS) * TILE, SmemAddr(&bars.qFull[i % QSLOTS]));
+        };
+        auto loadDO = [&](int i) {
+            if (i >= DOSLOTS)
+                ok = ok && MbarWaitWarp(SmemAddr(&bars.doEmpty[i % DOSLOTS]), (uint32_t)(i / DOSLOTS + 1) & 1u, abortPtr, p.status, 200);
+            if (ok)
+                load(&tmDO, p.aDO, i, doRing + (i % DOSLOTS) * TILE, SmemAddr(&bars.doFull[i % DOSLOTS]));
+        };
+        auto loadStat = [&](int i) {
+            if (i >= STATSLOTS)
+                ok = ok && MbarWaitWarp(SmemAddr(&bars.statEmpty[i % STATSLOTS]), (uint32_t)(i / STATSLOTS + 1) & 1u, abortPtr, p.status, 200);
+            if (ok && lane == 0) {
+                const int step = step0 + i, g = step / qTiles, qt = step - g * qTiles, h = kvHead * p.sh.group + g;
+                const float * src = p.work + (((long long)b * p.sh.headsQ + h) * p.tilesPerHead + qt) * (2 * XT);
+                const uint32_t bar = SmemAddr(&bars.statFull[i % STATSLOTS]);
+                MbarExpectTx(bar, SM::STAT);
+                asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                             :: "r"(statRing + (i % STATSLOTS) * SM::STAT), "l"(src), "r"((uint32_t)SM::STAT), "r"(bar) : "memory");
+            }
+            __syncwarp();
+        };
+        /* in the order of their use: q runs two steps ahead of the sums, do and the rows' numbers one */
+        if (n > 0) {
+            loadQ(0);
+            loadStat(0);
+            loadDO(0);
+            if (n > 1)
+                loadQ(1);
+        }
+        for (int i = 0; ok && i + 1 < n; i++) {
+            loadDO(i + 1);
+            loadStat(i + 1);
+            if (i + 2 < n)
+                loadQ(i + 2);
         }
     }
-    else if (warp >= GR_ISSUER) {
-        /* two issuing threads, as above: the scores and dv, the gradients of the weights and dk */
+    else if (warp == GR_ISSUER) {
         if (lane == 0 && n > 0) {
             constexpr uint32_t descS = XattnDesc(XT, 0), descD = XattnDesc(D, 1);
             auto product = [&](uint32_t dst, uint32_t aTile, uint32_t bTile) {
@@ -561,33 +638,60 @@ XattnGradKVKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
                     TcMmaTmemA(dst, aTmem + (ks >> 2) * 64 + (ks & 3) * 8, SmemDesc(bTile + ks * 16 * ROW_BYTES, XBOX_BYTES, 1024, 2), descD,
                                !first || ks != 0 ? 1u : 0u);
             };
-            auto full = [&](int i) { return WaitNow(SmemAddr(&barFull[i % STAGES]), (uint32_t)(i / STAGES) & 1u, abortPtr, p.status); };
-            const bool first = warp == GR_ISSUER;
-            /* (S, k, q, do) or (dP, v, do, q): the tile of the first product, its operands, the second product's */
-            const uint32_t tileT = tmemBase + (first ? TMEM_S : TMEM_DP), accT = tmemBase + (first ? TMEM_DV : TMEM_DK);
-            const uint32_t aTile = first ? kS : vS, bOff = first ? 0 : TILE, cOff = first ? TILE : 0;
-            const uint32_t barOut = first ? SmemAddr(&barS) : SmemAddr(&barDP), barIn = first ? SmemAddr(&barP) : SmemAddr(&barDS);
-            bool ok = WaitNow(SmemAddr(&barKV), 0, abortPtr, p.status) && full(0);
+            bool ok = WaitNow(SmemAddr(&bars.kv), 0, abortPtr, p.status) && WaitNow(SmemAddr(&bars.qFull[0]), 0, abortPtr, p.status);
             if (ok) {
                 TcFenceAfter();
-                product(tileT, aTile, ringS + bOff);
-                TcCommit(barOut);
+                product(tmemBase + TMEM_S, kS, ringS);
+                TcCommit(SmemAddr(&bars.s));
+                ok = WaitNow(SmemAddr(&bars.doFull[0]), 0, abortPtr, p.status);
+            }
+            if (ok) {
+                TcFenceAfter();
+                product(tmemBase + TMEM_DP, vS, doRing);
+                TcCommit(SmemAddr(&bars.dp));
             }
             for (int i = 0; ok && i < n; i++) {
-                const uint32_t cur = ringS + (i % STAGES) * STAGE, nxt = ringS + ((i + 1) % STAGES) * STAGE;
                 const bool more = i + 1 < n;
-                ok = (!more || full(i + 1)) && WaitNow(barIn, (uint32_t)i & 1u, abortPtr, p.status);
+                ok = WaitNow(SmemAddr(&bars.p), (uint32_t)i & 1u, abortPtr, p.status);
                 if (!ok)
                     break;
                 TcFenceAfter();
-                second(accT, tileT, cur + cOff, i == 0);
-                TcCommit(SmemAddr(&barEmpty[i % STAGES]));
+                second(tmemBase + TMEM_DV, tmemBase + TMEM_S, doRing + (i % DOSLOTS) * TILE, i == 0);
                 if (more) {
-                    product(tileT, aTile, nxt + bOff);
-                    TcCommit(barOut);
+                    product(tmemBase + TMEM_S, kS, ringS + ((i + 1) % QSLOTS) * TILE);
+                    TcCommit(SmemAddr(&bars.s));
+                }
+                ok = WaitNow(SmemAddr(&bars.ds), (uint32_t)i & 1u, abortPtr, p.status);
+                if (!ok)
+                    break;
+                TcFenceAfter();
+                second(tmemBase + TMEM_DK, tmemBase + TMEM_DP, ringS + (i % QSLOTS) * TILE, i == 0);
+                if (more) {
+                    product(tmemBase + TMEM_DP, vS, doRing + ((i + 1) % DOSLOTS) * TILE);
+                    TcCommit(SmemAddr(&bars.dp));
                 }
                 else
-                    TcCommit(SmemAddr(&barDone));
+                    TcCommit(SmemAddr(&bars.done));
+            }
+        }
+    }
+    else if (warp == GR_RELAY) {
+        /* as in the first kernel: the next step's copies are there */
+        if (lane == 0 && n > 0) {
+            bool ok = true;
+            for (int i = 0; ok && i < n; i++) {
+                if (i + 1 < n)
+                    ok = WaitNow(SmemAddr(&bars.qFull[(i + 1) % QSLOTS]), (uint32_t)((i + 1) / QSLOTS) & 1u, abortPtr, p.status);
+                if (ok && i > 0)
+                    ok = WaitNow(SmemAddr(&bars.p), (uint32_t)(i - 1) & 1u, abortPtr, p.status);
+                if (ok)
+                    MbarArrive(SmemAddr(&bars.p));
+                if (ok && i + 1 < n)
+                    ok = WaitNow(SmemAddr(&bars.doFull[(i + 1) % DOSLOTS]), (uint32_t)((i + 1) / DOSLOTS) & 1u, abortPtr, p.status);
+                if (ok && i > 0)
+                    ok = WaitNow(SmemAddr(&bars.ds), (uint32_t)(i - 1) & 1u, abortPtr, p.status);
+                if (ok)
+                    MbarArrive(SmemAddr(&bars.ds));
             }
         }
     }
@@ -596,17 +700,18 @@ XattnGradKVKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         const uint32_t laneBase = (uint32_t)(sub * 32) << 16;
         const int r = sub * 32 + lane;
         const uint32_t sT = tmemBase + laneBase + TMEM_S + hf * 64, dpT = tmemBase + laneBase + TMEM_DP + hf * 64;
-        const float4 * statsBase = (const float4 *)(smemRaw + (ringS - SmemAddr(smemRaw)) + 2 * TILE);
         bool ok = true;
         for (int i = 0; i < n; i++) {
             const uint32_t ph = (uint32_t)i & 1u;
-            const int st = i % STAGES;
-            const float4 * lse4 = statsBase + st * (STAGE / 16) + hf * 16, * delta4 = lse4 + XT / 4;
+            const float4 * lse4 = (const float4 *)(kvSmem + SM::KV_STATS + (i % STATSLOTS) * SM::STAT) + hf * 16, * delta4 = lse4 + XT / 4;
             /* every lane observes the copy's completion itself before it reads what was copied */
-            ok = WaitNowWarp(SmemAddr(&barFull[st]), (uint32_t)(i / STAGES) & 1u, abortPtr, p.status) &&
-                 WaitNowWarp(SmemAddr(&barS), ph, abortPtr, p.status);
+            ok = WaitNowWarp(SmemAddr(&bars.statFull[i % STATSLOTS]), (uint32_t)(i / STATSLOTS) & 1u, abortPtr, p.status) &&
+                 WaitNowWarp(SmemAddr(&bars.s), ph, abortPtr, p.status);
             if (!ok)
                 break;
+            /* these scores were issued behind the last product that reads the step before's do */
+            if (threadIdx.x == 0 && i >= 1)
+                MbarArrive(SmemAddr(&bars.doEmpty[(i - 1) % DOSLOTS]));
             TcFenceAfter();
             uint32_t x[64];
             TmemLoad64U(sT, x);
@@ -628,10 +733,15 @@ XattnGradKVKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
             }
             TmemWaitStore();
             TcFenceBefore();
-            MbarArrive(SmemAddr(&barP));
-            ok = WaitNowWarp(SmemAddr(&barDP), ph, abortPtr, p.status);
+            ArriveWarp(SmemAddr(&bars.p), lane);
+            ok = WaitNowWarp(SmemAddr(&bars.dp), ph, abortPtr, p.status);
             if (!ok)
                 break;
+            /* and this product behind the one that reads its q, which all softmax threads let go ahead */
+            if (threadIdx.x == 0 && i >= 1) {
+                MbarArrive(SmemAddr(&bars.qEmpty[(i - 1) % QSLOTS]));
+                MbarArrive(SmemAddr(&bars.statEmpty[(i - 1) % STATSLOTS]));
+            }
             TcFenceAfter();
 #pragma unroll
             for (int c = 0; c < 2; c++) {
@@ -653,10 +763,10 @@ XattnGradKVKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
             }
             TmemWaitStore();
             TcFenceBefore();
-            MbarArrive(SmemAddr(&barDS));
+            ArriveWarp(SmemAddr(&bars.ds), lane);
         }
         if (n > 0 && ok)
-            ok = WaitNowWarp(SmemAddr(&barDone), 0, abortPtr, p.status);
+            ok = WaitNowWarp(SmemAddr(&bars.done), 0, abortPtr, p.status);
         TcFenceAfter();
         const bool sums = n > 0 && ok, rowLive = k0 + r < nk;
         /* warps 0-3: dv, in the place of v; warps 4-7: dk, in the place of k */
@@ -748,6 +858,29 @@ int GradSplits(long long items, int steps, int smCount)
     return splits;
 }
 
+/* one or two launches: the items of a last wave that fills at most half of the GPU are split over it when they are long */
+struct GradPlan {
+    int item0, splits;
+    long long items;
+};
+int PlanGrad(long long items, int steps, int smCount, GradPlan * plan)
+{
+    if (items == 0)
+        return 0;
+    const int splits = GradSplits(items, steps, smCount);
+    const long long rest = items > smCount && splits == 1 ? items % smCount : 0;
+    int restSplits = 1;
+    while (rest > 0 && restSplits < 8 && rest * restSplits * 2 <= smCount && steps >= restSplits * 8)
+        restSplits *= 2;
+    if (restSplits == 1) {
+        plan[0] = { 0, splits, items };
+        return 1;
+    }
+    plan[0] = { 0, 1, items - rest };
+    plan[1] = { (int)(items - rest), restSplits, rest };
+    return 2;
+}
+
 template <int D>
 int LaunchGrad(const DeviceCtx & ctx, const GradCall & call, cudaStream_t stream)
 {
@@ -756,10 +889,6 @@ int LaunchGrad(const DeviceCtx & ctx, const GradCall & call, cudaStream_t stream
     XattnGradParams p;
     memset(&p, 0, sizeof(p));
     p.sh = s;
-    p.out = (const __half *)call.out;
-    p.dout = (const __half *)call.dout;
-    p.lOut = call.l[3];
-    p.lDO = call.l[4];
     p.lse = call.lse;
     p.work = call.work;
     p.tilesPerHead = (s.lenQ + XT - 1) / XT;
@@ -768,18 +897,15 @@ int LaunchGrad(const DeviceCtx & ctx, const GradCall & call, cudaStream_t stream
     p.scaleLog2 = call.scale * LOG2E;
     p.status = ctx.status;
     const long long itemsQ = (long long)s.batch * s.headsQ * p.tilesPerHead, itemsKV = (long long)s.batch * s.headsKV * p.keyTiles;
-    const int splitsQ = GradSplits(itemsQ, p.keyTiles, ctx.smCount);
     const long long steps = (long long)s.group * p.tilesPerHead;
-    if (steps > 0x3fffffffLL || itemsQ * splitsQ > 0x7fffffffLL)
+    if (steps > 0x3fffffffLL || itemsQ * 8 > 0x7fffffffLL || itemsKV * 8 > 0x7fffffffLL)
         return NTB_ERR_LIMIT;
-    const int splitsKV = GradSplits(itemsKV, (int)steps, ctx.smCount);
-    if (itemsKV * splitsKV > 0x7fffffffLL)
-        return NTB_ERR_LIMIT;
-    CUtensorMap tmQ, tmK, tmV, tmDO, tmDQ, tmDK, tmDV;
+    CUtensorMap tmQ, tmK, tmV, tmO, tmDO, tmDQ, tmDK, tmDV;
     HeadsAddr unused;
     int rc;
     if (s.lenQ > 0 &&
         ((rc = EncodeHeads(&tmQ, &p.aQ, call.q, s.dim, s.lenQ, s.headsQ, s.batch, call.l[0], XT)) != NTB_OK ||
+         (rc = EncodeHeads(&tmO, &p.aO, call.out, s.dim, s.lenQ, s.headsQ, s.batch, call.l[3], XT)) != NTB_OK ||
          (rc = EncodeHeads(&tmDO, &p.aDO, call.dout, s.dim, s.lenQ, s.headsQ, s.batch, call.l[4], XT)) != NTB_OK ||
          (rc = EncodeHeads(&tmDQ, &unused, call.dq, s.dim, s.lenQ, s.headsQ, s.batch, call.l[5], 32)) != NTB_OK))
         return rc;
@@ -802,20 +928,27 @@ int LaunchGrad(const DeviceCtx & ctx, const GradCall & call, cudaStream_t stream
     if (!optQ.Ensure((const void *)XattnGradQKernel<D>, SM::Q_TOTAL) || !optKV.Ensure((const void *)XattnGradKVKernel<D>, SM::KV_TOTAL))
         return NTB_ERR_CUDA;
     cudaError_t err = cudaSuccess;
-    if (itemsQ > 0) {
-        p.splits = splitsQ;
-        p.d0 = (__half *)call.dq;
-        p.l0 = call.l[5];
-        err = LaunchClusterPdl(XattnGradQKernel<D>, (unsigned)(itemsQ * splitsQ), GR_THREADS, SM::Q_TOTAL, splitsQ, stream, tmQ, tmK, tmV, tmDO, tmDQ, p);
+    GradPlan plan[2];
+    p.d0 = (__half *)call.dq;
+    p.l0 = call.l[5];
+    int parts = PlanGrad(itemsQ, p.keyTiles, ctx.smCount, plan);
+    for (int i = 0; i < parts && err == cudaSuccess; i++) {
+        p.item0 = plan[i].item0;
+        p.splits = plan[i].splits;
+        err = LaunchClusterPdl(XattnGradQKernel<D>, (unsigned)(plan[i].items * p.splits), GR_THREADS, SM::Q_TOTAL, p.splits, stream,
+                               tmQ, tmK, tmV, tmO, tmDO, tmDQ, p);
         CountLaunch();
     }
-    if (err == cudaSuccess && itemsKV > 0) {
-        p.splits = splitsKV;
-        p.d0 = (__half *)call.dk;
-        p.l0 = call.l[6];
-        p.d1 = (__half *)call.dv;
-        p.l1 = call.l[7];
-        err = LaunchClusterPdl(XattnGradKVKernel<D>, (unsigned)(itemsKV * splitsKV), GR_THREADS, SM::KV_TOTAL, splitsKV, stream, tmQ, tmK, tmV, tmDO, tmDK, tmDV, p);
+    p.d0 = (__half *)call.dk;
+    p.l0 = call.l[6];
+    p.d1 = (__half *)call.dv;
+    p.l1 = call.l[7];
+    parts = PlanGrad(itemsKV, (int)steps, ctx.smCount, plan);
+    for (int i = 0; i < parts && err == cudaSuccess; i++) {
+        p.item0 = plan[i].item0;
+        p.splits = plan[i].splits;
+        err = LaunchClusterPdl(XattnGradKVKernel<D>, (unsigned)(plan[i].items * p.splits), GR_THREADS, SM::KV_TOTAL, p.splits, stream,
+                               tmQ, tmK, tmV, tmDO, tmDK, tmDV, p);
         CountLaunch();
     }
     return (err == cudaSuccess && cudaGetLastError() == cudaSuccess) ? NTB_OK : NTB_ERR_CUDA;
