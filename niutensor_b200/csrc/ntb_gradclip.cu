@@ -5,7 +5,7 @@
  *
  * Two launches whatever the number of tensors (up to 1000; longer lists go in groups): the tensors' addresses
  * travel in the launch parameters, so there is no table to copy to the device and the call can be captured.
- * The list is cut into chunks of equal size that persistent CTAs walk.
+ * The list is cut into chunks of equal size.
  *
  * NormKernel: squares summed in fp64 for floats (a norm that fits a float may have squares that do not), in
  * fp32 over eight exact products and then fp64 for halves; one partial sum a CTA. ClipKernel: every CTA adds
@@ -229,9 +229,13 @@ __global__ void __launch_bounds__(CL_THREADS) ClipKernel(const __grid_constant__
     }
 }
 
+/* CTAs of the norm, each with a partial sum: 16 an SM. The clipping takes a CTA a chunk. 209 M floats, both passes,
+   us: 4 CTAs an SM in both 429; 4 and a CTA a chunk 387; 16 and 64 an SM 383; 16 and a CTA a chunk 374. Many
+   short CTAs keep reads and writes of different chunks in flight together where a persistent CTA alternates. */
+constexpr int CL_CTAS = 16;
 int Ctas(const DeviceCtx & ctx, int chunks)
 {
-    const int most = ctx.smCount * 4;
+    const int most = ctx.smCount * CL_CTAS;
     return chunks < 1 ? 1 : chunks < most ? chunks : most;
 }
 
@@ -273,7 +277,7 @@ int ClipGroups(const DeviceCtx & ctx, int count, const void * const * grads, voi
             const int grid = Ctas(ctx, l.chunks);
             at += grid;
             const cudaError_t err = pass == 0 ? LaunchPdl(NormKernel<MAX>, grid, CL_THREADS, 0, stream, l)
-                                              : LaunchPdl(ClipKernel<MAX>, grid, CL_THREADS, 0, stream, l);
+                                              : LaunchPdl(ClipKernel<MAX>, l.chunks < 1 ? 1 : l.chunks, CL_THREADS, 0, stream, l);
             CountLaunch();
             if (err != cudaSuccess || cudaGetLastError() != cudaSuccess) {
                 cudaGetLastError();
@@ -292,9 +296,9 @@ using namespace ntb;
 
 extern "C" long long ntb_clip_grad_norm_work(int count)
 {
-    /* partial sums: four CTAs an SM (of at most 256) a group of tensors */
+    /* partial sums: a group of tensors at a time, on at most 256 SMs */
     const long long groups = count <= CL_MANY ? 1 : (count + CL_MANY - 1) / CL_MANY;
-    return groups * 256 * 4 * (long long)sizeof(double);
+    return groups * 256 * CL_CTAS * (long long)sizeof(double);
 }
 
 extern "C" int ntb_clip_grad_norm(int devID, void * stream, int count, const void * const * grads, void * const * out,

@@ -231,22 +231,18 @@ def ScaledDotProductAttention(q, k, v, mask=None, scale=None, keep=None, drop_pr
     return out
 
 
-def _heads_layout(t):
-    """strides of a [batch, heads, len, dim] half tensor, as the kernels address it: dense rows, base and
-    strides on 16 bytes (the stride of an extent of one may be anything)"""
-    s = t.stride()
-    if s[3] != 1 or (s[0] | s[1] | s[2]) & 7:
-        n = t.shape
-        _check(s[3] == 1 or n[3] <= 1, "rows of the last dimension must be dense")
-        _check(all(n[i] <= 1 or s[i] % 8 == 0 for i in range(3)), "base and strides must be multiples of 16 bytes")
-    return s[:3]
-
-
-def _aligned(*addresses):
-    """the addresses, which the kernels want on 16 bytes"""
-    for a in addresses:
-        _check(a & 15 == 0, "base and strides must be multiples of 16 bytes")
-    return addresses
+def _heads_layouts(*tensors):
+    """strides of [batch, heads, len, dim] half tensors one behind the other, as the kernels address them: dense
+    rows, strides on 16 bytes (the stride of an extent of one may be anything; the library checks the bases)"""
+    flat = []
+    for t in tensors:
+        a, b, c, d = t.stride()
+        if d != 1 or (a | b | c) & 7:
+            n = t.shape
+            _check(d == 1 or n[3] <= 1, "rows of the last dimension must be dense")
+            _check(all(n[i] <= 1 or s % 8 == 0 for i, s in enumerate((a, b, c))), "base and strides must be multiples of 16 bytes")
+        flat += (a, b, c)
+    return array.array("q", flat)
 
 
 def _heads_like(t):
@@ -258,8 +254,9 @@ def _heads_like(t):
 def _cross_attention_checks(q, k, v, query_lens, key_lens, scale, others=()):
     """device index, shapes of q and k, scale"""
     dev = q.get_device()
-    for t in (q, k, v) + others:
-        if t.dtype is not torch.float16 or t.get_device() != dev or dev < 0 or t.dim() != 4:
+    half = torch.float16
+    for t in (q, k, v, *others):
+        if t.dtype is not half or t.get_device() != dev or dev < 0 or t.dim() != 4:
             _check(t.is_cuda and q.is_cuda, "this library has no CPU path: tensors must live on a CUDA device")
             _check(t.dtype == torch.float16, "Unsupported data type!")
             _check(t.get_device() == dev, "The code must be run on the same GPU!")
@@ -282,9 +279,6 @@ def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
-_Layouts4, _Layouts8 = ctypes.c_longlong * 12, ctypes.c_longlong * 24
-
-
 def CrossAttention(q, k, v, query_lens=None, key_lens=None, scale=None, out=None, with_lse=False):
     """softmax(scale * q k^T) v of a decoder's positions over an encoder's states of another length
     (the attention over the encoder's output in source/sample/transformer/submodel/Decoder.cpp).
@@ -303,11 +297,12 @@ def CrossAttention(q, k, v, query_lens=None, key_lens=None, scale=None, out=None
         out = _heads_like(q)
     else:
         _check(out.get_device() == dev and out.dtype is torch.float16 and out.shape == qs, "Incorrect tensor sizes!")
-    layouts = _Layouts4(*_heads_layout(q), *_heads_layout(k), *_heads_layout(v), *_heads_layout(out))
+    layouts = _heads_layouts(q, k, v, out)
     batch, heads, len_q, d = qs
     lse = torch.empty(qs[:3], dtype=torch.float32, device=q.device) if with_lse else None
-    rc = capi.lib().ntb_cross_attention(dev, _raw_stream(dev), *_aligned(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr()), _ptr(lse),
-                                        X_FLOAT16, batch, heads, ks[1], len_q, ks[2], d, layouts, _ptr(query_lens), _ptr(key_lens), scale)
+    rc = capi.lib().ntb_cross_attention(dev, _raw_stream(dev), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), None if lse is None else lse.data_ptr(),
+                                        X_FLOAT16, batch, heads, ks[1], len_q, ks[2], d, layouts.buffer_info()[0],
+                                        None if query_lens is None else query_lens.data_ptr(), None if key_lens is None else key_lens.data_ptr(), scale)
     if rc:
         _raise_rc(rc, "CrossAttention")
     return (out, lse) if with_lse else out
@@ -324,14 +319,12 @@ def GradCrossAttention(q, k, v, out, lse, dedo, query_lens=None, key_lens=None, 
     _check(lse.get_device() == dev and lse.dtype is torch.float32 and lse.is_contiguous() and lse.shape == qs[:3],
            "lse must be the packed fp32 CUDA tensor of the forward call")
     dedq, dedk, dedv = _heads_like(q), _heads_like(k), _heads_like(v)
-    layouts = _Layouts8(*_heads_layout(q), *_heads_layout(k), *_heads_layout(v), *_heads_layout(out), *_heads_layout(dedo),
-                        *_heads_layout(dedq), *_heads_layout(dedk), *_heads_layout(dedv))
+    layouts = _heads_layouts(q, k, v, out, dedo, dedq, dedk, dedv)
     lib = capi.lib()
     need = lib.ntb_cross_attention_grad_work(batch, heads, len_q)
     work = torch.empty(need, dtype=torch.uint8, device=q.device)
-    pq, pk, pv, po, pdo = _aligned(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), dedo.data_ptr())
-    rc = lib.ntb_cross_attention_grad(dev, _raw_stream(dev), pq, pk, pv, po, lse.data_ptr(), pdo, dedq.data_ptr(), dedk.data_ptr(), dedv.data_ptr(),
-                                      work.data_ptr(), need, X_FLOAT16, batch, heads, ks[1], len_q, ks[2], d, layouts,
+    rc = lib.ntb_cross_attention_grad(dev, _raw_stream(dev), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), dedo.data_ptr(), dedq.data_ptr(), dedk.data_ptr(), dedv.data_ptr(),
+                                      work.data_ptr(), need, X_FLOAT16, batch, heads, ks[1], len_q, ks[2], d, layouts.buffer_info()[0],
                                       _ptr(query_lens), _ptr(key_lens), scale)
     if rc:
         _raise_rc(rc, "GradCrossAttention")
@@ -358,7 +351,7 @@ def Embedding(w, ids, scale=1.0, pos=None):
                "positions must be a packed matrix of the words' type and width")
         rows = pos.shape[0]
         _check(tokens == 0 or (rows > 0 and tokens % rows == 0), "Incorrect tensor sizes!")
-    out = torch.empty(ids.shape + (d,), dtype=w.dtype, device=w.device)
+    out = w.new_empty(ids.shape + (d,))
     rc = capi.lib().ntb_embedding(dev, _raw_stream(dev), ids.data_ptr(), w.data_ptr(), _ptr(pos) if rows else None, out.data_ptr(), dtype,
                                   tokens, vocab, d, pitch if vocab > 1 else d, d, rows, scale)
     if rc:
