@@ -183,6 +183,9 @@ XattnGradQKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
     const int tile0 = rank * perSplit < keyTiles ? rank * perSplit : keyTiles;
     const int tile1 = tile0 + perSplit < keyTiles ? tile0 + perSplit : keyTiles;
     const int n = tile1 - tile0;
+    /* All keys in one tile: delta_i = sum_j p_ij dp_ij is taken from the tile. From the rounded out it would be off by
+       2^-11 of sum |do out|, which shows when few keys leave dp - delta small. */
+    const bool single = keyTiles == 1;
     /* the last tile reaches past the sequence's keys into rows that exist: those rows of k are cleared */
     const bool fix = n > 0 && tile1 * XT > nk && nk < p.sh.lenK;
 
@@ -191,12 +194,13 @@ XattnGradQKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
             bool ok = true;
             /* tiles in the order of their use: k 0, v 0, k 1, v 1, ... The last three slots first hold this item's rows of
                q, do and out, on their way to tensor memory. */
-            MbarExpectTx(SmemAddr(&barRows), 3 * TILE);
+            MbarExpectTx(SmemAddr(&barRows), (single ? 2 : 3) * TILE);
 #pragma unroll
             for (int dc = 0; dc < DC; dc++) {
                 TmaLoad4D(ringS + ROWS0 * TILE + dc * XBOX_BYTES, &tmQ, SmemAddr(&barRows), dc * 64, q0, h * p.aQ.mulHead, b * p.aQ.mulBatch);
                 TmaLoad4D(ringS + (ROWS0 + 1) * TILE + dc * XBOX_BYTES, &tmDO, SmemAddr(&barRows), dc * 64, q0, h * p.aDO.mulHead, b * p.aDO.mulBatch);
-                TmaLoad4D(ringS + (ROWS0 + 2) * TILE + dc * XBOX_BYTES, &tmO, SmemAddr(&barRows), dc * 64, q0, h * p.aO.mulHead, b * p.aO.mulBatch);
+                if (!single)
+                    TmaLoad4D(ringS + (ROWS0 + 2) * TILE + dc * XBOX_BYTES, &tmO, SmemAddr(&barRows), dc * 64, q0, h * p.aO.mulHead, b * p.aO.mulBatch);
             }
             for (int i = 0; ok && i < 2 * n; i++) {
                 if (i == ROWS0)
@@ -330,9 +334,10 @@ XattnGradQKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                 uint32_t xs[4], ys[4], zs[4];
                 LoadShared16(at, zs);
                 LoadShared16(at + TILE, ys);
-                LoadShared16(at + 2 * TILE, xs);
+                if (!single)
+                    LoadShared16(at + 2 * TILE, xs);
 #pragma unroll
-                for (int e = 0; e < 4; e++) {
+                for (int e = 0; e < 4 && !single; e++) {
                     const float2 xf = __half22float2(*(const __half2 *)&xs[e]), yf = __half22float2(*(const __half2 *)&ys[e]);
                     part = fmaf(xf.x, yf.x, part);
                     part = fmaf(xf.y, yf.y, part);
@@ -353,19 +358,25 @@ XattnGradQKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         if (hf == 0)
             sDelta[r] = part + sDelta[r];
         GradBarrier();
-        const float delta = sDelta[r];
+        float delta = sDelta[r];
         /* exponents of 2; plus infinity makes every weight of an empty row 0 */
         const float lse2 = rowLive ? p.lse[((long long)b * p.sh.headsQ + h) * p.sh.lenQ + row] * LOG2E : INFINITY;
-        if (hf == 0 && rank == 0) {          /* the second kernel's exponents carry the factor of p; dP and delta its inverse */
-            float * w = p.work + (long long)item * (2 * XT);
-            w[r] = lse2 - P_SCALE_LOG2;
-            w[XT + r] = delta * P_SCALE_INV;
-        }
+        /* for the second kernel, whose exponents carry the factor of p; dP and delta its inverse */
+        auto leaveRow = [&]() {
+            if (hf == 0 && rank == 0) {
+                float * w = p.work + (long long)item * (2 * XT);
+                w[r] = lse2 - P_SCALE_LOG2;
+                w[XT + r] = delta * P_SCALE_INV;
+            }
+        };
+        if (!single)
+            leaveRow();
         const uint32_t sT = tmemBase + laneBase + TMEM_S + hf * 64, dpT = tmemBase + laneBase + TMEM_DP + hf * 64;
-        for (int j = 0; ok && j < n; j++) {
+        /* with a single tile no warp leaves out the barriers of the joint sum, whatever became of its waits */
+        for (int j = 0; (ok || single) && j < n; j++) {
             const uint32_t ph = (uint32_t)j & 1u;
-            ok = WaitNowWarp(SmemAddr(&barS), ph, abortPtr, p.status);
-            if (!ok)
+            ok = WaitNowWarp(SmemAddr(&barS), ph, abortPtr, p.status) && ok;
+            if (!ok && !single)
                 break;
             TcFenceAfter();
             uint32_t x[64];
@@ -376,13 +387,33 @@ XattnGradQKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
             for (int e = 0; e < 64; e++)
                 x[e] = __float_as_uint(Exp2(fmaf(__uint_as_float(x[e]), p.scaleLog2, -lse2)));
             const int valid = nk - (tile0 + j) * XT - hf * 64;
-            ok = WaitNowWarp(SmemAddr(&barDP), ph, abortPtr, p.status);
-            if (!ok)
+            ok = WaitNowWarp(SmemAddr(&barDP), ph, abortPtr, p.status) && ok;
+            if (!ok && !single)
                 break;
             /* v of this tile and k of the one before have been read */
             if (threadIdx.x == 0)
                 MbarArrive(SmemAddr(&barEvent[j % GR_EVENTS]));
             TcFenceAfter();
+            if (single) {
+                float sum = 0.f;
+#pragma unroll
+                for (int c = 0; c < 2; c++) {
+                    uint32_t y[32];
+                    TmemLoad32Async(dpT + c * 32, y);
+                    TmemWaitLoad();
+#pragma unroll
+                    for (int e = 0; e < 32; e++)
+                        sum += c * 32 + e < valid ? __uint_as_float(x[c * 32 + e]) * __uint_as_float(y[e]) : 0.f;
+                }
+                if (hf == 1)
+                    sDelta[r] = sum;
+                GradBarrier();
+                if (hf == 0)
+                    sDelta[r] = sum + sDelta[r];
+                GradBarrier();
+                delta = rowLive ? sDelta[r] : 0.f;
+                leaveRow();
+            }
 #pragma unroll
             for (int c = 0; c < 2; c++) {
                 uint32_t y[32], w[16];
