@@ -10,15 +10,19 @@
  * frequent words, so the tokens are sorted first and equal words summed as runs:
  *
  *   TokenSortKernel   a stable radix sort of (id, t) in ONE launch: one cluster of CTAs, digits of at most
- *                     9 bits. Every warp owns a contiguous piece of the list; per pass it counts its digits,
- *                     the counts are prefixed over warps and (through distributed shared memory) over the
- *                     cluster's CTAs, and it walks its piece again, 32 tokens at a time, to scatter them. The
- *                     steps are separated by the hardware's cluster barrier. Meanwhile the other CTAs of
- *                     the grid clear dw (beta = 0), which takes longer than the sort for large vocabularies.
+ *                     9 bits. Every CTA owns a contiguous part of the list; per pass it counts its digits, the
+ *                     counts are prefixed over the cluster's CTAs through distributed shared memory, and the
+ *                     part, tile by tile, is ranked (a warp its own piece, 32 tokens at a time), put in its new
+ *                     order in shared memory and written out from there. The steps are separated by the
+ *                     hardware's cluster barrier. Meanwhile the other CTAs of the grid clear dw (beta = 0).
  *   RunSumKernel      the sorted list cut into equal blocks, whatever the words' frequencies; a thread owns
  *                     16 bytes of the columns and adds the rows of a block one after the other. Runs inside a
  *                     block go straight to dw, pieces of runs that cross an edge to fp32 partial rows.
  *   RunJoinKernel     adds up the pieces of a crossing run, in block order.
+ *
+ * Up to FEW_TOKENS tokens: FewTokensKernel, one launch without a workspace. The first token of a word finds its
+ * others by looking through the list in shared memory and adds their rows; other CTAs meanwhile clear the rows
+ * of dw whose words do not occur (beta = 0), known from a bit map of the list.
  *
  * Sums are fp32 in a fixed order. Ids outside [0, vocab) stand for no word.
  */
@@ -218,12 +222,10 @@ __global__ void __launch_bounds__(SORT_THREADS) TokenSortKernel(const SortParams
     const long long lo = rank * per < p.tokens ? rank * per : p.tokens;
     const long long hi = lo + per < p.tokens ? lo + per : p.tokens;
     const unsigned before = (1u << lane) - 1u;
-    /* a list of one tile stays in shared memory between the passes; a part of one tile is loaded once a pass */
-    const bool resident = p.ctas == 1 && p.tokens <= SORT_TILE, once = hi - lo <= SORT_TILE;
+    const bool once = hi - lo <= SORT_TILE;                       /* a part of one tile is loaded once a pass */
 
     for (int pass = 0; pass < p.passes; pass++) {
         const int shift = pass * p.bits;
-        const bool last = pass == p.passes - 1;
         /* the last pass writes a */
         int2 * dst = ((p.passes - 1 - pass) & 1) == 0 ? p.a : p.b;
         const int2 * src = dst == p.a ? p.b : p.a;
@@ -232,7 +234,7 @@ __global__ void __launch_bounds__(SORT_THREADS) TokenSortKernel(const SortParams
                 const int id = p.ids[i];
                 return make_int2(id >= 0 && id < p.vocab ? id : p.vocab, (int)i);
             }
-            return resident ? stage[i] : __ldcg(src + i);
+            return __ldcg(src + i);
         };
         auto digit = [&](const int2 & x) { return (x.x >> shift) & (R - 1); };
         /* a warp's tokens lie one behind the other: ranks within a digit follow the list's order */
@@ -249,49 +251,47 @@ __global__ void __launch_bounds__(SORT_THREADS) TokenSortKernel(const SortParams
         };
         if (once)
             loadTile(lo);
-        if (!resident) {
-            if ((int)threadIdx.x < R)
-                totals[threadIdx.x] = 0;
-            __syncthreads();
-            if (once) {
+        if ((int)threadIdx.x < R)
+            totals[threadIdx.x] = 0;
+        __syncthreads();
+        if (once) {
+#pragma unroll
+            for (int u = 0; u < SORT_AHEAD; u++)
+                if (u < each && (warp * each + u) * 32 + lane < count)
+                    atomicAdd(totals + digit(x[u]), 1);
+        }
+        else {
+            for (long long i0 = lo + threadIdx.x; i0 < hi; i0 += SORT_TILE) {
+                int d[SORT_AHEAD];
 #pragma unroll
                 for (int u = 0; u < SORT_AHEAD; u++)
-                    if (u < each && (warp * each + u) * 32 + lane < count)
-                        atomicAdd(totals + digit(x[u]), 1);
+                    d[u] = i0 + u * SORT_THREADS < hi ? digit(load(i0 + u * SORT_THREADS)) : -1;
+#pragma unroll
+                for (int u = 0; u < SORT_AHEAD; u++)
+                    if (d[u] >= 0)
+                        atomicAdd(totals + d[u], 1);
             }
-            else {
-                for (long long i0 = lo + threadIdx.x; i0 < hi; i0 += SORT_TILE) {
-                    int d[SORT_AHEAD];
-#pragma unroll
-                    for (int u = 0; u < SORT_AHEAD; u++)
-                        d[u] = i0 + u * SORT_THREADS < hi ? digit(load(i0 + u * SORT_THREADS)) : -1;
-#pragma unroll
-                    for (int u = 0; u < SORT_AHEAD; u++)
-                        if (d[u] >= 0)
-                            atomicAdd(totals + d[u], 1);
-                }
-            }
-            ClusterSync();
-            /* where a digit's tokens start: all smaller digits, then the same digit in the CTAs before this one */
-            int all = 0, ahead = 0;
-            if ((int)threadIdx.x < R) {
-                int n[SORT_CTAS];
-#pragma unroll
-                for (int c = 0; c < SORT_CTAS; c++) {
-                    n[c] = 0;
-                    if (c < p.ctas)
-                        asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(n[c]) : "r"(MapShared(SmemAddr(totals + threadIdx.x), c)) : "memory");
-                }
-#pragma unroll
-                for (int c = 0; c < SORT_CTAS; c++) {
-                    all += n[c];
-                    ahead += c < rank ? n[c] : 0;
-                }
-            }
-            const int start = BlockScan(all, warpSums[0], warp, lane) + ahead;
-            if ((int)threadIdx.x < R)
-                bases[threadIdx.x] = start;
         }
+        ClusterSync();
+        /* where a digit's tokens start: all smaller digits, then the same digit in the CTAs before this one */
+        int all = 0, ahead = 0;
+        if ((int)threadIdx.x < R) {
+            int n[SORT_CTAS];
+#pragma unroll
+            for (int c = 0; c < SORT_CTAS; c++) {
+                n[c] = 0;
+                if (c < p.ctas)
+                    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(n[c]) : "r"(MapShared(SmemAddr(totals + threadIdx.x), c)) : "memory");
+            }
+#pragma unroll
+            for (int c = 0; c < SORT_CTAS; c++) {
+                all += n[c];
+                ahead += c < rank ? n[c] : 0;
+            }
+        }
+        const int start = BlockScan(all, warpSums[0], warp, lane) + ahead;
+        if ((int)threadIdx.x < R)
+            bases[threadIdx.x] = start;
 
         for (long long tile = lo; tile < hi; tile += SORT_TILE) {
             if (!once)
@@ -337,26 +337,18 @@ __global__ void __launch_bounds__(SORT_THREADS) TokenSortKernel(const SortParams
                     stage[localBases[d] + mine[d] + place[u]] = x[u];
                 }
             __syncthreads();
-            if (resident) {
-                if (last)
-                    for (int i = threadIdx.x; i < count; i += SORT_THREADS)
-                        dst[i] = stage[i];
+            /* in the new order neighbours go to neighbouring places: whole lines instead of one store a token */
+            for (int i = threadIdx.x; i < count; i += SORT_THREADS) {
+                const int2 y = stage[i];
+                const int d = digit(y);
+                __stcg(dst + bases[d] + i - localBases[d], y);
             }
-            else {
-                /* in the new order neighbours go to neighbouring places: whole lines instead of one store a token */
-                for (int i = threadIdx.x; i < count; i += SORT_THREADS) {
-                    const int2 y = stage[i];
-                    const int d = digit(y);
-                    __stcg(dst + bases[d] + i - localBases[d], y);
-                }
-                __syncthreads();
-                if ((int)threadIdx.x < R)
-                    bases[threadIdx.x] += run;
-            }
+            __syncthreads();
+            if ((int)threadIdx.x < R)
+                bases[threadIdx.x] += run;
         }
         /* the list in its new order is complete, and the totals have been read, before the next pass */
-        if (!resident)
-            ClusterSync();
+        ClusterSync();
     }
 }
 
@@ -488,6 +480,253 @@ __global__ void RunSumKernel(const RunParams p)
     }
 }
 
+/* ---------------------------------------------------------------- few tokens */
+
+/* Whole gradient, us in graph replay, few-tokens kernel / sort and runs, vocabulary 32000 of 512 halves and 5000 of
+   1024: 256 tokens 7.2 / 14.4 and 5.3; 1000 8.8 / 16.0 and 7.9; 2048 11.4 / 18.0 and 14.7; 4096 19.8 / 19.4 and
+   30.6 / 23.8 (the search grows with the square of the list). */
+constexpr int FEW_TOKENS = 2048;
+constexpr int FEW_THREADS = 256, FEW_WARPS = FEW_THREADS / 32;
+constexpr int FEW_LIST = 24;              /* tokens of a word up to which one warp adds them all */
+constexpr int FEW_CLEAR_ROWS = 4096;      /* rows of dw a clearing CTA looks after at a time: its bit map */
+
+/* columns of a CTA: 16 bytes a lane, or four columns a lane one at a time */
+template <int N> constexpr int FEW_COLS = N > 1 ? 32 * N : 128;
+
+struct FewParams {
+    const int * ids;
+    const void * dout;
+    void * dw;
+    int tokens, vocab, dim;
+    long long ldo, ldw;
+    float scale;
+    int accumulate;
+    int sumCtas, colBlocks;   /* sumCtas x colBlocks CTAs sum; the others clear */
+};
+
+/* the rows at[0 .. n) of dout, one after the other, into N columns of dw's row id */
+template <typename TO, typename TW, bool VEC>
+__device__ __forceinline__ void AddRows(const FewParams & p, const unsigned short * at, int n, int col, float * acc)
+{
+    constexpr int N = VEC ? EmVec<TO>::N : 1;
+    constexpr int U = 8;
+    for (int i0 = 0; i0 < n; i0 += U) {
+        uint4 raw[VEC ? U : 1];
+        float one[VEC ? 1 : U];
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const TO * src = (const TO *)p.dout + (long long)at[i0 + u < n ? i0 + u : n - 1] * p.ldo + col;
+            if (VEC)
+                raw[u] = *(const uint4 *)src;
+            else
+                one[u] = Get(src);
+        }
+#pragma unroll
+        for (int u = 0; u < U; u++)
+            if (i0 + u < n) {
+                if (VEC) {
+                    float v[EmVec<TO>::N];
+                    UnpackRow(raw[u], v, (const TO *)nullptr);
+#pragma unroll
+                    for (int e = 0; e < N; e++)
+                        acc[e] += v[e];
+                }
+                else
+                    acc[0] += one[u];
+            }
+    }
+}
+
+template <typename TO, typename TW, bool VEC>
+__device__ __forceinline__ void PutRow(const FewParams & p, int id, int col, const float * acc)
+{
+    constexpr int N = VEC ? EmVec<TO>::N : 1;
+    TW * dst = (TW *)p.dw + id * p.ldw + col;
+    if (VEC) {
+        constexpr int PN = EmVec<TW>::N;
+#pragma unroll
+        for (int k = 0; k < N; k += PN) {
+            float v[PN];
+#pragma unroll
+            for (int e = 0; e < PN; e++)
+                v[e] = 0.f;
+            if (p.accumulate)
+                UnpackRow(*(const uint4 *)(dst + k), v, (const TW *)nullptr);
+#pragma unroll
+            for (int e = 0; e < PN; e++)
+                v[e] = fmaf(acc[(k + e) % N], p.scale, v[e]);
+            *(uint4 *)(dst + k) = PackRow(v, (const TW *)nullptr);
+        }
+    }
+    else
+        Put(dst, fmaf(acc[0], p.scale, p.accumulate ? Get(dst) : 0.f));
+}
+
+template <typename TO, typename TW, bool VEC>
+__global__ void __launch_bounds__(FEW_THREADS) FewTokensKernel(const FewParams p)
+{
+    constexpr int N = VEC ? EmVec<TO>::N : 1;
+    __shared__ __align__(16) int words[FEW_TOKENS];
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int block = blockIdx.x % (p.sumCtas > 0 ? p.sumCtas : 1);
+    if ((int)blockIdx.x >= p.sumCtas * p.colBlocks) {
+        /* clear the rows of the words that do not occur */
+        unsigned * seen = (unsigned *)words;
+        const int ctas = gridDim.x - p.sumCtas * p.colBlocks;
+        const int each = (p.vocab + ctas - 1) / ctas;
+        const long long first = (long long)(blockIdx.x - p.sumCtas * p.colBlocks) * each;
+        const int end = first + each < p.vocab ? (int)(first + each) : p.vocab;
+        for (long long lo64 = first; lo64 < end; lo64 += FEW_CLEAR_ROWS) {
+            const int lo = (int)lo64, hi = end - lo < FEW_CLEAR_ROWS ? end : lo + FEW_CLEAR_ROWS;
+            __syncthreads();
+            for (int i = threadIdx.x; i < FEW_CLEAR_ROWS / 32; i += FEW_THREADS)
+                seen[i] = 0u;
+            __syncthreads();
+            for (int i = threadIdx.x; i < p.tokens; i += FEW_THREADS) {
+                const int id = p.ids[i];
+                if (id >= lo && id < hi)
+                    atomicOr(seen + ((id - lo) >> 5), 1u << ((id - lo) & 31));
+            }
+            __syncthreads();
+            for (int v = lo + warp; v < hi; v += FEW_WARPS)
+                if (((seen[(v - lo) >> 5] >> ((v - lo) & 31)) & 1u) == 0u)
+                    ClearWarp((unsigned char *)((TW *)p.dw + v * p.ldw), (long long)p.dim * sizeof(TW), lane);
+        }
+        return;
+    }
+    __shared__ unsigned short lists[FEW_WARPS][FEW_LIST];
+    __shared__ int counts[FEW_WARPS];
+    __shared__ float parts[FEW_WARPS][32 * (VEC ? EmVec<TO>::N : 1)];
+    /* whole steps of 256: what lies behind the list is no word */
+    for (int i = threadIdx.x; i < (p.tokens + 255) / 256 * 256; i += FEW_THREADS)
+        words[i] = i < p.tokens ? p.ids[i] : -1;
+    __syncthreads();
+    /* a warp a token: if the word has no earlier token, how many it has, and the first of them. Frequent words occur
+       early: neighbours in the list go to different CTAs. */
+    const unsigned before = (1u << lane) - 1u;
+    const int t = warp * p.sumCtas + block;
+    const int colLo = blockIdx.x / p.sumCtas * FEW_COLS<N>, colHi = colLo + FEW_COLS<N> < p.dim ? colLo + FEW_COLS<N> : p.dim;
+    int count = 0;
+    if (t < p.tokens) {
+        const int id = words[t];
+        if (id >= 0 && id < p.vocab) {
+            /* four tokens a lane at a time: most steps find nothing */
+            bool earlier = false;
+            for (int i0 = 0; i0 < t && !earlier; i0 += 256) {
+                const int i = i0 + lane * 4;
+                const int4 a = *(const int4 *)(words + i), b = *(const int4 *)(words + i + 128);
+                const bool hit = (a.x == id && i < t) || (a.y == id && i + 1 < t) || (a.z == id && i + 2 < t) || (a.w == id && i + 3 < t) ||
+                                 (b.x == id && i + 128 < t) || (b.y == id && i + 129 < t) || (b.z == id && i + 130 < t) || (b.w == id && i + 131 < t);
+                earlier = __any_sync(0xffffffffu, hit);
+            }
+            if (!earlier)
+                for (int i0 = t & ~127; i0 < p.tokens; i0 += 128) {
+                    const int i = i0 + lane * 4;
+                    const int4 a = *(const int4 *)(words + i);
+                    const bool h[4] = { a.x == id && i >= t, a.y == id && i + 1 >= t, a.z == id && i + 2 >= t, a.w == id && i + 3 >= t };
+                    if (!__any_sync(0xffffffffu, h[0] || h[1] || h[2] || h[3]))
+                        continue;
+                    int place = count;
+                    unsigned votes = 0;
+#pragma unroll
+                    for (int k = 0; k < 4; k++) {
+                        const unsigned vote = __ballot_sync(0xffffffffu, h[k]);
+                        place += __popc(vote & before);
+                        votes += __popc(vote);
+                    }
+#pragma unroll
+                    for (int k = 0; k < 4; k++)
+                        if (h[k]) {
+                            if (place < FEW_LIST)
+                                lists[warp][place] = (unsigned short)(i + k);
+                            place++;
+                        }
+                    count += votes;
+                }
+        }
+    }
+    if (lane == 0)
+        counts[warp] = count;
+    __syncwarp();
+    if (count > 0 && count <= FEW_LIST)
+        for (int col = colLo + lane * N; col < colHi; col += 32 * N) {
+            float acc[N];
+#pragma unroll
+            for (int e = 0; e < N; e++)
+                acc[e] = 0.f;
+            AddRows<TO, TW, VEC>(p, lists[warp], count, col, acc);
+            PutRow<TO, TW, VEC>(p, words[t], col, acc);
+        }
+    __syncthreads();
+    /* frequent words, one after the other: the CTA's warps share the list in equal pieces */
+    for (int w = 0; w < FEW_WARPS; w++) {
+        if (counts[w] <= FEW_LIST)
+            continue;
+        const int id = words[w * p.sumCtas + block];
+        const int each = ((p.tokens + FEW_WARPS - 1) / FEW_WARPS + 31) / 32 * 32;
+        const int lo = warp * each, hi = lo + each < p.tokens ? lo + each : p.tokens;
+        for (int col0 = colLo; col0 < colHi; col0 += 32 * N) {
+            const int col = col0 + lane * N;
+            float acc[N];
+#pragma unroll
+            for (int e = 0; e < N; e++)
+                acc[e] = 0.f;
+            int have = 0;
+            for (int i0 = lo; i0 < hi || have > 0; i0 += 32) {
+                unsigned vote = 0u;
+                if (i0 < hi) {
+                    const int i = i0 + lane;
+                    const bool hit = i < hi && words[i] == id;
+                    vote = __ballot_sync(0xffffffffu, hit);
+                }
+                /* the list takes 24: a step of 32 tokens is taken in two halves */
+#pragma unroll
+                for (int half = 0; half < 2; half++) {
+                    const unsigned bits = half == 0 ? vote & 0xffffu : vote >> 16;
+                    if (have + __popc(bits) > FEW_LIST || (i0 >= hi && have > 0)) {
+                        __syncwarp();
+                        if (col < colHi)
+                            AddRows<TO, TW, VEC>(p, lists[warp], have, col, acc);
+                        have = 0;
+                        __syncwarp();
+                    }
+                    if (lane < 16 && ((bits >> lane) & 1u))
+                        lists[warp][have + __popc(bits & ((1u << lane) - 1u))] = (unsigned short)(i0 + half * 16 + lane);
+                    have += __popc(bits);
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < N; e++)
+                parts[warp][lane * N + e] = acc[e];
+            __syncthreads();
+            if (warp == 0 && col < colHi) {
+                for (int k = 1; k < FEW_WARPS; k++)
+#pragma unroll
+                    for (int e = 0; e < N; e++)
+                        acc[e] += parts[k][lane * N + e];
+                PutRow<TO, TW, VEC>(p, id, col, acc);
+            }
+            __syncthreads();
+        }
+    }
+}
+
+template <typename TO, typename TW>
+cudaError_t LaunchFew(FewParams p, bool vec, int clearing, cudaStream_t stream)
+{
+    const int cols = vec ? FEW_COLS<EmVec<TO>::N> : FEW_COLS<1>;
+    p.colBlocks = (p.dim + cols - 1) / cols;
+    const long long grid = (long long)p.sumCtas * p.colBlocks + clearing;
+    if (grid > 0x7fffffffLL)
+        return cudaErrorInvalidValue;
+    const cudaError_t err = vec ? LaunchPdl(FewTokensKernel<TO, TW, true>, (int)grid, FEW_THREADS, 0, stream, p)
+                                : LaunchPdl(FewTokensKernel<TO, TW, false>, (int)grid, FEW_THREADS, 0, stream, p);
+    CountLaunch();
+    return err;
+}
+
 /* block i: the run, if any, that begins in block i of the list and goes on behind it */
 template <typename TW>
 __global__ void RunJoinKernel(const RunParams p)
@@ -547,12 +786,11 @@ int RunBlock(int tokens)
     return block;
 }
 
-/* CTAs that sort. Whole call on a B200 with 512 halves a row, us in graph replay with 1 / 8 / 16 CTAs: 2048 tokens
-   17.9 / 18.0 / 18.8, 4096 22.5 / 19.8 / 20.2, 8192 32 / 22 / 22, 20000 96 / 33 / 32, 100000 391 / 109 / 85. One CTA keeps
-   its passes in shared memory and needs no barriers of the cluster; more rank fewer tokens each. */
+/* CTAs that sort. Whole call on a B200 with 512 halves a row, us in graph replay with 4 / 8 / 16 CTAs: 4096 tokens
+   22.6 / 19.8 / 20.2, 8192 27 / 22 / 22, 20000 48 / 33 / 32, 100000 185 / 109 / 85. */
 int SortCtas(int tokens)
 {
-    return tokens <= 2048 ? 1 : tokens <= 16384 ? 8 : SORT_CTAS;
+    return tokens <= 16384 ? 8 : SORT_CTAS;
 }
 
 bool RowsAligned(const void * p, long long pitch, int dim, int size)
@@ -561,10 +799,15 @@ bool RowsAligned(const void * p, long long pitch, int dim, int size)
 }
 
 template <typename TO, typename TW>
+bool WideRows(const void * dout, long long ldo, const void * dw, long long ldw, int dim)
+{
+    return RowsAligned(dout, ldo, dim, sizeof(TO)) && RowsAligned(dw, ldw, dim, sizeof(TW)) && dim % EmVec<TO>::N == 0;
+}
+
+template <typename TO, typename TW>
 cudaError_t LaunchRuns(const RunParams & p, cudaStream_t stream)
 {
-    const bool vec = RowsAligned(p.dout, p.ldo, p.dim, sizeof(TO)) && RowsAligned(p.dw, p.ldw, p.dim, sizeof(TW)) &&
-                     (p.dim % EmVec<TO>::N) == 0;
+    const bool vec = WideRows<TO, TW>(p.dout, p.ldo, p.dw, p.ldw, p.dim);
     const int threadsNeeded = vec ? p.dim / EmVec<TO>::N : p.dim;
     const int block = threadsNeeded >= 256 ? 256 : (threadsNeeded + 31) / 32 * 32;
     cudaLaunchConfig_t cfg = {};
@@ -659,6 +902,31 @@ extern "C" int ntb_embedding_grad(int devID, void * stream, const int * ids, con
     if (!ctx)
         return NTB_ERR_CUDA;
     cudaStream_t st = (cudaStream_t)stream;
+    const bool halves = dtypeOut == NTB_X_FLOAT16, halfW = dtypeW == NTB_X_FLOAT16;
+    if (tokens <= FEW_TOKENS) {
+        FewParams f;
+        memset(&f, 0, sizeof(f));
+        f.ids = ids;
+        f.dout = dout;
+        f.dw = dw;
+        f.tokens = tokens; f.vocab = vocab; f.dim = dim;
+        f.ldo = ldo; f.ldw = ldw;
+        f.scale = scale;
+        f.accumulate = beta == 1.f;
+        f.sumCtas = (tokens + FEW_WARPS - 1) / FEW_WARPS;
+        int clearing = 0;
+        if (beta == 0.f) {
+            const int most = 4 * ctx->smCount, want = (vocab + FEW_WARPS - 1) / FEW_WARPS;
+            clearing = want < most ? want : most;
+        }
+        const cudaError_t e = !halves ? LaunchFew<float, float>(f, WideRows<float, float>(dout, ldo, dw, ldw, dim), clearing, st)
+            : !halfW ? LaunchFew<__half, float>(f, WideRows<__half, float>(dout, ldo, dw, ldw, dim), clearing, st)
+                     : LaunchFew<__half, __half>(f, WideRows<__half, __half>(dout, ldo, dw, ldw, dim), clearing, st);
+        if (e == cudaSuccess && cudaGetLastError() == cudaSuccess)
+            return NTB_OK;
+        cudaGetLastError();
+        return NTB_ERR_CUDA;
+    }
     SortParams s;
     memset(&s, 0, sizeof(s));
     s.ids = ids;
@@ -673,9 +941,7 @@ extern "C" int ntb_embedding_grad(int devID, void * stream, const int * ids, con
     s.bits = (keyBits + s.passes - 1) / s.passes;
     s.bits = s.bits < 2 ? 2 : s.bits;                       /* counters are cleared four at a time */
     s.ctas = SortCtas(tokens);
-    int grid = tokens > 0 ? s.ctas : 0;
-    if (tokens == 0)
-        s.ctas = 0;
+    int grid = s.ctas;
     const int size = dtypeW == NTB_X_FLOAT16 ? 2 : 4;
     if (beta == 0.f) {
         s.clear = (unsigned char *)dw;
@@ -683,9 +949,8 @@ extern "C" int ntb_embedding_grad(int devID, void * stream, const int * ids, con
         s.clearPitch = ldw * size;
         s.clearBytes = (long long)dim * size;
         /* whole clusters up to one CTA an SM */
-        const int unit = s.ctas > 0 ? s.ctas : 1;
-        const int extra = (ctx->smCount - grid) / unit * unit;
-        grid += extra > unit ? extra : unit;
+        const int extra = (ctx->smCount - grid) / s.ctas * s.ctas;
+        grid += extra > s.ctas ? extra : s.ctas;
     }
     const int smem = SORT_TILE * (int)sizeof(int2) + SORT_WARPS * (1 << s.bits) * (int)sizeof(int);
     static SmemOptIn optIn;
@@ -695,9 +960,9 @@ extern "C" int ntb_embedding_grad(int devID, void * stream, const int * ids, con
     static ClusterOptIn wide;
     if (s.ctas > 8 && !wide.Ensure((const void *)TokenSortKernel))
         return NTB_ERR_CUDA;
-    cudaError_t err = LaunchClusterPdl(TokenSortKernel, (unsigned)grid, SORT_THREADS, smem, s.ctas > 0 ? s.ctas : 1, st, s);
+    cudaError_t err = LaunchClusterPdl(TokenSortKernel, (unsigned)grid, SORT_THREADS, smem, s.ctas, st, s);
     CountLaunch();
-    if (err == cudaSuccess && tokens > 0) {
+    if (err == cudaSuccess) {
         RunParams p;
         memset(&p, 0, sizeof(p));
         p.sorted = s.a;
