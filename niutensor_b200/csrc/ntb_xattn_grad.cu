@@ -506,7 +506,7 @@ XattnGradKVKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     extern __shared__ __align__(1024) uint8_t kvSmem[];
     struct Bars {
         uint64_t qFull[QSLOTS], qEmpty[QSLOTS], doFull[DOSLOTS], doEmpty[DOSLOTS], statFull[STATSLOTS], statEmpty[STATSLOTS];
-        uint64_t kv, load, s, p, dp, ds, done;
+        uint64_t k, v, load, s, p, dp, ds, done;
         uint32_t tmem;
         int abort;
     };
@@ -541,7 +541,8 @@ XattnGradKVKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
             MbarInit(SmemAddr(&bars.statFull[i]), 1);
             MbarInit(SmemAddr(&bars.statEmpty[i]), 1);
         }
-        MbarInit(SmemAddr(&bars.kv), 1);
+        MbarInit(SmemAddr(&bars.k), 1);
+        MbarInit(SmemAddr(&bars.v), 1);
         MbarInit(SmemAddr(&bars.load), 1);
         MbarInit(SmemAddr(&bars.s), 1);
         MbarInit(SmemAddr(&bars.p), 9);                    /* the softmax warps and the relay */
@@ -580,14 +581,15 @@ XattnGradKVKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     if (warp == GR_PRODUCER) {
         bool ok = true;
         uint32_t edges = 0;
-        if (n > 0 && lane == 0) {
-            MbarExpectTx(SmemAddr(&bars.kv), 2 * TILE);
+        auto loadOwn = [&](const CUtensorMap * map, const HeadsAddr & a, uint32_t dst, uint32_t bar) {
+            if (lane == 0) {
+                MbarExpectTx(bar, TILE);
 #pragma unroll
-            for (int dc = 0; dc < DC; dc++) {
-                TmaLoad4D(kS + dc * XBOX_BYTES, &tmK, SmemAddr(&bars.kv), dc * 64, k0, kvHead * p.aK.mulHead, b * p.aK.mulBatch);
-                TmaLoad4D(vS + dc * XBOX_BYTES, &tmV, SmemAddr(&bars.kv), dc * 64, k0, kvHead * p.aV.mulHead, b * p.aV.mulBatch);
+                for (int dc = 0; dc < DC; dc++)
+                    TmaLoad4D(dst + dc * XBOX_BYTES, map, bar, dc * 64, k0, kvHead * a.mulHead, b * a.mulBatch);
             }
-        }
+            __syncwarp();
+        };
         /* one tile of q or do into its ring; a tile with rows past the sequence arrives on the producer's own barrier,
            has them cleared (their weights are 0, and 0 * NaN would reach the sums), and is handed on by the warp */
         auto load = [&](const CUtensorMap * map, const HeadsAddr & a, int i, uint32_t dst, uint32_t full) {
@@ -639,8 +641,10 @@ XattnGradKVKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         };
         /* in the order of their use: q runs two steps ahead of the sums, do and the rows' numbers one */
         if (n > 0) {
+            loadOwn(&tmK, p.aK, kS, SmemAddr(&bars.k));
             loadQ(0);
             loadStat(0);
+            loadOwn(&tmV, p.aV, vS, SmemAddr(&bars.v));
             loadDO(0);
             if (n > 1)
                 loadQ(1);
@@ -669,12 +673,12 @@ XattnGradKVKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
                     TcMmaTmemA(dst, aTmem + (ks >> 2) * 64 + (ks & 3) * 8, SmemDesc(bTile + ks * 16 * ROW_BYTES, XBOX_BYTES, 1024, 2), descD,
                                !first || ks != 0 ? 1u : 0u);
             };
-            bool ok = WaitNow(SmemAddr(&bars.kv), 0, abortPtr, p.status) && WaitNow(SmemAddr(&bars.qFull[0]), 0, abortPtr, p.status);
+            bool ok = WaitNow(SmemAddr(&bars.k), 0, abortPtr, p.status) && WaitNow(SmemAddr(&bars.qFull[0]), 0, abortPtr, p.status);
             if (ok) {
                 TcFenceAfter();
                 product(tmemBase + TMEM_S, kS, ringS);
                 TcCommit(SmemAddr(&bars.s));
-                ok = WaitNow(SmemAddr(&bars.doFull[0]), 0, abortPtr, p.status);
+                ok = WaitNow(SmemAddr(&bars.v), 0, abortPtr, p.status) && WaitNow(SmemAddr(&bars.doFull[0]), 0, abortPtr, p.status);
             }
             if (ok) {
                 TcFenceAfter();
