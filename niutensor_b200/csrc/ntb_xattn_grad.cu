@@ -506,7 +506,8 @@ XattnGradKVKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     extern __shared__ __align__(1024) uint8_t kvSmem[];
     struct Bars {
         uint64_t qFull[QSLOTS], qEmpty[QSLOTS], doFull[DOSLOTS], doEmpty[DOSLOTS], statFull[STATSLOTS], statEmpty[STATSLOTS];
-        uint64_t k, v, load, s, p, dp, ds, done;
+        uint64_t qRaw[QSLOTS], doRaw[DOSLOTS];               /* loads of tiles with rows to be cleared */
+        uint64_t k, v, s, p, dp, ds, done;
         uint32_t tmem;
         int abort;
     };
@@ -532,10 +533,12 @@ XattnGradKVKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         for (int i = 0; i < QSLOTS; i++) {
             MbarInit(SmemAddr(&bars.qFull[i]), 1);
             MbarInit(SmemAddr(&bars.qEmpty[i]), 1);
+            MbarInit(SmemAddr(&bars.qRaw[i]), 1);
         }
         for (int i = 0; i < DOSLOTS; i++) {
             MbarInit(SmemAddr(&bars.doFull[i]), 1);
             MbarInit(SmemAddr(&bars.doEmpty[i]), 1);
+            MbarInit(SmemAddr(&bars.doRaw[i]), 1);
         }
         for (int i = 0; i < STATSLOTS; i++) {
             MbarInit(SmemAddr(&bars.statFull[i]), 1);
@@ -543,7 +546,6 @@ XattnGradKVKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         }
         MbarInit(SmemAddr(&bars.k), 1);
         MbarInit(SmemAddr(&bars.v), 1);
-        MbarInit(SmemAddr(&bars.load), 1);
         MbarInit(SmemAddr(&bars.s), 1);
         MbarInit(SmemAddr(&bars.p), 9);                    /* the softmax warps and the relay */
         MbarInit(SmemAddr(&bars.dp), 1);
@@ -576,11 +578,12 @@ XattnGradKVKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     const int step0 = rank * perSplit < steps ? rank * perSplit : steps;
     const int step1 = step0 + perSplit < steps ? step0 + perSplit : steps;
     const int n = step1 - step0;
-    const bool ragged = nq < p.sh.lenQ && nq % XT != 0;       /* a head's last query tile reaches into rows past the sequence */
+    /* a head's last query tile may reach into rows past the sequence */
+    const bool ragged = nq < p.sh.lenQ && nq % XT != 0;
+    auto edge = [&](int i) { return ragged && (step0 + i) % qTiles == qTiles - 1; };
 
     if (warp == GR_PRODUCER) {
         bool ok = true;
-        uint32_t edges = 0;
         auto loadOwn = [&](const CUtensorMap * map, const HeadsAddr & a, uint32_t dst, uint32_t bar) {
             if (lane == 0) {
                 MbarExpectTx(bar, TILE);
@@ -590,12 +593,11 @@ XattnGradKVKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
             }
             __syncwarp();
         };
-        /* one tile of q or do into its ring; a tile with rows past the sequence arrives on the producer's own barrier,
-           has them cleared (their weights are 0, and 0 * NaN would reach the sums), and is handed on by the warp */
-        auto load = [&](const CUtensorMap * map, const HeadsAddr & a, int i, uint32_t dst, uint32_t full) {
+        /* one tile of q or do into its ring; a tile with rows past the sequence arrives on a barrier of its own, and the
+           relay hands it on */
+        auto load = [&](const CUtensorMap * map, const HeadsAddr & a, int i, uint32_t dst, uint32_t full, uint32_t raw) {
             const int step = step0 + i, g = step / qTiles, qt = step - g * qTiles, h = kvHead * p.sh.group + g;
-            const bool edge = ragged && qt == qTiles - 1;
-            const uint32_t bar = edge ? SmemAddr(&bars.load) : full;
+            const uint32_t bar = edge(i) ? raw : full;
             if (lane == 0) {
                 MbarExpectTx(bar, TILE);
 #pragma unroll
@@ -603,28 +605,18 @@ XattnGradKVKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
                     TmaLoad4D(dst + dc * XBOX_BYTES, map, bar, dc * 64, qt * XT, h * a.mulHead, b * a.mulBatch);
             }
             __syncwarp();
-            if (edge) {
-                ok = WaitNowWarp(bar, edges++ & 1u, abortPtr, p.status);
-                if (!ok)
-                    return;
-                ZeroTileRows(dst, DC, nq - qt * XT, lane);
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                __syncwarp();
-                if (lane == 0)
-                    MbarArrive(full);
-            }
         };
         auto loadQ = [&](int i) {
             if (i >= QSLOTS)
                 ok = ok && MbarWaitWarp(SmemAddr(&bars.qEmpty[i % QSLOTS]), (uint32_t)(i / QSLOTS + 1) & 1u, abortPtr, p.status, 200);
             if (ok)
-                load(&tmQ, p.aQ, i, ringS + (i % QSLOTS) * TILE, SmemAddr(&bars.qFull[i % QSLOTS]));
+                load(&tmQ, p.aQ, i, ringS + (i % QSLOTS) * TILE, SmemAddr(&bars.qFull[i % QSLOTS]), SmemAddr(&bars.qRaw[i % QSLOTS]));
         };
         auto loadDO = [&](int i) {
             if (i >= DOSLOTS)
                 ok = ok && MbarWaitWarp(SmemAddr(&bars.doEmpty[i % DOSLOTS]), (uint32_t)(i / DOSLOTS + 1) & 1u, abortPtr, p.status, 200);
             if (ok)
-                load(&tmDO, p.aDO, i, doRing + (i % DOSLOTS) * TILE, SmemAddr(&bars.doFull[i % DOSLOTS]));
+                load(&tmDO, p.aDO, i, doRing + (i % DOSLOTS) * TILE, SmemAddr(&bars.doFull[i % DOSLOTS]), SmemAddr(&bars.doRaw[i % DOSLOTS]));
         };
         auto loadStat = [&](int i) {
             if (i >= STATSLOTS)
@@ -711,24 +703,44 @@ XattnGradKVKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         }
     }
     else if (warp == GR_RELAY) {
-        /* as in the first kernel: the next step's copies are there */
-        if (lane == 0 && n > 0) {
-            bool ok = true;
-            for (int i = 0; ok && i < n; i++) {
-                if (i + 1 < n)
-                    ok = WaitNow(SmemAddr(&bars.qFull[(i + 1) % QSLOTS]), (uint32_t)((i + 1) / QSLOTS) & 1u, abortPtr, p.status);
-                if (ok && i > 0)
-                    ok = WaitNow(SmemAddr(&bars.p), (uint32_t)(i - 1) & 1u, abortPtr, p.status);
-                if (ok)
-                    MbarArrive(SmemAddr(&bars.p));
-                if (ok && i + 1 < n)
-                    ok = WaitNow(SmemAddr(&bars.doFull[(i + 1) % DOSLOTS]), (uint32_t)((i + 1) / DOSLOTS) & 1u, abortPtr, p.status);
-                if (ok && i > 0)
-                    ok = WaitNow(SmemAddr(&bars.ds), (uint32_t)(i - 1) & 1u, abortPtr, p.status);
-                if (ok)
-                    MbarArrive(SmemAddr(&bars.ds));
-            }
+        /* as in the first kernel: the next step's copies are there, those with rows past the sequence cleared of them
+           (their weights are 0, and 0 * NaN would reach the sums). Done by the producer, that held up the loads behind. */
+        bool ok = true;
+        uint32_t qRound = 0, doRound = 0;                    /* a bit a slot: the phase of its next raw load */
+        auto ready = [&](int i, bool isQ) {
+            const int slot = isQ ? i % QSLOTS : i % DOSLOTS;
+            const uint32_t full = isQ ? SmemAddr(&bars.qFull[slot]) : SmemAddr(&bars.doFull[slot]);
+            if (!edge(i))
+                return MbarWaitWarp(full, (uint32_t)(isQ ? i / QSLOTS : i / DOSLOTS) & 1u, abortPtr, p.status, 0);
+            const uint32_t rounds = isQ ? qRound : doRound;
+            if (!WaitNowWarp(isQ ? SmemAddr(&bars.qRaw[slot]) : SmemAddr(&bars.doRaw[slot]), rounds >> slot & 1u, abortPtr, p.status))
+                return false;
+            if (isQ)
+                qRound ^= 1u << slot;
+            else
+                doRound ^= 1u << slot;
+            ZeroTileRows(isQ ? ringS + slot * TILE : doRing + slot * TILE, DC, nq - (qTiles - 1) * XT, lane);
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            ArriveWarp(full, lane);
+            return true;
+        };
+        if (n > 0 && edge(0))
+            ok = ready(0, true) && ready(0, false);
+        for (int i = 0; ok && i < n; i++) {
+            if (i + 1 < n)
+                ok = ready(i + 1, true);
+            if (ok && i > 0)
+                ok = MbarWaitWarp(SmemAddr(&bars.p), (uint32_t)(i - 1) & 1u, abortPtr, p.status, 0);
+            if (ok)
+                ArriveWarp(SmemAddr(&bars.p), lane);
+            if (ok && i + 1 < n)
+                ok = ready(i + 1, false);
+            if (ok && i > 0)
+                ok = MbarWaitWarp(SmemAddr(&bars.ds), (uint32_t)(i - 1) & 1u, abortPtr, p.status, 0);
+            if (ok)
+                ArriveWarp(SmemAddr(&bars.ds), lane);
         }
+        __syncwarp();
     }
     else {
         const int hf = warp >> 2, sub = warp & 3;
