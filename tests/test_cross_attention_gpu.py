@@ -246,3 +246,17 @@ def test_agrees_with_the_fused_self_attention():
     q, k, v = make(2, 4, 4, 200, 256, 64)
     a, b = ops.CrossAttention(q, k, v), ops.ScaledDotProductAttention(q, k, v)
     assert (a.double() - b.double()).norm() / b.double().norm() <= 2e-3
+
+
+def test_a_last_wave_split_over_the_gpu():
+    """more long items than SMs, the rest of them in a launch of split items"""
+    check(*make(5, 16, 16, 150, 3000, 64))
+    check(*make(10, 16, 16, 200, 2950, 64), kl=lens([2950, 100, 1, 2000, 0, 2950, 129, 64, 2900, 17]))
+
+
+def test_two_devices_are_told_apart():
+    """the tensors' device counts, not the current one"""
+    if torch.cuda.device_count() < 2:
+        pytest.skip("one device")
+    q, k, v = (x.to("cuda:1") for x in make(1, 2, 2, 3, 40, 64))
+    assert ops.CrossAttention(q, k, v).device == q.device

@@ -190,3 +190,9 @@ def test_repeats_streams_and_capture():
     for g, res in graphs:
         for a, b in zip(res, want):
             assert torch.equal(a, b)
+
+
+def test_a_last_wave_split_over_the_gpu():
+    """more items than SMs on either side, the rest of them in a launch of split items"""
+    check(*make(10, 16, 16, 100, 1100, 64))
+    check(*make(10, 16, 16, 1100, 100, 64), ql=lens([1100, 5, 0, 128, 999, 1, 640, 641, 1100, 77]))
