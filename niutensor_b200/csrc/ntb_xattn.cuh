@@ -32,6 +32,23 @@ struct XattnCall {
     float scale;
 };
 
+/* a gradient call after its checks */
+struct XattnGradCall {
+    XattnShape sh;
+    const void * q;
+    const void * k;
+    const void * v;
+    const void * out;
+    const void * dout;
+    const float * lse;
+    void * dq;
+    void * dk;
+    void * dv;
+    float * work;
+    const ntb_heads_layout * l;      /* q, k, v, out, dout, dq, dk, dv */
+    float scale;
+};
+
 constexpr int XATTN_STEP_ROWS = 32;      /* query rows a key head up to which the step kernel is used */
 
 namespace {

@@ -29,6 +29,8 @@
 
 namespace ntb {
 
+int LaunchXattnGradStep(const DeviceCtx & ctx, const XattnGradCall & call, cudaStream_t stream);
+
 namespace {
 
 constexpr int GR_THREADS = 352;
@@ -879,22 +881,6 @@ XattnGradKVKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" :: "r"(tmemBase), "r"(512u) : "memory");
 }
 
-struct GradCall {
-    XattnShape sh;
-    const void * q;
-    const void * k;
-    const void * v;
-    const void * out;
-    const void * dout;
-    const float * lse;
-    void * dq;
-    void * dk;
-    void * dv;
-    float * work;
-    const ntb_heads_layout * l;      /* q, k, v, out, dout, dq, dk, dv */
-    float scale;
-};
-
 /* CTAs of a cluster that share one item's walk: until one wave is full, while a part keeps two steps; and parts
    short enough that the tensor core's accumulator, which rounds toward zero at every instruction, stays good */
 int GradSplits(long long items, int steps, int smCount)
@@ -929,7 +915,7 @@ int PlanGrad(long long items, int steps, int smCount, GradPlan * plan)
 }
 
 template <int D>
-int LaunchGrad(const DeviceCtx & ctx, const GradCall & call, cudaStream_t stream)
+int LaunchGrad(const DeviceCtx & ctx, const XattnGradCall & call, cudaStream_t stream)
 {
     using SM = XattnGradSmem<D>;
     const XattnShape & s = call.sh;
@@ -1020,7 +1006,7 @@ extern "C" int ntb_cross_attention_grad(int devID, void * stream, const void * q
                                         int dtype, int batch, int headsQ, int headsKV, int lenQ, int lenK, int dim,
                                         const ntb_heads_layout * layouts, const int * queryLens, const int * keyLens, float scale)
 {
-    GradCall call;
+    XattnGradCall call;
     memset(&call, 0, sizeof(call));
     int rc = XattnShapeOf(call.sh, dtype, batch, headsQ, headsKV, lenQ, lenK, dim, queryLens, keyLens, scale);
     if (rc != NTB_OK)
@@ -1048,7 +1034,10 @@ extern "C" int ntb_cross_attention_grad(int devID, void * stream, const void * q
     DeviceCtx * ctx = CtxFor(devID);
     if (!ctx)
         return NTB_ERR_CUDA;
-    rc = dim <= 64 ? LaunchGrad<64>(*ctx, call, (cudaStream_t)stream) : LaunchGrad<128>(*ctx, call, (cudaStream_t)stream);
+    if (lenQ > 0 && (long long)call.sh.group * lenQ <= XATTN_STEP_ROWS)
+        rc = LaunchXattnGradStep(*ctx, call, (cudaStream_t)stream);
+    else
+        rc = dim <= 64 ? LaunchGrad<64>(*ctx, call, (cudaStream_t)stream) : LaunchGrad<128>(*ctx, call, (cudaStream_t)stream);
     if (rc == NTB_ERR_CUDA)
         cudaGetLastError();
     return rc;

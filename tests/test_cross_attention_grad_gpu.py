@@ -196,3 +196,48 @@ def test_a_last_wave_split_over_the_gpu():
     """more items than SMs on either side, the rest of them in a launch of split items"""
     check(*make(10, 16, 16, 100, 1100, 64))
     check(*make(10, 16, 16, 1100, 100, 64), ql=lens([1100, 5, 0, 128, 999, 1, 640, 641, 1100, 77]))
+
+
+@pytest.mark.parametrize("shape", [
+    (1, 1, 1, 1, 63, 8), (2, 2, 2, 15, 64, 64), (2, 4, 2, 8, 65, 128), (1, 6, 2, 5, 128, 104), (2, 16, 1, 2, 129, 64), (1, 8, 1, 4, 1000, 128),
+    (3, 3, 3, 32, 260, 128), (2, 2, 2, 17, 4097, 72), (1, 2, 2, 11, 9000, 40), (60, 8, 8, 15, 243, 104), (1, 4, 4, 32, 1, 128),
+])
+@pytest.mark.parametrize("split", [False, True])
+def test_few_rows(shape, split):
+    check(*make(*shape, split=split), split=split)
+
+
+@pytest.mark.parametrize("shape,ql,kl", [
+    ((6, 2, 2, 15, 300, 64), [15, 0, 1, 14, 8, 7], [300, 10, 0, 128, 127, 1]),
+    ((5, 6, 2, 9, 200, 128), [9, 1, 5, 0, 8], [200, 100, 3, 50, 0]),
+    ((2, 8, 1, 4, 5000, 104), [4, 3], [4400, 1]),                                 # a split walk whose second sentence ends in its first part
+    ((3, 1, 1, 32, 90, 32), [-4, 99, 30], [90, -1, 1000]),
+    ((2, 4, 4, 3, 700, 128), None, [640, 65]),
+])
+def test_few_rows_with_lengths_and_garbage_behind_them(shape, ql, kl):
+    for split in (False, True):
+        q, k, v = make(*shape, split=split)
+        tq, tk = None if ql is None else lens(ql), lens(kl)
+        out, lse, do, clean = check(q, k, v, tq, tk, split=split)
+        out = out.clone()
+        for b, length in enumerate(kl):
+            k[b, :, max(0, length):], v[b, :, max(0, length):] = NAN, INF
+            if ql is not None:
+                for x in (q, do, out):
+                    x[b, :, max(0, ql[b]):] = NAN
+        for a, c in zip(ops.GradCrossAttention(q, k, v, out, lse, do, tq, tk), clean):
+            assert torch.equal(a, c)
+
+
+@pytest.mark.parametrize("rows", [6, 200])
+def test_a_row_that_is_infinite(rows):
+    """in one sentence it leaves the others, and the keys behind its end, alone"""
+    q, k, v = make(3, 2, 2, rows, 100, 64)
+    tk = lens([70, 70, 70])
+    out, lse, do, clean = check(q, k, v, None, tk)
+    do = do.clone()
+    do[1, :, 2] = INF
+    got = ops.GradCrossAttention(q, k, v, out, lse, do, None, tk)
+    for a, c in zip(got, clean):
+        assert torch.equal(a[0], c[0]) and torch.equal(a[2], c[2])
+    assert (got[1][1, :, 70:] == 0).all() and (got[2][1, :, 70:] == 0).all()
