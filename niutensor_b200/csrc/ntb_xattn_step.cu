@@ -413,11 +413,15 @@ struct StepGradParams {
     int * status;
 };
 
+/* Four warps, one of which also starts the loads: a fifth would leave the sub-partition that gets two of them to set
+   the registers of all (168 for two CTAs an SM instead of 255). */
+constexpr int SG_THREADS = 128;
+
 template <int D, int MT> struct StepGradSmem {
     static constexpr int DC = D / 64;
     static constexpr int ROWS_BYTES = DC * MT * 16 * ROW_BYTES;       /* q, or do */
     static constexpr int TILE = DC * ST_BOX;
-    static constexpr int STAGES = D == 64 ? 4 : 3;        /* a stage comes free a tile late, when its stores have read it */
+    static constexpr int STAGES = 2;
     static constexpr int RESIDENT = 2;
     static constexpr int RING_BYTES = STAGES * 2 * TILE;
     static constexpr int PART_BYTES = 4 * MT * 16 * D * 4;
@@ -432,7 +436,7 @@ __device__ __forceinline__ uint32_t MoveTrans(uint32_t x)
 }
 
 template <int D, int MT>
-__global__ void __launch_bounds__(ST_THREADS, D * MT > 128 ? 1 : 2)
+__global__ void __launch_bounds__(SG_THREADS, MT == 1 ? 3 : 2)
 XattnGradStepKernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmDK,
                     const __grid_constant__ CUtensorMap tmDV, const StepGradParams p)
 {
@@ -448,7 +452,7 @@ XattnGradStepKernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
     const uint32_t ring = base, qS = base + (SM::TOTAL - 1024 - 2 * SM::ROWS_BYTES), doS = qS + SM::ROWS_BYTES;
     volatile int * abortPtr = &abortFlag;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    if (threadIdx.x == 128) {
+    if (threadIdx.x == 0) {
         PrefetchTensorMap(&tmK);
         PrefetchTensorMap(&tmV);
         PrefetchTensorMap(&tmDK);
@@ -477,30 +481,24 @@ XattnGradStepKernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
     /* all keys in this CTA's ring: delta from the weights (ntb_xattn_grad.cu says why) */
     const bool resident = tiles <= SM::RESIDENT && p.splits == 1;
 
-    if (warp == 4) {
-        if (lane == 0) {
-            bool ok = true;
-            for (int j = 0; ok && j < n; j++) {
-                const int st = j % STAGES;
-                if (j >= STAGES)
-                    ok = MbarWait(SmemAddr(&barEmpty[st]), (uint32_t)(j / STAGES + 1) & 1u, abortPtr, p.status);
-                if (!ok)
-                    break;
-                const uint32_t bar = SmemAddr(&barFull[st]), dst = ring + st * 2 * SM::TILE;
-                const int row = (tile0 + j) * ST_KEYS;
-                MbarExpectTx(bar, 2 * SM::TILE);
+    /* the first thread's: tile j into its stage */
+    auto load = [&](int j) {
+        const int st = j % STAGES, row = (tile0 + j) * ST_KEYS;
+        const uint32_t bar = SmemAddr(&barFull[st]), dst = ring + st * 2 * SM::TILE;
+        MbarExpectTx(bar, 2 * SM::TILE);
 #pragma unroll
-                for (int dc = 0; dc < DC; dc++) {
-                    TmaLoad4D(dst + dc * ST_BOX, &tmK, bar, dc * 64, row, kvHead * p.aK.mulHead, b * p.aK.mulBatch);
-                    TmaLoad4D(dst + SM::TILE + dc * ST_BOX, &tmV, bar, dc * 64, row, kvHead * p.aV.mulHead, b * p.aV.mulBatch);
-                }
-            }
+        for (int dc = 0; dc < DC; dc++) {
+            TmaLoad4D(dst + dc * ST_BOX, &tmK, bar, dc * 64, row, kvHead * p.aK.mulHead, b * p.aK.mulBatch);
+            TmaLoad4D(dst + SM::TILE + dc * ST_BOX, &tmV, bar, dc * 64, row, kvHead * p.aV.mulHead, b * p.aV.mulBatch);
         }
-        __syncwarp();
-    }
-    else {
+    };
+    if (threadIdx.x == 0)
+        for (int j = 0; j < STAGES && j < n; j++)
+            load(j);
+    __syncwarp();
+    {
         /* the rows of q and do into swizzled tiles, delta and lse beside them */
-        for (int r = threadIdx.x >> 3; r < R; r += 16) {
+        for (int r = threadIdx.x >> 3; r < R; r += SG_THREADS / 8) {
             const int part = threadIdx.x & 7;                          /* eight threads a row, 16 bytes each */
             const int g = r / p.sh.lenQ, i = r - g * p.sh.lenQ, h = kvHead * p.sh.group + g;
             const bool live = r < p.rows && i < nq && nk > 0;
@@ -534,11 +532,11 @@ XattnGradStepKernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
                 sLse[r] = live ? p.lse[((long long)b * p.sh.headsQ + h) * p.sh.lenQ + i] * LOG2E : INFINITY;
             }
         }
-        asm volatile("bar.sync 1, 128;" ::: "memory");
     }
+    __syncthreads();
 
     float dq[MT][D / 8][4];
-    if (warp < 4) {
+    {
 #pragma unroll
         for (int mt = 0; mt < MT; mt++)
 #pragma unroll
@@ -621,7 +619,7 @@ XattnGradStepKernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
                     if ((lane & 3) == 0)
                         sSum[warp][mt * 16 + hf * 8 + (lane >> 2)] = sum[mt][hf];
                 }
-            asm volatile("bar.sync 1, 128;" ::: "memory");
+            __syncthreads();
 #pragma unroll
             for (int mt = 0; mt < MT; mt++)
 #pragma unroll
@@ -632,6 +630,13 @@ XattnGradStepKernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
         }
         for (int j = 0; ok && j < n; j++) {
             const int st = j % STAGES;
+            if (warp == 0 && j > 0 && j - 1 + STAGES < n) {
+                /* the tile before has been left by all: the one STAGES behind it takes its place */
+                const int before = j - 1;
+                if (lane == 0 && MbarWait(SmemAddr(&barEmpty[before % STAGES]), (uint32_t)(before / STAGES) & 1u, abortPtr, p.status))
+                    load(before + STAGES);
+                __syncwarp();
+            }
             ok = MbarWaitWarp(SmemAddr(&barFull[st]), (uint32_t)(j / STAGES) & 1u, abortPtr, p.status, 200);
             if (!ok)
                 break;
@@ -715,14 +720,11 @@ XattnGradStepKernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
                     }
                 }
                 asm volatile("cp.async.bulk.commit_group;" ::: "memory");
-                asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
-                if (j > 0)
-                    MbarArrive(SmemAddr(&barEmpty[(j - 1) % STAGES]));
+                asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+                MbarArrive(SmemAddr(&barEmpty[st]));
             }
             __syncwarp();
         }
-        if (lane == 0)
-            asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
     }
     if (*abortPtr) {
         const long long t0 = clock64();
@@ -730,7 +732,7 @@ XattnGradStepKernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
     }
     __syncthreads();                          /* the ring is idle */
     float * part = (float *)(smemRaw + (ring - SmemAddr(smemRaw)));       /* [warp][row][D] */
-    if (warp < 4) {
+    {
 #pragma unroll
         for (int mt = 0; mt < MT; mt++)
 #pragma unroll
@@ -742,7 +744,7 @@ XattnGradStepKernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
                 }
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < p.rows * (D / 4); i += ST_THREADS) {
+    for (int i = threadIdx.x; i < p.rows * (D / 4); i += SG_THREADS) {
         const int r = i / (D / 4), c = (i - r * (D / 4)) * 4;
         float4 a = *(const float4 *)(part + r * D + c);
 #pragma unroll
@@ -757,7 +759,7 @@ XattnGradStepKernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
     else
         __syncthreads();
     const int chunks = D / 8;
-    for (int i = rank * ST_THREADS + threadIdx.x; i < p.rows * chunks; i += p.splits * ST_THREADS) {
+    for (int i = rank * SG_THREADS + threadIdx.x; i < p.rows * chunks; i += p.splits * SG_THREADS) {
         const int r = i / chunks, c = (i - r * chunks) * 8;
         const int g = r / p.sh.lenQ, iq = r - g * p.sh.lenQ, h = kvHead * p.sh.group + g;
         if (c >= p.sh.dim)
@@ -780,7 +782,7 @@ XattnGradStepKernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
     }
     /* keys behind the last tile */
     const int behind = tiles * ST_KEYS < p.sh.lenK ? p.sh.lenK - tiles * ST_KEYS : 0, per = p.sh.dim / 8;
-    for (long long i = rank * ST_THREADS + threadIdx.x; i < (long long)behind * per; i += p.splits * ST_THREADS) {
+    for (long long i = rank * SG_THREADS + threadIdx.x; i < (long long)behind * per; i += p.splits * SG_THREADS) {
         const long long row = tiles * ST_KEYS + i / per;
         const int c = (int)(i % per) * 8;
         *(uint4 *)(p.dk + b * p.lDK.batch + kvHead * p.lDK.head + row * p.lDK.row + c) = make_uint4(0u, 0u, 0u, 0u);
@@ -815,7 +817,7 @@ int LaunchGradStep(const XattnGradCall & call, const StepGradParams & base, cuda
     if (!optIn.Ensure((const void *)XattnGradStepKernel<D, MT>, SM::TOTAL))
         return NTB_ERR_CUDA;
     const unsigned grid = (unsigned)((long long)p.sh.batch * p.sh.headsKV * p.splits);
-    const cudaError_t err = LaunchClusterPdl(XattnGradStepKernel<D, MT>, grid, ST_THREADS, SM::TOTAL, p.splits, stream, tmK, tmV, tmDK, tmDV, p);
+    const cudaError_t err = LaunchClusterPdl(XattnGradStepKernel<D, MT>, grid, SG_THREADS, SM::TOTAL, p.splits, stream, tmK, tmV, tmDK, tmDV, p);
     CountLaunch();
     return (err == cudaSuccess && cudaGetLastError() == cudaSuccess) ? NTB_OK : NTB_ERR_CUDA;
 }
