@@ -8,7 +8,7 @@
  * four warps works on 16 keys of every tile with mma.sync (16 x 8 x 16: the row count that fits;
  * a tcgen05 tile would be 128 rows, mostly empty, and the tensor pipe is idle most of the time either
  * way). The weights go from the first product's accumulators straight into the second's A operand.
- * Warps join their sums through shared memory, the CTAs of a cluster (1 to 8, or 16) through
+ * Warps join their sums through shared memory, the CTAs of a cluster (1 to 8) through
  * distributed shared memory, in a fixed order: one launch, no workspace, no atomics.
  *
  * XattnGradStepKernel is the backward pass of such calls (training on short targets): every warp makes dk and dv of
@@ -835,6 +835,26 @@ int StepSplits(const DeviceCtx & ctx, const XattnShape & s)
 
 }
 
+/* Gradients: the parts with the shortest walk in tiles, over the waves that the GPU's places make of them. A CTA's
+   rows, first loads and sums cost it about four tiles. (64 x 8 heads) x 16 x 1000 x 128 in two parts takes 110 us, in
+   one 119; (20 x 16) x 16 x 2000 x 128 in one 123, in four 137. */
+int GradStepSplits(const DeviceCtx & ctx, const XattnShape & s, int places)
+{
+    const long long heads = (long long)s.batch * s.headsKV;
+    const int tiles = (s.lenK + ST_KEYS - 1) / ST_KEYS;
+    long long best = 0;
+    int splits = 1;
+    for (int n = 1; n == 1 || (n <= 8 && tiles >= 2 * n); n *= 2) {
+        const long long slots = (long long)places * ctx.smCount;
+        const long long cost = (heads * n + slots - 1) / slots * ((tiles + n - 1) / n + 4);
+        if (n == 1 || cost < best) {
+            best = cost;
+            splits = n;
+        }
+    }
+    return splits;
+}
+
 int LaunchXattnGradStep(const DeviceCtx & ctx, const XattnGradCall & call, cudaStream_t stream)
 {
     const XattnShape & s = call.sh;
@@ -858,7 +878,7 @@ int LaunchXattnGradStep(const DeviceCtx & ctx, const XattnGradCall & call, cudaS
     p.scale = call.scale;
     p.scaleLog2 = call.scale * LOG2E;
     p.status = ctx.status;
-    p.splits = StepSplits(ctx, s);
+    p.splits = GradStepSplits(ctx, s, p.rows > 16 ? 2 : 3);
     if ((long long)s.batch * s.headsKV * p.splits > 0x7fffffffLL)
         return NTB_ERR_LIMIT;
     const bool two = p.rows > 16;
