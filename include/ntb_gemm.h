@@ -152,7 +152,7 @@ int ntb_attention_dropout(int devID, void * stream,
  * (source/sample/transformer/submodel/Attention.cpp:198-206). Rows are dense; bases and strides are
  * multiples of 16 bytes (the stride of an extent of one may be anything), else NTB_ERR_ARG; a batch or
  * head stride of 0 broadcasts q, k or v. dim: a multiple of 8 up to 128, else NTB_ERR_LIMIT.
- * dtype X_FLOAT16, else NTB_ERR_DTYPE. scale: positive and finite.
+ * dtype X_FLOAT16, else NTB_ERR_DTYPE. scale: positive, at most 2e38.
  *
  * queryLens, keyLens: device arrays of `batch` ints, or NULL for whole lengths; values are clamped to
  * [0, lenQ] and [0, lenK]. They stand for the padding masks of a batch of sentences: rows of q, k and v
@@ -181,7 +181,8 @@ int ntb_cross_attention(int devID, void * stream,
  * the forward call's. Rows past a sequence's end may hold anything in q, k, v, out and dout, and get zeros in
  * dq, dk, dv. work: device scratch of ntb_cross_attention_grad_work() bytes on a 16-byte boundary, the
  * caller's, so that calls on several streams or in several captured graphs do not share it; its content
- * need not survive the call. No atomics: results do not depend on timing. The reference has no such
+ * need not survive the call (calls with at most 32 query rows for a key head do without, and read k and v once).
+ * No atomics: results do not depend on timing. The reference has no such
  * node; its backward pass runs the chain's own (source/network/XBackwardMath.cpp:714-786 for the products).
  */
 long long ntb_cross_attention_grad_work(int batch, int headsQ, int lenQ);
@@ -245,7 +246,7 @@ int ntb_embedding_grad(int devID, void * stream, const int * ids, const void * d
  *
  * grads, out, dtypes, counts: HOST arrays of `count` entries (device pointers, X_FLOAT16 or X_FLOAT, element
  * counts); out[i] may be grads[i] (in place); different entries must not overlap. norm: one float on the
- * device. A norm that is not finite leaves the gradients' values as they are (the caller reads *norm and skips
+ * device. A norm that is not finite (as a float) leaves the gradients' values as they are (the caller reads *norm and skips
  * the step); maxNorm infinite only takes the norm. maxNorm must not be negative or NaN. The sum is
  * fp64 (fp32 within eight exact products of halves); its order is fixed by the sizes. work: device scratch
  * of ntb_clip_grad_norm_work(count) bytes on an 8-byte boundary, the caller's. The arrays are read before

@@ -49,7 +49,10 @@ struct XattnGradCall {
     float scale;
 };
 
-constexpr int XATTN_STEP_ROWS = 32;      /* query rows a key head up to which the step kernel is used */
+/* Query rows a key head up to which the kernels of 16-row tiles are used: two tiles are what a warp's registers hold.
+   The others pad to 128 rows. Gradients of 32 rows, us, here / there: 64 x 8 heads, 64 keys of 64 15 / 44; 200 of 128
+   48 / 88; 1000 of 128 120 / 283; one head, 8192 keys of 64 28 / 22 (here at most eight CTAs share a head). */
+constexpr int XATTN_STEP_ROWS = 32;
 
 namespace {
 
@@ -196,12 +199,6 @@ __device__ __forceinline__ uint64_t Add2(uint64_t a, uint64_t b)
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
     return r;
 }
-__device__ __forceinline__ uint64_t Mul2(uint64_t a, uint64_t b)
-{
-    uint64_t r;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
 
 __device__ __forceinline__ uint32_t PackHalf2(float lo, float hi)
 {
@@ -319,7 +316,7 @@ inline int XattnShapeOf(XattnShape & s, int dtype, int batch, int headsQ, int he
         return NTB_ERR_ARG;
     if (dtype != NTB_X_FLOAT16)
         return NTB_ERR_DTYPE;
-    if (!(scale > 0.f) || scale > 3.0e38f)
+    if (!(scale > 0.f) || scale > 2.0e38f)                       /* times log2 e it is finite, too */
         return NTB_ERR_ARG;
     if (headsQ > 0 && (headsKV == 0 || headsQ % headsKV != 0))
         return NTB_ERR_SHAPE;

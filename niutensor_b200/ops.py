@@ -271,7 +271,7 @@ def _cross_attention_checks(q, k, v, query_lens, key_lens, scale, others=()):
             _check(lens.get_device() == dev and lens.dtype is torch.int32 and lens.is_contiguous() and lens.dim() == 1 and lens.numel() == qs[0],
                    "lengths must be a packed int32 CUDA vector with one entry a sentence")
     scale = 1.0 / (d ** 0.5) if scale is None else float(scale)
-    _check(0.0 < scale < 3.0e38, "the scale must be positive and finite")
+    _check(0.0 < scale <= 2.0e38, "the scale must be positive and finite")
     return dev, qs, ks, scale
 
 

@@ -144,3 +144,11 @@ def test_repeats_streams_and_capture():
     for _, res in graphs:
         for a, b in zip(res, [n] + want):
             assert torch.equal(a, b)
+
+
+def test_a_norm_past_a_float():
+    """it reads as infinite, so the values stay as they are"""
+    x = torch.full((5,), 3.0e38, device=DEV)
+    out = torch.empty_like(x)
+    assert math.isinf(ops.ClipGradNorm([x], 1.0, out=[out]).item()) and torch.equal(out, x)
+    assert math.isinf(ops.ClipGradNorm([x], 1.0).item()) and (x == 3.0e38).all()
