@@ -181,7 +181,7 @@ int ntb_cross_attention(int devID, void * stream,
  * the forward call's. Rows past a sequence's end may hold anything in q, k, v, out and dout, and get zeros in
  * dq, dk, dv. work: device scratch of ntb_cross_attention_grad_work() bytes on a 16-byte boundary, the
  * caller's, so that calls on several streams or in several captured graphs do not share it; its content
- * need not survive the call (calls with at most 32 query rows for a key head do without, and read k and v once).
+ * need not survive the call (calls with few query rows for a key head or few keys do without, and read all once).
  * No atomics: results do not depend on timing. The reference has no such
  * node; its backward pass runs the chain's own (source/network/XBackwardMath.cpp:714-786 for the products).
  */

@@ -50,7 +50,7 @@ struct XattnGradCall {
 };
 
 /* Query rows a key head up to which the kernels of 16-row tiles are used: two tiles are what a warp's registers hold.
-   The others pad to 128 rows. Gradients of 32 rows, us, here / there: 64 x 8 heads, 64 keys of 64 15 / 44; 200 of 128
+   The others pad to 128 rows. Gradients of 32 rows, us, here / there: 64 x 8 heads, 200 keys of 128
    48 / 88; 1000 of 128 120 / 283; one head, 8192 keys of 64 28 / 22 (here at most eight CTAs share a head). */
 constexpr int XATTN_STEP_ROWS = 32;
 
@@ -225,6 +225,33 @@ __device__ __forceinline__ void ZeroTileRows(uint32_t tile, int boxes, int from,
     for (int box = 0; box < boxes; box++)
         for (int i = lane; i < n; i += 32)
             StoreShared16(tile + box * XBOX_BYTES + from * ROW_BYTES + i * 16, 0u, 0u, 0u, 0u);
+}
+
+/* D += A B of one warp, 16 x 8 x 16 halves, and the loads of its operands */
+__device__ __forceinline__ void Mma16816(float * c, const uint32_t * a, uint32_t b0, uint32_t b1)
+{
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ void LdMatrix4(uint32_t * r, uint32_t addr)
+{
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+
+__device__ __forceinline__ void LdMatrix4Trans(uint32_t * r, uint32_t addr)
+{
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+
+/* an 8 x 8 block of halves over a warp's lanes, transposed */
+__device__ __forceinline__ uint32_t MoveTrans(uint32_t x)
+{
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
 }
 
 __device__ __forceinline__ void ClusterSync()

@@ -5,7 +5,8 @@
  *     dv_j = sum_i p_ij do_i           dp_ij = do_i . v_j        delta_i = do_i . out_i
  *     ds_ij = p_ij (dp_ij - delta_i)   dq_i = scale sum_j ds_ij k_j   dk_j = scale sum_i ds_ij q_i
  *
- * Two kernels, because the sums over j and over i run along different sides of the same score tiles and
+ * Calls with few query rows or few keys go to the kernels of ntb_xattn_step.cu and ntb_xattn_short.cu. Here:
+ * two kernels, because the sums over j and over i run along different sides of the same score tiles and
  * one kernel for both would have to add to dq with atomics, in an order that changes from run to run:
  *
  * XattnGradQKernel: a CTA owns a 128-row query tile of one head and walks the key tiles: S = q k^T,
@@ -35,6 +36,8 @@
 namespace ntb {
 
 int LaunchXattnGradStep(const DeviceCtx & ctx, const XattnGradCall & call, cudaStream_t stream);
+bool XattnGradIsShort(const DeviceCtx & ctx, const XattnShape & s);
+int LaunchXattnGradShort(const DeviceCtx & ctx, const XattnGradCall & call, cudaStream_t stream);
 
 namespace {
 
@@ -1039,7 +1042,9 @@ extern "C" int ntb_cross_attention_grad(int devID, void * stream, const void * q
     DeviceCtx * ctx = CtxFor(devID);
     if (!ctx)
         return NTB_ERR_CUDA;
-    if (lenQ > 0 && (long long)call.sh.group * lenQ <= XATTN_STEP_ROWS)
+    if (XattnGradIsShort(*ctx, call.sh))
+        rc = LaunchXattnGradShort(*ctx, call, (cudaStream_t)stream);
+    else if (lenQ > 0 && (long long)call.sh.group * lenQ <= XATTN_STEP_ROWS)
         rc = LaunchXattnGradStep(*ctx, call, (cudaStream_t)stream);
     else
         rc = dim <= 64 ? LaunchGrad<64>(*ctx, call, (cudaStream_t)stream) : LaunchGrad<128>(*ctx, call, (cudaStream_t)stream);

@@ -52,24 +52,6 @@ template <int D, int MT> struct StepSmem {
     static constexpr int TOTAL = (RING_BYTES > PART_BYTES ? RING_BYTES : PART_BYTES) + 1024;
 };
 
-__device__ __forceinline__ void Mma16816(float * c, const uint32_t * a, uint32_t b0, uint32_t b1)
-{
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-
-__device__ __forceinline__ void LdMatrix4(uint32_t * r, uint32_t addr)
-{
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
-}
-
-__device__ __forceinline__ void LdMatrix4Trans(uint32_t * r, uint32_t addr)
-{
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
-}
-
 template <int D, int MT>
 __global__ void __launch_bounds__(ST_THREADS)
 XattnStepKernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const StepParams p)
@@ -431,13 +413,6 @@ template <int D, int MT> struct StepGradSmem {
     static constexpr int PART_BYTES = 4 * MT * 16 * D * 4;
     static constexpr int TOTAL = 2 * ROWS_BYTES + (RING_BYTES > PART_BYTES ? RING_BYTES : PART_BYTES) + 1024;
 };
-
-__device__ __forceinline__ uint32_t MoveTrans(uint32_t x)
-{
-    uint32_t y;
-    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
-    return y;
-}
 
 template <int D, int MT>
 __global__ void __launch_bounds__(SG_THREADS, MT == 1 ? 3 : 2)

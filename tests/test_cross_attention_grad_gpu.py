@@ -229,7 +229,7 @@ def test_few_rows_with_lengths_and_garbage_behind_them(shape, ql, kl):
             assert torch.equal(a, c)
 
 
-@pytest.mark.parametrize("rows", [6, 200])
+@pytest.mark.parametrize("rows", [6, 60, 200])
 def test_a_row_that_is_infinite(rows):
     """in one sentence it leaves the others, and the keys behind its end, alone"""
     q, k, v = make(3, 2, 2, rows, 100, 64)
@@ -241,3 +241,34 @@ def test_a_row_that_is_infinite(rows):
     for a, c in zip(got, clean):
         assert torch.equal(a[0], c[0]) and torch.equal(a[2], c[2])
     assert (got[1][1, :, 70:] == 0).all() and (got[2][1, :, 70:] == 0).all()
+
+
+@pytest.mark.parametrize("shape", [
+    (60, 4, 4, 100, 50, 128), (60, 4, 4, 130, 120, 64), (2, 4, 4, 32, 100, 128), (1, 3, 3, 64, 128, 104), (2, 2, 2, 33, 65, 72), (1, 1, 1, 50, 64, 40),
+    (2, 6, 3, 31, 127, 64), (57, 8, 4, 40, 17, 128), (1, 2, 2, 1, 1, 64), (1, 2, 2, 17, 16, 32), (40, 6, 6, 500, 33, 64), (3, 2, 1, 20, 96, 96),
+])
+@pytest.mark.parametrize("split", [False, True])
+def test_few_keys(shape, split):
+    check(*make(*shape, split=split), split=split)
+
+
+@pytest.mark.parametrize("shape,ql,kl", [
+    ((6, 2, 2, 60, 64, 64), [60, 0, 1, 33, 32, 31], [64, 10, 0, 63, 17, 1]),
+    ((5, 4, 2, 30, 128, 128), [30, 1, 5, 0, 8], [128, 100, 65, 50, 0]),
+    ((80, 3, 3, 150, 60, 104), list(range(71, 151)), list(range(60, -20, -1))),   # no keys or all behind the end, too
+    ((3, 1, 1, 32, 90, 32), [-4, 99, 30], [90, -1, 1000]),
+    ((2, 4, 4, 64, 120, 64), None, [97, 16]),
+])
+def test_few_keys_with_lengths_and_garbage_behind_them(shape, ql, kl):
+    for split in (False, True):
+        q, k, v = make(*shape, split=split)
+        tq, tk = None if ql is None else lens(ql), lens(kl)
+        out, lse, do, clean = check(q, k, v, tq, tk, split=split)
+        out = out.clone()
+        for b, length in enumerate(kl):
+            k[b, :, max(0, length):], v[b, :, max(0, length):] = NAN, INF
+            if ql is not None:
+                for x in (q, do, out):
+                    x[b, :, max(0, ql[b]):] = NAN
+        for a, c in zip(ops.GradCrossAttention(q, k, v, out, lse, do, tq, tk), clean):
+            assert torch.equal(a, c)
