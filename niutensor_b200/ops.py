@@ -299,7 +299,7 @@ def CrossAttention(q, k, v, query_lens=None, key_lens=None, scale=None, out=None
         _check(out.get_device() == dev and out.dtype is torch.float16 and out.shape == qs, "Incorrect tensor sizes!")
     layouts = _heads_layouts(q, k, v, out)
     batch, heads, len_q, d = qs
-    lse = torch.empty(qs[:3], dtype=torch.float32, device=q.device) if with_lse else None
+    lse = q.new_empty((batch, heads, len_q), dtype=torch.float32) if with_lse else None
     rc = capi.lib().ntb_cross_attention(dev, _raw_stream(dev), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), None if lse is None else lse.data_ptr(),
                                         X_FLOAT16, batch, heads, ks[1], len_q, ks[2], d, layouts.buffer_info()[0],
                                         None if query_lens is None else query_lens.data_ptr(), None if key_lens is None else key_lens.data_ptr(), scale)
