@@ -4,6 +4,8 @@
 `ops`   -- host-side mirror of the reference operators of this path (_MatrixMul,
            _MatrixMul2D, _MatrixMulBatched, MatrixMul, MatrixMulBatched/BMMul) over torch
            CUDA tensors; shape rules and error behaviour follow the reference.
+           What a training or decoding step needs between the products, too: CrossAttention and
+           GradCrossAttention, Embedding and GradEmbedding, ClipGradNorm, LogSoftmax.
 `shard` -- column / batch sharding of one product across the ranks of a process group.
 """
 from . import capi  # noqa: F401
