@@ -20,7 +20,7 @@
  *                     block go straight to dw, pieces of runs that cross an edge to fp32 partial rows.
  *   RunJoinKernel     adds up the pieces of a crossing run, in block order.
  *
- * Up to FEW_TOKENS tokens: FewTokensKernel, one launch without a workspace. The first token of a word finds its
+ * Up to FEW_TOKENS tokens (half as many without 16-byte accesses): FewTokensKernel, one launch without a workspace. The first token of a word finds its
  * others by looking through the list in shared memory and adds their rows; other CTAs meanwhile clear the rows
  * of dw whose words do not occur (beta = 0), known from a bit map of the list.
  *
@@ -487,7 +487,8 @@ __global__ void RunSumKernel(const RunParams p)
 
 /* Whole gradient, us in graph replay, few-tokens kernel / sort and runs, vocabulary 32000 of 512 halves and 5000 of
    1024: 256 tokens 7.2 / 14.4 and 5.3; 1000 8.8 / 16.0 and 7.9; 2048 11.4 / 18.0 and 14.7; 4096 19.8 / 19.4 and
-   30.6 / 23.8 (the search grows with the square of the list). */
+   30.6 / 23.8 (the search grows with the square of the list). Rows without wide accesses (300 halves, 20000 words of
+   513 floats): 1000 tokens 13 / 19 and 16 / 21, 2048 20 / 19 and 26 / 21, so half as many there. */
 constexpr int FEW_TOKENS = 2048;
 constexpr int FEW_THREADS = 256, FEW_WARPS = FEW_THREADS / 32;
 constexpr int FEW_LIST = 24;              /* tokens of a word up to which one warp adds them all */
@@ -808,9 +809,8 @@ bool WideRows(const void * dout, long long ldo, const void * dw, long long ldw, 
 }
 
 template <typename TO, typename TW>
-cudaError_t LaunchRuns(const RunParams & p, cudaStream_t stream)
+cudaError_t LaunchRuns(const RunParams & p, bool vec, cudaStream_t stream)
 {
-    const bool vec = WideRows<TO, TW>(p.dout, p.ldo, p.dw, p.ldw, p.dim);
     const int threadsNeeded = vec ? p.dim / EmVec<TO>::N : p.dim;
     const int block = threadsNeeded >= 256 ? 256 : (threadsNeeded + 31) / 32 * 32;
     cudaLaunchConfig_t cfg = {};
@@ -906,7 +906,9 @@ extern "C" int ntb_embedding_grad(int devID, void * stream, const int * ids, con
         return NTB_ERR_CUDA;
     cudaStream_t st = (cudaStream_t)stream;
     const bool halves = dtypeOut == NTB_X_FLOAT16, halfW = dtypeW == NTB_X_FLOAT16;
-    if (tokens <= FEW_TOKENS) {
+    const bool wide = !halves ? WideRows<float, float>(dout, ldo, dw, ldw, dim)
+        : !halfW ? WideRows<__half, float>(dout, ldo, dw, ldw, dim) : WideRows<__half, __half>(dout, ldo, dw, ldw, dim);
+    if (tokens <= (wide ? FEW_TOKENS : FEW_TOKENS / 2)) {
         FewParams f;
         memset(&f, 0, sizeof(f));
         f.ids = ids;
@@ -922,9 +924,8 @@ extern "C" int ntb_embedding_grad(int devID, void * stream, const int * ids, con
             const int most = 4 * ctx->smCount, want = (vocab + FEW_WARPS - 1) / FEW_WARPS;
             clearing = want < most ? want : most;
         }
-        const cudaError_t e = !halves ? LaunchFew<float, float>(f, WideRows<float, float>(dout, ldo, dw, ldw, dim), clearing, st)
-            : !halfW ? LaunchFew<__half, float>(f, WideRows<__half, float>(dout, ldo, dw, ldw, dim), clearing, st)
-                     : LaunchFew<__half, __half>(f, WideRows<__half, __half>(dout, ldo, dw, ldw, dim), clearing, st);
+        const cudaError_t e = !halves ? LaunchFew<float, float>(f, wide, clearing, st)
+            : !halfW ? LaunchFew<__half, float>(f, wide, clearing, st) : LaunchFew<__half, __half>(f, wide, clearing, st);
         if (e == cudaSuccess && cudaGetLastError() == cudaSuccess)
             return NTB_OK;
         cudaGetLastError();
@@ -960,8 +961,8 @@ extern "C" int ntb_embedding_grad(int devID, void * stream, const int * ids, con
     if (!optIn.Ensure((const void *)TokenSortKernel, SORT_TILE * (int)sizeof(int2) + SORT_WARPS * SORT_RADIX * (int)sizeof(int)))
         return NTB_ERR_CUDA;
     /* clusters of more than 8 CTAs are an opt-in of the kernel's on the device */
-    static ClusterOptIn wide;
-    if (s.ctas > 8 && !wide.Ensure((const void *)TokenSortKernel))
+    static ClusterOptIn large;
+    if (s.ctas > 8 && !large.Ensure((const void *)TokenSortKernel))
         return NTB_ERR_CUDA;
     cudaError_t err = LaunchClusterPdl(TokenSortKernel, (unsigned)grid, SORT_THREADS, smem, s.ctas, st, s);
     CountLaunch();
@@ -979,8 +980,8 @@ extern "C" int ntb_embedding_grad(int devID, void * stream, const int * ids, con
         p.ldo = ldo; p.ldw = ldw;
         p.scale = scale;
         p.accumulate = beta == 1.f;
-        err = dtypeOut == NTB_X_FLOAT ? LaunchRuns<float, float>(p, st)
-            : dtypeW == NTB_X_FLOAT ? LaunchRuns<__half, float>(p, st) : LaunchRuns<__half, __half>(p, st);
+        err = !halves ? LaunchRuns<float, float>(p, wide, st)
+            : !halfW ? LaunchRuns<__half, float>(p, wide, st) : LaunchRuns<__half, __half>(p, wide, st);
     }
     if (err == cudaSuccess && cudaGetLastError() == cudaSuccess)
         return NTB_OK;

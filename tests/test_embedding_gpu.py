@@ -99,6 +99,13 @@ def test_gradient(to, tw, kind, tokens, vocab, d):
     grad_check(ids, do, dw, 0.125, 0.0)
 
 
+@pytest.mark.parametrize("tokens", [1024, 1025, 2048])
+@pytest.mark.parametrize("to,tw", [(F16, F16), (F16, F32), (F32, F32)])
+def test_gradient_of_rows_without_wide_accesses(to, tw, tokens):
+    for kind in ("one", "padded"):
+        test_gradient(to, tw, kind, tokens, 700, 301)
+
+
 def test_gradient_shapes_pitches_and_nothing_at_all():
     g = gen(9)
     for d in (64, 33):
