@@ -252,18 +252,53 @@ __global__ void __launch_bounds__(SORT_THREADS) TokenSortKernel(const SortParams
                 x[u] = u < each && i < count ? load(tile + i) : make_int2(0, 0);
             }
         };
-        if (once)
-            loadTile(lo);
-        if ((int)threadIdx.x < R)
-            totals[threadIdx.x] = 0;
-        __syncthreads();
-        if (once) {
+        int place[SORT_AHEAD];
+        /* ranks of the tile's tokens among those of their digit in the warp's piece, and those of all pieces before it
+           (counters); returns how many tokens the tile has of the thread's digit */
+        auto rankTile = [&]() {
+            for (int i = threadIdx.x; i < SORT_WARPS * R / 4; i += SORT_THREADS)
+                ((int4 *)counters)[i] = make_int4(0, 0, 0, 0);
+            __syncthreads();
 #pragma unroll
-            for (int u = 0; u < SORT_AHEAD; u++)
-                if (u < each && (warp * each + u) * 32 + lane < count)
-                    atomicAdd(totals + digit(x[u]), 1);
+            for (int u = 0; u < SORT_AHEAD; u++) {
+                if (u < each) {
+                    const bool in = (warp * each + u) * 32 + lane < count;
+                    const int d = digit(x[u]);
+                    const unsigned same = SameDigit(d, p.bits, in);
+                    place[u] = mine[d] + __popc(same & before);
+                    __syncwarp();
+                    if (in && (same & before) == 0)
+                        mine[d] += __popc(same);
+                    __syncwarp();
+                }
+            }
+            __syncthreads();
+            int run = 0;
+            if ((int)threadIdx.x < R) {
+                int c[SORT_WARPS];
+#pragma unroll
+                for (int w = 0; w < SORT_WARPS; w++)
+                    c[w] = counters[w * R + threadIdx.x];
+#pragma unroll
+                for (int w = 0; w < SORT_WARPS; w++) {
+                    counters[w * R + threadIdx.x] = run;
+                    run += c[w];
+                }
+            }
+            return run;
+        };
+        int run = 0;
+        if (once) {
+            /* the ranking counts the digits, too */
+            loadTile(lo);
+            run = rankTile();
+            if ((int)threadIdx.x < R)
+                totals[threadIdx.x] = run;
         }
         else {
+            if ((int)threadIdx.x < R)
+                totals[threadIdx.x] = 0;
+            __syncthreads();
             for (long long i0 = lo + threadIdx.x; i0 < hi; i0 += SORT_TILE) {
                 int d[SORT_AHEAD];
 #pragma unroll
@@ -297,37 +332,9 @@ __global__ void __launch_bounds__(SORT_THREADS) TokenSortKernel(const SortParams
             bases[threadIdx.x] = start;
 
         for (long long tile = lo; tile < hi; tile += SORT_TILE) {
-            if (!once)
+            if (!once) {
                 loadTile(tile);
-            int place[SORT_AHEAD];
-            for (int i = threadIdx.x; i < SORT_WARPS * R / 4; i += SORT_THREADS)
-                ((int4 *)counters)[i] = make_int4(0, 0, 0, 0);
-            __syncthreads();
-#pragma unroll
-            for (int u = 0; u < SORT_AHEAD; u++) {
-                if (u < each) {
-                    const bool in = (warp * each + u) * 32 + lane < count;
-                    const int d = digit(x[u]);
-                    const unsigned same = SameDigit(d, p.bits, in);
-                    place[u] = mine[d] + __popc(same & before);
-                    __syncwarp();
-                    if (in && (same & before) == 0)
-                        mine[d] += __popc(same);
-                    __syncwarp();
-                }
-            }
-            __syncthreads();
-            int run = 0;
-            if ((int)threadIdx.x < R) {
-                int c[SORT_WARPS];
-#pragma unroll
-                for (int w = 0; w < SORT_WARPS; w++)
-                    c[w] = counters[w * R + threadIdx.x];
-#pragma unroll
-                for (int w = 0; w < SORT_WARPS; w++) {
-                    counters[w * R + threadIdx.x] = run;
-                    run += c[w];
-                }
+                run = rankTile();
             }
             const int local = BlockScan(run, warpSums[1], warp, lane);
             if ((int)threadIdx.x < R)
