@@ -25,7 +25,10 @@
  * Bound by the steps' products and the shared memory that feeds them, on long walks (2 x 16 query and 4 key heads,
  * 1777 rows, 4100 keys of 128: 405 us, 298 GFLOP of the formulas' five products, 418 of the seven done, 1.03 PFLOP/s;
  * a step takes some 2570 clocks in the first kernel and 3275 in the second), by the loads before an item's first
- * product and the stores behind its last on short ones (64 x 4 heads, 100 to 200 rows and keys of 128: 70 us).
+ * product and the stores behind its last on short ones (64 x 4 heads, 100 to 200 rows and keys of 128: 65 us).
+ *
+ * What a CTA runs once (the rows' way to tensor memory, the results' out of it) is kept in loops: unrolled, its
+ * instructions came from L2 for every tile, 0.5 to 1 us of the 8 a short item takes (sentences 69.4 -> 65.2 us).
  *
  * Rounding: p is at most 1 and may be tiny (1 / lenK); for dv it is rounded to half as 2^12 p, exact powers
  * of two away from half's subnormals. ds is rounded to half as it is: its scale is that of the gradients,
@@ -337,7 +340,7 @@ XattnGradQKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         bool ok = true;
         if (n > 0) {
             ok = WaitNowWarp(SmemAddr(&barRows), 0, abortPtr, p.status);
-#pragma unroll
+#pragma unroll 2
             for (int c = 0; c < D / 16; c++) {
                 const int col = hf * (D / 2) + c * 8;
                 const uint32_t at = ringS + ROWS0 * TILE + (col >> 6) * XBOX_BYTES + r * ROW_BYTES + ((((col >> 3) & 7) ^ (r & 7)) << 4);
@@ -448,7 +451,7 @@ XattnGradQKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         TcFenceAfter();
         const bool sums = n > 0 && ok;
         const uint32_t dqT = tmemBase + laneBase + TMEM_DQ;
-#pragma unroll
+#pragma unroll 1
         for (int c = hf * (D / 64); c < (hf + 1) * (D / 64); c++) {       /* 32 columns a step; this half's D / 2 */
             uint32_t o[32];
             if (sums) {
@@ -830,17 +833,27 @@ XattnGradKVKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         const uint32_t accT = tmemBase + laneBase + (hf == 0 ? TMEM_DV : TMEM_DK);
         const uint32_t box = (hf == 0 ? vS : kS) + sub * 32 * ROW_BYTES;
         const float factor = hf == 0 ? P_SCALE_INV : p.scale;
-#pragma unroll
-        for (int c = 0; c < D / 32; c++) {
-            uint32_t o[32];
-            if (sums) {
-                TmemLoad32Async(accT + c * 32, o);
-                TmemWaitLoad();
-            }
-            if (p.splits == 1)
+        if (p.splits == 1) {
+#pragma unroll 1
+            for (int c = 0; c < D / 32; c++) {
+                uint32_t o[32];
+                if (sums) {
+                    TmemLoad32Async(accT + c * 32, o);
+                    TmemWaitLoad();
+                }
                 StageHalf32(box + (c >> 1) * XBOX_BYTES + lane * ROW_BYTES, lane, (c & 1) * 4, o, factor, sums && rowLive);
-            else
+            }
+        }
+        else {
+#pragma unroll 1
+            for (int c = 0; c < D / 32; c++) {
+                uint32_t o[32];
+                if (sums) {
+                    TmemLoad32Async(accT + c * 32, o);
+                    TmemWaitLoad();
+                }
                 StorePartial(ringS + (hf * XT + r) * D * 4, r, c * 8, o, sums);
+            }
         }
         if (p.splits == 1 && ok) {
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
