@@ -272,3 +272,46 @@ def test_few_keys_with_lengths_and_garbage_behind_them(shape, ql, kl):
                     x[b, :, max(0, ql[b]):] = NAN
         for a, c in zip(ops.GradCrossAttention(q, k, v, out, lse, do, tq, tk), clean):
             assert torch.equal(a, c)
+
+
+@pytest.mark.parametrize("n,m,d", [(3, 300, 64), (20, 150, 128), (40, 60, 64), (30, 100, 128), (64, 128, 128), (150, 300, 64)])
+def test_every_kernel_takes_broadcasts_far_offsets_and_graphs(n, m, d):
+    q, k, v = make(2, 4, 4, n, m, d)
+    kl, ql = lens([m, m // 2]), lens([n - 1, n])
+    # k and v of one sentence for both, then of one head for all
+    for k1, v1 in ((k[:1].expand(2, 4, m, d), v[:1].expand(2, 4, m, d)), (k[:, :1].expand(2, 4, m, d), v[:, :1].expand(2, 4, m, d))):
+        out, lse, do, a = check(q, k1, v1, ql, kl)
+        for x, y in zip(a, ops.GradCrossAttention(q, k1.contiguous(), v1.contiguous(), out, lse, do, ql, kl)):
+            assert torch.equal(x, y)
+    # rows, heads and sentences far apart: the last lie behind 2^31 elements
+    def far(x):
+        rows = x.shape[2]
+        pool = torch.empty(2 ** 31 + 2 ** 27, device=DEV, dtype=torch.float16)
+        view = pool.as_strided((2, 4, rows, d), (2 ** 31 - 4 * 2 ** 20, 2 ** 20, 2 ** 11, 1), pool.numel() - (2 ** 31 + 3 * 2 ** 20))
+        return view.copy_(x)
+    do = torch.nan_to_num(do)
+    out, lse = ops.CrossAttention(q, k, v, ql, kl, with_lse=True)
+    want = ops.GradCrossAttention(q, k, v, out, lse, do, ql, kl)
+    for at in range(2):                                   # three of the five, and the other two: each takes 4.5 GB
+        qs, ks, vs, os, ds = (far(x) if i % 2 == at else x for i, x in enumerate((q, k, v, out, do)))
+        for x, y in zip(ops.GradCrossAttention(qs, ks, vs, os, lse, ds, ql, kl), want):
+            assert torch.equal(x, y)
+        del qs, ks, vs, os, ds
+    # another stream, and two graphs replayed in turn
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        again = ops.GradCrossAttention(q, k, v, out, lse, do, ql, kl)
+    torch.cuda.current_stream().wait_stream(side)
+    graphs = []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            res = ops.GradCrossAttention(q, k, v, out, lse, do, ql, kl)
+        graphs.append((g, res))
+    for g, res in graphs:
+        g.replay()
+    torch.cuda.synchronize()
+    for got in (again, graphs[0][1], graphs[1][1]):
+        for x, y in zip(got, want):
+            assert torch.equal(x, y)
