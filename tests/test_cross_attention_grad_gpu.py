@@ -315,3 +315,12 @@ def test_every_kernel_takes_broadcasts_far_offsets_and_graphs(n, m, d):
     for got in (again, graphs[0][1], graphs[1][1]):
         for x, y in zip(got, want):
             assert torch.equal(x, y)
+
+
+@pytest.mark.parametrize("n,m", [(200, 0), (40, 0), (0, 300), (3, 0)])
+def test_empty_sides_of_other_sizes(n, m):
+    q, k, v = make(2, 4, 2, n, m, 128)
+    out, lse = ops.CrossAttention(q, k, v, with_lse=True)
+    for x, like in zip(ops.GradCrossAttention(q, k, v, out, lse, torch.ones_like(q)), (q, k, v)):
+        assert x.shape == like.shape and (x == 0).all()
+    assert capi.lib().ntb_device_status(0) == capi.OK
