@@ -158,7 +158,8 @@ int ntb_attention_dropout(int devID, void * stream,
  * [0, lenQ] and [0, lenK]. They stand for the padding masks of a batch of sentences: rows of q, k and v
  * past a length may hold anything, infinities and NaN too. Rows of out past queryLens[b] and rows
  * without any key are written as zeros. lse: NULL or [batch, headsQ, lenQ] packed fp32; minus infinity
- * in the rows that are zeros. It is what the gradient call needs.
+ * in the rows that are zeros. It is what the gradient call needs. What is not finite in a row or key that the
+ * lengths leave in reaches the result as the formula has it: NaN, and not zeros.
  *
  * Calls with at most 32 query rows for a key head ((headsQ / headsKV) * lenQ: a decoding step, the
  * hypotheses of a beam as lenQ rows of one sentence) read k and v once for all of them; fewer rows

@@ -407,8 +407,10 @@ XattnKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
         TcFenceAfter();
         const bool sums = mine && n > 0 && ok;
         const int row = myQ0 + r;
+        /* The lengths alone say which rows are empty. In a live row a sum that is NaN or 0 (scores of NaN; all scores minus
+           infinity) makes the result NaN, as the formula has it. */
         const bool rowLive = mine && row < nq && n > 0;
-        const float inv = rowLive && l > 0.f ? 1.f / l : 0.f;
+        const float inv = 1.f / l;
         if (p.splits > 1 && hf == 0) {
             sM[s * XT + r] = sums ? m : -INFINITY;
             sL[s * XT + r] = sums ? l : 0.f;
@@ -478,11 +480,14 @@ XattnKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
                 float top = -INFINITY;
                 for (int t = 0; t < p.splits; t++)
                     top = fmaxf(top, LoadRemote(MapShared(SmemAddr(&sM[s * XT + r]), t)));
-                const bool rowLive = row < nq && top != -INFINITY;
+                const bool rowLive = row < nq && nk > 0;
+                /* A part whose scores are all NaN has a reference of minus infinity and a sum of NaN: weighed by 0 it still
+                   makes the total NaN. A part without keys has zeros. */
+                const float ref = top == -INFINITY ? 0.f : top;
                 float total = 0.f, acc[8] = { 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f };
                 if (rowLive) {
                     for (int t = 0; t < p.splits; t++) {
-                        const float f = Exp2(LoadRemote(MapShared(SmemAddr(&sM[s * XT + r]), t)) - top);
+                        const float f = Exp2(LoadRemote(MapShared(SmemAddr(&sM[s * XT + r]), t)) - ref);
                         total += f * LoadRemote(MapShared(SmemAddr(&sL[s * XT + r]), t));
                         const uint32_t base = MapShared(ringS + (s * XT + r) * D * 4, t);
 #pragma unroll
@@ -493,7 +498,7 @@ XattnKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
                         }
                     }
                 }
-                const float inv = rowLive && total > 0.f ? 1.f / total : 0.f;
+                const float inv = 1.f / total;
                 if (c * 8 < p.sh.dim) {
                     uint4 w = make_uint4(0u, 0u, 0u, 0u);
                     if (rowLive)

@@ -279,25 +279,24 @@ XattnStepKernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
     const int rows = p.rows;
     for (int i = threadIdx.x; i < rows * (D / 4); i += ST_THREADS) {
         const int r = i / (D / 4), c = (i - r * (D / 4)) * 4;
-        const float top = fmaxf(fmaxf(sM[0][r], sM[1][r]), fmaxf(sM[2][r], sM[3][r]));
+        const float top = fmaxf(fmaxf(sM[0][r], sM[1][r]), fmaxf(sM[2][r], sM[3][r])), ref = top == -INFINITY ? 0.f : top;
         float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (top != -INFINITY)
 #pragma unroll
-            for (int w = 0; w < 4; w++) {
-                const float f = Exp2(sM[w][r] - top);
-                const float4 v = *(const float4 *)(part + (w * MT * 16 + r) * D + c);
-                a.x += f * v.x; a.y += f * v.y; a.z += f * v.z; a.w += f * v.w;
-            }
+        for (int w = 0; w < 4; w++) {
+            /* a warp whose scores are all NaN has a reference of minus infinity and sums of NaN: 0 times those is NaN still */
+            const float f = Exp2(sM[w][r] - ref);
+            const float4 v = *(const float4 *)(part + (w * MT * 16 + r) * D + c);
+            a.x += f * v.x; a.y += f * v.y; a.z += f * v.z; a.w += f * v.w;
+        }
         *(float4 *)(part + r * D + c) = a;
     }
     __syncthreads();
     if (threadIdx.x < rows) {
         const int r = threadIdx.x;
-        const float top = fmaxf(fmaxf(sM[0][r], sM[1][r]), fmaxf(sM[2][r], sM[3][r]));
+        const float top = fmaxf(fmaxf(sM[0][r], sM[1][r]), fmaxf(sM[2][r], sM[3][r])), ref = top == -INFINITY ? 0.f : top;
         float t = 0.f;
-        if (top != -INFINITY)
-            for (int w = 0; w < 4; w++)
-                t += Exp2(sM[w][r] - top) * sL[w][r];
+        for (int w = 0; w < 4; w++)
+            t += Exp2(sM[w][r] - ref) * sL[w][r];
         sM[0][r] = top;
         sL[0][r] = t;
     }
@@ -324,21 +323,23 @@ XattnStepKernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
         else {
             for (int t = 0; t < p.splits; t++)
                 top = fmaxf(top, LoadRemote(MapShared(SmemAddr(&sM[0][r]), t)));
-            if (top != -INFINITY)
-                for (int t = 0; t < p.splits; t++) {
-                    const float f = Exp2(LoadRemote(MapShared(SmemAddr(&sM[0][r]), t)) - top);
-                    total += f * LoadRemote(MapShared(SmemAddr(&sL[0][r]), t));
-                    const uint32_t src = MapShared(ring + (r * D + c) * 4, t);
+            const float ref = top == -INFINITY ? 0.f : top;
+            for (int t = 0; t < p.splits; t++) {
+                const float f = Exp2(LoadRemote(MapShared(SmemAddr(&sM[0][r]), t)) - ref);
+                total += f * LoadRemote(MapShared(SmemAddr(&sL[0][r]), t));
+                const uint32_t src = MapShared(ring + (r * D + c) * 4, t);
 #pragma unroll
-                    for (int hf = 0; hf < 2; hf++) {
-                        const float4 v = LoadRemote4(src + hf * 16);
-                        acc[hf * 4 + 0] += f * v.x; acc[hf * 4 + 1] += f * v.y;
-                        acc[hf * 4 + 2] += f * v.z; acc[hf * 4 + 3] += f * v.w;
-                    }
+                for (int hf = 0; hf < 2; hf++) {
+                    const float4 v = LoadRemote4(src + hf * 16);
+                    acc[hf * 4 + 0] += f * v.x; acc[hf * 4 + 1] += f * v.y;
+                    acc[hf * 4 + 2] += f * v.z; acc[hf * 4 + 3] += f * v.w;
                 }
+            }
         }
-        const bool rowLive = iq < nq && top != -INFINITY;
-        const float inv = rowLive && total > 0.f ? 1.f / total : 0.f;
+        /* the lengths alone say which rows are empty: a sum of NaN, or of 0 where all scores are minus infinity, makes a live
+           row NaN, as the formula has it */
+        const bool rowLive = iq < nq && nk > 0;
+        const float inv = 1.f / total;
         if (c < p.sh.dim) {
             uint4 w = make_uint4(0u, 0u, 0u, 0u);
             if (rowLive)
