@@ -4,7 +4,7 @@
  *     out[b, h, i] = sum_j p_ij v[b, h', j],  p_ij = exp(s_ij - lse_i),  s_ij = scale * q_i . k_j,
  *     lse_i = log sum_j exp(s_ij),  j < keyLens[b],  i < queryLens[b],  h' = h / (headsQ / headsKV)
  *
- * in one pass over the keys: with a running reference m of the row's maximum, every key tile adds
+ * in one pass over the keys: with a running reference m somewhat below the row's maximum, every key tile adds
  * exp(s - m) to the row's sum and exp(s - m) v to its accumulator, and both are rescaled when the
  * maximum has grown. It serves the sublayer of the transformer sample's decoder that looks at the
  * encoder's output (source/sample/transformer/submodel/Attention.cpp:188-243 with another length
@@ -23,8 +23,8 @@
  *
  * XattnStepKernel (ntb_xattn_step.cu) takes the calls with at most 32 query rows a key head.
  *
- * Weights are rounded to half after the maximum is taken off, so a rounding is 2^-11 of a weight at most
- * 2^8 (the reference m may lag the true maximum by 8 in the exponent); sums, maxima and accumulators
+ * Weights are rounded to half for the second product, after a reference is taken off that gives them the upper part of
+ * half's range (ntb_xattn.cuh says which); sums, maxima and accumulators
  * are fp32. Waits are bounded as in the matrix-product kernels.
  */
 #include "ntb_xattn.cuh"
@@ -348,11 +348,10 @@ XattnKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
                 for (int e = 0; e < 64; e += 2)
                     m4[(e >> 1) & 3] = fmaxf(fmaxf(m4[(e >> 1) & 3], __uint_as_float(x[e])), __uint_as_float(x[e + 1]));
                 const float top = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * p.scaleLog2;
-                /* Both threads of a row use one reference. It follows the maximum once that is 8 ahead in some row of
-                   the stream (weights up to 2^8 are as exact in half as weights up to 1), which the first tile
-                   settles and later ones rarely need. */
-                if (StreamAny(1 + s, j == 0 || top > m + 8.f)) {
-                    const float mNew = fmaxf(m, Joint(s, hf, &sHalf[s][r], top, [](float a, float b) { return fmaxf(a, b); }));
+                /* Both threads of a row use one reference. It follows the maximum once that is far ahead in some row of
+                   the stream, which the first tile settles and later ones rarely need. */
+                if (StreamAny(1 + s, j == 0 || top > m + XATTN_AHEAD)) {
+                    const float mNew = fmaxf(m, Joint(s, hf, &sHalf[s][r], top, [](float a, float b) { return fmaxf(a, b); }) - XATTN_BELOW);
                     const float f = mNew > m ? Exp2(m - mNew) : 1.f;
                     m = mNew;
                     l *= f;

@@ -60,6 +60,13 @@ constexpr int XT = 128;                               /* rows of a query tile an
 constexpr int XBOX_BYTES = XT * ROW_BYTES;            /* 128 rows x 64 halves: one swizzled box of an operand tile */
 constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
 
+/* The reference that the forward kernels take off the exponents (of 2): XATTN_BELOW under the row's maximum when it
+   is set, and set again once the maximum is more than XATTN_AHEAD over it. Weights, which are halves in the second product,
+   so reach 2^15, below half's 65504; those of 2^-14 and more, 2^-21 of the largest at least, are normal and off by
+   2^-11 of themselves, lighter ones by 2^-25, 2^-32 of the largest. With the maximum itself as the reference the tail of
+   131072 keys, each 2^-25 of the first, would be lost: 0.4 % of the sum. */
+constexpr float XATTN_BELOW = 7.f, XATTN_AHEAD = 15.f;
+
 /* how an operand's tensor map is addressed: a broadcast extent (stride 0) is mapped with one
    element and its coordinate multiplied by 0 */
 struct HeadsAddr {

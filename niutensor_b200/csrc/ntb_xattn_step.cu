@@ -198,12 +198,12 @@ XattnStepKernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
                         t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 2));
                         top[hf] = t * p.scaleLog2;
                     }
-                    /* the reference follows the maximum once it is 8 (in the exponent) behind */
-                    if (__any_sync(0xffffffffu, top[0] > m[mt][0] + 8.f || top[1] > m[mt][1] + 8.f)) {
+                    /* the reference follows the maximum once it is far behind */
+                    if (__any_sync(0xffffffffu, top[0] > m[mt][0] + XATTN_AHEAD || top[1] > m[mt][1] + XATTN_AHEAD)) {
                         float f[2];
 #pragma unroll
                         for (int hf = 0; hf < 2; hf++) {
-                            const float mNew = fmaxf(m[mt][hf], top[hf]);
+                            const float mNew = fmaxf(m[mt][hf], top[hf] - XATTN_BELOW);
                             f[hf] = mNew > m[mt][hf] ? Exp2(m[mt][hf] - mNew) : 1.f;
                             m[mt][hf] = mNew;
                             l[mt][hf] *= f[hf];
