@@ -348,12 +348,16 @@ XattnKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
                 for (int e = 0; e < 64; e += 2)
                     m4[(e >> 1) & 3] = fmaxf(fmaxf(m4[(e >> 1) & 3], __uint_as_float(x[e])), __uint_as_float(x[e + 1]));
                 const float top = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * p.scaleLog2;
-                /* Both threads of a row use one reference. It follows the maximum once that is far ahead in some row of
-                   the stream, which the first tile settles and later ones rarely need. */
-                if (StreamAny(1 + s, j == 0 || top > m + XATTN_AHEAD)) {
-                    const float mNew = fmaxf(m, Joint(s, hf, &sHalf[s][r], top, [](float a, float b) { return fmaxf(a, b); }) - XATTN_BELOW);
-                    const float f = mNew > m ? Exp2(m - mNew) : 1.f;
-                    m = mNew;
+                /* Both threads of a row use one reference. It follows the maximum once that is far ahead, which the first
+                   tile settles and later ones rarely need. Rows behind the end have no say, and a row's reference moves by
+                   its own scores alone, whoever called for the step: its result depends on no other row. */
+                if (StreamAny(1 + s, j == 0 || (myQ0 + r < nq && top > m + XATTN_AHEAD))) {
+                    const float both = Joint(s, hf, &sHalf[s][r], top, [](float a, float b) { return fmaxf(a, b); });
+                    float f = 1.f;
+                    if (both > m + XATTN_AHEAD) {
+                        f = Exp2(m - (both - XATTN_BELOW));
+                        m = both - XATTN_BELOW;
+                    }
                     l *= f;
                     if (j > 0) {
                         /* the scores' commit covers the second product before it: the accumulator is current */

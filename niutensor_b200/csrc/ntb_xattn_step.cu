@@ -122,8 +122,8 @@ XattnStepKernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
 #pragma unroll
             for (int hf = 0; hf < 2; hf++) {
                 const int r = mt * 16 + hf * 8 + (lane >> 2);
-                const bool rowOk = r < p.rows;
-                const int g = rowOk ? r / p.sh.lenQ : 0, i = rowOk ? r - g * p.sh.lenQ : 0;
+                const int g = r < p.rows ? r / p.sh.lenQ : 0, i = r < p.rows ? r - g * p.sh.lenQ : 0;
+                const bool rowOk = r < p.rows && i < nq;               /* rows behind the end are not looked at */
                 const __half * src = p.q + b * p.lQ.batch + (kvHead * p.sh.group + g) * p.lQ.head + i * p.lQ.row;
 #pragma unroll
                 for (int ks = 0; ks < D / 16; ks++)
@@ -198,14 +198,16 @@ XattnStepKernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
                         t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 2));
                         top[hf] = t * p.scaleLog2;
                     }
-                    /* the reference follows the maximum once it is far behind */
+                    /* the reference follows the maximum once it is far behind, in each row by its own scores alone */
                     if (__any_sync(0xffffffffu, top[0] > m[mt][0] + XATTN_AHEAD || top[1] > m[mt][1] + XATTN_AHEAD)) {
                         float f[2];
 #pragma unroll
                         for (int hf = 0; hf < 2; hf++) {
-                            const float mNew = fmaxf(m[mt][hf], top[hf] - XATTN_BELOW);
-                            f[hf] = mNew > m[mt][hf] ? Exp2(m[mt][hf] - mNew) : 1.f;
-                            m[mt][hf] = mNew;
+                            f[hf] = 1.f;
+                            if (top[hf] > m[mt][hf] + XATTN_AHEAD) {
+                                f[hf] = Exp2(m[mt][hf] - (top[hf] - XATTN_BELOW));
+                                m[mt][hf] = top[hf] - XATTN_BELOW;
+                            }
                             l[mt][hf] *= f[hf];
                         }
 #pragma unroll
