@@ -207,6 +207,40 @@ __device__ __forceinline__ uint64_t Add2(uint64_t a, uint64_t b)
     return r;
 }
 
+__device__ __forceinline__ uint64_t Mul2(uint64_t a, uint64_t b)
+{
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+
+/*
+ * The gradient kernels' ds = p (dp - delta) go into their products as halves. They are smaller than what they are
+ * summed to by p, about 1 / lenK, and left as they are would be subnormal or 0 where dq and dk are ordinary halves, or,
+ * with large v and a small scale, infinite. So every row of a product's ds carries a power of two, taken out of its sums in
+ * fp32, that brings its largest to [2^DS_TOP, 2^(DS_TOP + 1)) when it is set, and is set again when ds have grown past
+ * DS_MOST. ds down to 2^-21 of the largest are then off by 2^-11 of themselves, smaller ones by 2^-32 of the largest.
+ */
+constexpr float DS_MOST = 32768.f, DS_UNSET = 1208925819614629174706176.f;      /* 2^15; 2^80: nothing but zeros so far */
+constexpr int DS_TOP = 7;
+
+/* the power of two that brings `top` to [2^e, 2^(e + 1)), at most 2^80: ds, which are less than 2^41, times it are
+   finite as floats */
+__device__ __forceinline__ float PowerFor(float top, int e)
+{
+    const int b = 254 + e - (int)(__float_as_uint(top) >> 23);
+    return __uint_as_float((uint32_t)(b < 207 ? b : 207) << 23);
+}
+/* 1 / power, for powers of two that are normal both ways */
+__device__ __forceinline__ float PowerInverse(float power) { return __uint_as_float(0x7f000000u - __float_as_uint(power)); }
+/* What a row's sums of ds, which carry a factor, are multiplied by at last: its inverse and the scale. Where that is past a
+   float the sums are 0 or their results past a half: 0 stays 0, the others become infinite. Where it is below a float's
+   range the results, from sums below 2^62, are below a half's. */
+__device__ __forceinline__ float SumsFactor(float power, float scale) { return fminf(power * scale, 3.402823466e38f); }
+/* whether the factor has to be set again for a row with this largest |ds| (an infinity makes the row's sums infinite
+   or NaN, whatever the factor) */
+__device__ __forceinline__ bool DsPast(float top, float factor) { return top * factor > DS_MOST && top < INFINITY; }
+
 __device__ __forceinline__ uint32_t PackHalf2(float lo, float hi)
 {
     const __half2 h = __floats2half2_rn(lo, hi);

@@ -31,8 +31,9 @@
  * instructions came from L2 for every tile, 0.5 to 1 us of the 8 a short item takes (sentences 69.4 -> 65.2 us).
  *
  * Rounding: p is at most 1 and may be tiny (1 / lenK); for dv it is rounded to half as 2^12 p, exact powers
- * of two away from half's subnormals. ds is rounded to half as it is: its scale is that of the gradients,
- * which are halves themselves. Sums are fp32.
+ * of two away from half's subnormals. ds is rounded to half times a power of two of its row (of the query's for dq, of
+ * the key's for dk; ntb_xattn.cuh says why), which follows the row's largest ds as the walk goes on: a vote of
+ * the softmax threads in every step, and where one of them calls for it, the accumulators scaled. Sums are fp32.
  */
 #include "ntb_xattn.cuh"
 
@@ -53,7 +54,7 @@ struct XattnGradParams {
     XattnShape sh;
     HeadsAddr aQ, aK, aV, aO, aDO;
     const float * lse;
-    float * work;              /* [batch, headsQ, tilesPerHead][2][128]: lse in the second kernel's units, delta */
+    float * work;              /* [batch, headsQ, tilesPerHead][2][128]: lse and minus delta in the second kernel's units */
     int tilesPerHead, keyTiles;
     int splits, item0;         /* of this launch */
     float scale, scaleLog2;
@@ -70,23 +71,99 @@ template <int D> struct XattnGradSmem {
     /* first kernel: a ring of k and v tiles (q and do are in tensor memory) */
     static constexpr int SLOTS = 7;
     static constexpr int Q_TOTAL = SLOTS * TILE + 1024;
-    /* second kernel: k, v, rings of q, of do, and of the query rows' (lse, delta); barriers */
+    /* second kernel: k, v, rings of q, of do, and of the query rows' (lse, delta); barriers; a word a row */
     static constexpr int QSLOTS = 3, DOSLOTS = 2, STATSLOTS = 2, STAT = 2 * XT * 4;
     static constexpr int KV_RING = 2 * TILE, KV_STATS = KV_RING + (QSLOTS + DOSLOTS) * TILE, KV_BARS = KV_STATS + STATSLOTS * STAT;
-    static constexpr int KV_TOTAL = KV_BARS + 256;
+    static constexpr int KV_WORDS = KV_BARS + 256, KV_TOTAL = KV_WORDS + XT * 4;
     static_assert(SLOTS * TILE >= XT * D * 4 && (QSLOTS + DOSLOTS) * TILE >= 2 * XT * D * 4, "the split's partial sums take the place of the rings");
     static_assert(KV_TOTAL <= 232448, "shared memory of a CTA");
 };
 
 __device__ __forceinline__ void GradBarrier() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
+__device__ __forceinline__ bool GradAny(bool say)
+{
+    uint32_t any;
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 q, %1, 0;\n\tbarrier.cta.red.or.aligned.pred p, 1, 256, q;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                 : "=r"(any) : "r"((uint32_t)say) : "memory");
+    return any != 0;
+}
 
-/* one thread's 32 accumulator columns into its row of a split's partial sums, 16-byte chunks permuted by the row */
-__device__ __forceinline__ void StorePartial(uint32_t rowBase, int r, int chunk0, const uint32_t * o, bool have)
+/* 32 columns of a thread's ds as halves */
+__device__ __forceinline__ void PackDs(uint32_t dsT, const uint32_t * ds)
+{
+    uint32_t w[16];
+#pragma unroll
+    for (int e = 0; e < 16; e++)
+        w[e] = PackHalf2(__uint_as_float(ds[2 * e]), __uint_as_float(ds[2 * e + 1]));
+    TmemStore16Async(dsT, w);
+}
+__device__ __forceinline__ float LargestDs(const uint32_t * ds)
+{
+    float m[4] = { 0.f, 0.f, 0.f, 0.f };
+#pragma unroll
+    for (int e = 0; e < 32; e += 2)
+        m[(e >> 1) & 3] = fmaxf(fmaxf(m[(e >> 1) & 3], fabsf(__uint_as_float(ds[e]))), fabsf(__uint_as_float(ds[e + 1])));
+    return fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
+}
+
+/*
+ * The end of a step's ds: one thread has 64 columns of its row, times the row's factor (in the first step 1), in
+ * registers, of which the largest is `top`. Behind the first step they are in tensor memory already, and all threads vote
+ * on whether some live row's are too large. If so, and in the first step, the two threads of a row settle on a factor,
+ * scale the row's sums of the steps before, half of the columns each, and store their ds again. All 256 threads call;
+ * word: one a row, in shared memory.
+ */
+template <int D>
+__device__ __forceinline__ void SettleDs(uint32_t * ds, float top, float & factor, bool rowLive, bool first, int hf, volatile float * word,
+                                         uint32_t dsT, uint32_t accT)
+{
+    if (first || GradAny(rowLive && DsPast(top, 1.f))) {
+        if (hf == 1)
+            *word = top;
+        GradBarrier();
+        if (hf == 0) {
+            top = fmaxf(top, *word);
+            *word = top;
+        }
+        GradBarrier();
+        top = *word;
+        const float f = first ? (top < INFINITY ? PowerFor(top, DS_TOP) : 1.f) : DsPast(top, 1.f) ? PowerFor(top, DS_TOP) : 1.f;
+        factor *= f;
+        if (!first) {
+            TmemWaitStore();
+#pragma unroll 1
+            for (int c = hf * (D / 2); c < (hf + 1) * (D / 2); c += 8) {
+                uint32_t o[8];
+                TmemLoad8Async(accT + c, o);
+                TmemWaitLoad();
+#pragma unroll
+                for (int e = 0; e < 8; e++)
+                    o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+                TmemStore4Async(accT + c, o);
+                TmemStore4Async(accT + c + 4, o + 4);
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < 64; e++)
+            ds[e] = __float_as_uint(__uint_as_float(ds[e]) * f);
+        PackDs(dsT, ds);
+        PackDs(dsT + 16, ds + 32);
+    }
+    TmemWaitStore();
+}
+
+/* one thread's 32 accumulator columns times a power of two into its row of a split's partial sums, 16-byte chunks permuted
+   by the row */
+__device__ __forceinline__ void StorePartial(uint32_t rowBase, int r, int chunk0, const uint32_t * o, float power, bool have)
 {
 #pragma unroll
-    for (int jj = 0; jj < 8; jj++)
-        StoreShared16(rowBase + (((chunk0 + jj) ^ (r & 7)) << 4), have ? o[jj * 4] : 0u, have ? o[jj * 4 + 1] : 0u,
-                      have ? o[jj * 4 + 2] : 0u, have ? o[jj * 4 + 3] : 0u);
+    for (int jj = 0; jj < 8; jj++) {
+        uint32_t w[4];
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+            w[e] = have ? __float_as_uint(__uint_as_float(o[jj * 4 + e]) * power) : 0u;
+        StoreShared16(rowBase + (((chunk0 + jj) ^ (r & 7)) << 4), w[0], w[1], w[2], w[3]);
+    }
 }
 
 /* eight columns of a row summed over the cluster in rank order */
@@ -379,18 +456,18 @@ XattnGradQKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
             if (hf == 0 && rank == 0) {
                 float * w = p.work + (long long)item * (2 * XT);
                 w[r] = lse2 - P_SCALE_LOG2;
-                w[XT + r] = delta * P_SCALE_INV;
+                w[XT + r] = -delta * P_SCALE_INV;
             }
         };
         if (!single)
             leaveRow();
         const uint32_t sT = tmemBase + laneBase + TMEM_S + hf * 64, dpT = tmemBase + laneBase + TMEM_DP + hf * 64;
-        /* with a single tile no warp leaves out the barriers of the joint sum, whatever became of its waits */
-        for (int j = 0; (ok || single) && j < n; j++) {
+        const uint32_t dqT = tmemBase + laneBase + TMEM_DQ;
+        float factor = 1.f;                                  /* of this row's ds */
+        /* no warp leaves out a step's barriers, whatever became of its waits (after one that ran out the next return at once) */
+        for (int j = 0; j < n; j++) {
             const uint32_t ph = (uint32_t)j & 1u;
             ok = WaitNowWarp(SmemAddr(&barS), ph, abortPtr, p.status) && ok;
-            if (!ok && !single)
-                break;
             TcFenceAfter();
             uint32_t x[64];
             TmemLoad64U(sT, x);
@@ -401,8 +478,6 @@ XattnGradQKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                 x[e] = __float_as_uint(Exp2(fmaf(__uint_as_float(x[e]), p.scaleLog2, -lse2)));
             const int valid = nk - (tile0 + j) * XT - hf * 64;
             ok = WaitNowWarp(SmemAddr(&barDP), ph, abortPtr, p.status) && ok;
-            if (!ok && !single)
-                break;
             /* v of this tile and k of the one before have been read */
             if (threadIdx.x == 0)
                 MbarArrive(SmemAddr(&barEvent[j % GR_EVENTS]));
@@ -427,22 +502,27 @@ XattnGradQKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                 delta = rowLive ? sDelta[r] : 0.f;
                 leaveRow();
             }
+            const uint64_t factor2 = Pair(factor, factor), delta2 = Pair(-delta * factor, -delta * factor);
+            float top = 0.f;
 #pragma unroll
             for (int c = 0; c < 2; c++) {
-                uint32_t y[32], w[16];
+                uint32_t y[32];
                 TmemLoad32Async(dpT + c * 32, y);
                 TmemWaitLoad();
 #pragma unroll
-                for (int e = 0; e < 32; e++) {
-                    const float ds = __uint_as_float(x[c * 32 + e]) * (__uint_as_float(y[e]) - delta);
-                    y[e] = valid >= 64 || c * 32 + e < valid ? __float_as_uint(ds) : 0u;
+                for (int e = 0; e < 32; e += 2) {
+                    const uint64_t d = Fma2(Pair(__uint_as_float(y[e]), __uint_as_float(y[e + 1])), factor2, delta2);
+                    float a, b;
+                    Unpair(Mul2(Pair(__uint_as_float(x[c * 32 + e]), __uint_as_float(x[c * 32 + e + 1])), d), a, b);
+                    x[c * 32 + e] = valid >= 64 || c * 32 + e < valid ? __float_as_uint(a) : 0u;
+                    x[c * 32 + e + 1] = valid >= 64 || c * 32 + e + 1 < valid ? __float_as_uint(b) : 0u;
                 }
-#pragma unroll
-                for (int e = 0; e < 16; e++)
-                    w[e] = PackHalf2(__uint_as_float(y[2 * e]), __uint_as_float(y[2 * e + 1]));
-                TmemStore16Async(dpT + c * 16, w);
+                top = fmaxf(top, LargestDs(x + c * 32));
+                if (j > 0)
+                    PackDs(dpT + c * 16, x + c * 32);
             }
-            TmemWaitStore();
+            /* the step before's product is done: its sums may be scaled */
+            SettleDs<D>(x, top, factor, rowLive, j == 0, hf, &sDelta[r], dpT, dqT);
             TcFenceBefore();
             ArriveWarp(SmemAddr(&barDS), lane);
         }
@@ -450,7 +530,7 @@ XattnGradQKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
             ok = WaitNowWarp(SmemAddr(&barDone), 0, abortPtr, p.status);
         TcFenceAfter();
         const bool sums = n > 0 && ok;
-        const uint32_t dqT = tmemBase + laneBase + TMEM_DQ;
+        const float power = PowerInverse(factor), out = SumsFactor(power, p.scale);
 #pragma unroll 1
         for (int c = hf * (D / 64); c < (hf + 1) * (D / 64); c++) {       /* 32 columns a step; this half's D / 2 */
             uint32_t o[32];
@@ -459,9 +539,9 @@ XattnGradQKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                 TmemWaitLoad();
             }
             if (p.splits == 1)
-                StageHalf32(outS + (c >> 1) * XBOX_BYTES + r * ROW_BYTES, lane, (c & 1) * 4, o, p.scale, sums && rowLive);
+                StageHalf32(outS + (c >> 1) * XBOX_BYTES + r * ROW_BYTES, lane, (c & 1) * 4, o, out, sums && rowLive);
             else
-                StorePartial(ringS + r * D * 4, r, c * 8, o, sums);
+                StorePartial(ringS + r * D * 4, r, c * 8, o, power, sums);
         }
         if (p.splits == 1) {
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -526,6 +606,7 @@ XattnGradKVKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     };
     static_assert(sizeof(Bars) <= 256, "place of the barriers");
     Bars & bars = *(Bars *)(kvSmem + SM::KV_BARS);
+    float * sWord = (float *)(kvSmem + SM::KV_WORDS);        /* what the two threads of a row tell each other */
 
     const int warp = threadIdx.x >> 5;
     const int lane = threadIdx.x & 31;
@@ -760,15 +841,16 @@ XattnGradKVKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         const uint32_t laneBase = (uint32_t)(sub * 32) << 16;
         const int r = sub * 32 + lane;
         const uint32_t sT = tmemBase + laneBase + TMEM_S + hf * 64, dpT = tmemBase + laneBase + TMEM_DP + hf * 64;
+        const bool rowLive = k0 + r < nk;
+        float factor = 1.f;                                  /* of this key's ds */
         bool ok = true;
+        /* as in the first kernel, no warp leaves out a step's barriers */
         for (int i = 0; i < n; i++) {
             const uint32_t ph = (uint32_t)i & 1u;
             const float4 * lse4 = (const float4 *)(kvSmem + SM::KV_STATS + (i % STATSLOTS) * SM::STAT) + hf * 16, * delta4 = lse4 + XT / 4;
             /* every lane observes the copy's completion itself before it reads what was copied */
             ok = WaitNowWarp(SmemAddr(&bars.statFull[i % STATSLOTS]), (uint32_t)(i / STATSLOTS) & 1u, abortPtr, p.status) &&
-                 WaitNowWarp(SmemAddr(&bars.s), ph, abortPtr, p.status);
-            if (!ok)
-                break;
+                 WaitNowWarp(SmemAddr(&bars.s), ph, abortPtr, p.status) && ok;
             /* these scores were issued behind the last product that reads the step before's do */
             if (threadIdx.x == 0 && i >= 1)
                 MbarArrive(SmemAddr(&bars.doEmpty[(i - 1) % DOSLOTS]));
@@ -794,45 +876,51 @@ XattnGradKVKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
             TmemWaitStore();
             TcFenceBefore();
             ArriveWarp(SmemAddr(&bars.p), lane);
-            ok = WaitNowWarp(SmemAddr(&bars.dp), ph, abortPtr, p.status);
-            if (!ok)
-                break;
+            ok = WaitNowWarp(SmemAddr(&bars.dp), ph, abortPtr, p.status) && ok;
             /* and this product behind the one that reads its q, which all softmax threads let go ahead */
             if (threadIdx.x == 0 && i >= 1) {
                 MbarArrive(SmemAddr(&bars.qEmpty[(i - 1) % QSLOTS]));
                 MbarArrive(SmemAddr(&bars.statEmpty[(i - 1) % STATSLOTS]));
             }
             TcFenceAfter();
+            const uint64_t inv2 = Pair(P_SCALE_INV, P_SCALE_INV), factor2 = Pair(factor, factor);
+            float top = 0.f;
 #pragma unroll
             for (int c = 0; c < 2; c++) {
-                uint32_t y[32], w[16];
+                uint32_t y[32];
                 TmemLoad32Async(dpT + c * 32, y);
                 TmemWaitLoad();
 #pragma unroll
                 for (int e4 = 0; e4 < 8; e4++) {
-                    const float4 de = delta4[c * 8 + e4];
+                    const float4 de = delta4[c * 8 + e4];        /* -2^-12 delta */
                     const int e = e4 * 4, xe = c * 32 + e;
-                    const float d0 = __uint_as_float(x[xe]) * fmaf(__uint_as_float(y[e]), P_SCALE_INV, -de.x);
-                    const float d1 = __uint_as_float(x[xe + 1]) * fmaf(__uint_as_float(y[e + 1]), P_SCALE_INV, -de.y);
-                    const float d2 = __uint_as_float(x[xe + 2]) * fmaf(__uint_as_float(y[e + 2]), P_SCALE_INV, -de.z);
-                    const float d3 = __uint_as_float(x[xe + 3]) * fmaf(__uint_as_float(y[e + 3]), P_SCALE_INV, -de.w);
-                    w[e4 * 2] = PackHalf2(d0, d1);
-                    w[e4 * 2 + 1] = PackHalf2(d2, d3);
+                    const uint64_t d0 = Fma2(Pair(__uint_as_float(y[e]), __uint_as_float(y[e + 1])), inv2, Pair(de.x, de.y));
+                    const uint64_t d1 = Fma2(Pair(__uint_as_float(y[e + 2]), __uint_as_float(y[e + 3])), inv2, Pair(de.z, de.w));
+                    float a, b;
+                    Unpair(Mul2(Mul2(Pair(__uint_as_float(x[xe]), __uint_as_float(x[xe + 1])), factor2), d0), a, b);
+                    x[xe] = __float_as_uint(a);
+                    x[xe + 1] = __float_as_uint(b);
+                    Unpair(Mul2(Mul2(Pair(__uint_as_float(x[xe + 2]), __uint_as_float(x[xe + 3])), factor2), d1), a, b);
+                    x[xe + 2] = __float_as_uint(a);
+                    x[xe + 3] = __float_as_uint(b);
                 }
-                TmemStore16Async(dpT + c * 16, w);
+                top = fmaxf(top, LargestDs(x + c * 32));
+                if (i > 0)
+                    PackDs(dpT + c * 16, x + c * 32);
             }
-            TmemWaitStore();
+            /* the step before's product for dk is done: its sums may be scaled */
+            SettleDs<D>(x, top, factor, rowLive, i == 0, hf, &sWord[r], dpT, tmemBase + laneBase + TMEM_DK);
             TcFenceBefore();
             ArriveWarp(SmemAddr(&bars.ds), lane);
         }
         if (n > 0 && ok)
             ok = WaitNowWarp(SmemAddr(&bars.done), 0, abortPtr, p.status);
         TcFenceAfter();
-        const bool sums = n > 0 && ok, rowLive = k0 + r < nk;
+        const bool sums = n > 0 && ok;
         /* warps 0-3: dv, in the place of v; warps 4-7: dk, in the place of k */
         const uint32_t accT = tmemBase + laneBase + (hf == 0 ? TMEM_DV : TMEM_DK);
         const uint32_t box = (hf == 0 ? vS : kS) + sub * 32 * ROW_BYTES;
-        const float factor = hf == 0 ? P_SCALE_INV : p.scale;
+        const float power = hf == 0 ? P_SCALE_INV : PowerInverse(factor), out = SumsFactor(power, hf == 0 ? 1.f : p.scale);
         if (p.splits == 1) {
 #pragma unroll 1
             for (int c = 0; c < D / 32; c++) {
@@ -841,7 +929,7 @@ XattnGradKVKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
                     TmemLoad32Async(accT + c * 32, o);
                     TmemWaitLoad();
                 }
-                StageHalf32(box + (c >> 1) * XBOX_BYTES + lane * ROW_BYTES, lane, (c & 1) * 4, o, factor, sums && rowLive);
+                StageHalf32(box + (c >> 1) * XBOX_BYTES + lane * ROW_BYTES, lane, (c & 1) * 4, o, out, sums && rowLive);
             }
         }
         else {
@@ -852,7 +940,7 @@ XattnGradKVKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
                     TmemLoad32Async(accT + c * 32, o);
                     TmemWaitLoad();
                 }
-                StorePartial(ringS + (hf * XT + r) * D * 4, r, c * 8, o, sums);
+                StorePartial(ringS + (hf * XT + r) * D * 4, r, c * 8, o, power, sums);
             }
         }
         if (p.splits == 1 && ok) {
@@ -885,7 +973,7 @@ XattnGradKVKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
                     continue;
                 uint4 w = make_uint4(0u, 0u, 0u, 0u);
                 if (row < nk && steps > 0)
-                    w = SumPartials(ringS + (which * XT + r) * D * 4, r, c, p.splits, which == 0 ? P_SCALE_INV : p.scale);
+                    w = SumPartials(ringS + (which * XT + r) * D * 4, r, c, p.splits, which == 0 ? 1.f : p.scale);
                 if (which == 0)
                     *(uint4 *)(p.d1 + b * p.l1.batch + kvHead * p.l1.head + row * p.l1.row + c * 8) = w;
                 else

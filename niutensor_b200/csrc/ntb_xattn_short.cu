@@ -7,8 +7,8 @@
  * dq = ds k. Everything is read once and written once, summed in a fixed order, without atomics or a workspace.
  *
  * The next chunk's rows of q and do travel to registers under the products of this one. delta comes from the weights,
- * as all keys are here (ntb_xattn_grad.cu says what that is good for). Rounding as there: ds and 2^12 p to half, sums
- * in fp32. Bound by the latency of a chunk's four steps, which other CTAs of the SM fill: hence few keys and registers
+ * as all keys are here (ntb_xattn_grad.cu says what that is good for). Rounding as there: ds, times powers of two (of the
+ * query's row for dq, of the warp for dk), and 2^12 p to half, sums in fp32. Bound by the latency of a chunk's four steps, which other CTAs of the SM fill: hence few keys and registers
  * a CTA. 64 x 8 heads, 48 rows, 48 keys of 64: 16.7 us, 22 MB at 1.3 TB/s.
  */
 #include "ntb_xattn.cuh"
@@ -56,7 +56,8 @@ XattnGradShortKernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
     extern __shared__ uint8_t smemRaw[];
     __shared__ __align__(8) uint64_t barFull;
     __shared__ int abortFlag;
-    __shared__ float sLse[SH_ROWS], sSum[WARPS][SH_ROWS];
+    __shared__ float sLse[SH_ROWS], sOut[SH_ROWS];
+    __shared__ float2 sSum[WARPS][SH_ROWS];                /* a warp's sum of p dp in a row, and the largest |p dp| */
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t base = (SmemAddr(smemRaw) + 1023u) & ~1023u;
     const uint32_t kT = base, vT = kT + SM::TILE, qS = vT + SM::TILE, doS = qS + SM::ROWS_BYTES, dsS = doS + SM::ROWS_BYTES;
@@ -159,6 +160,7 @@ XattnGradShortKernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
 #pragma unroll
         for (int e = 0; e < 4; e++)
             dk[i][e] = dv[i][e] = 0.f;
+    float factorK = DS_UNSET;                                 /* of this warp's ds in dk (ntb_xattn.cuh) */
 
     for (int c = 0; c < chunks; c++) {
         __syncthreads();                                  /* the chunk's rows are there, the last chunk's ds has been read */
@@ -207,43 +209,75 @@ XattnGradShortKernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
         for (int mt = 0; mt < 2; mt++)
 #pragma unroll
             for (int hf = 0; hf < 2; hf++) {
-                float sum = 0.f;
+                float sum = 0.f, top = 0.f;
 #pragma unroll
                 for (int nb = 0; nb < 2; nb++)
 #pragma unroll
-                    for (int e = hf * 2; e < hf * 2 + 2; e++)
+                    for (int e = hf * 2; e < hf * 2 + 2; e++) {
                         sum = fmaf(w[mt][nb][e], g[mt][nb][e], sum);
+                        top = fmaxf(top, fabsf(w[mt][nb][e] * g[mt][nb][e]));
+                    }
                 sum += __shfl_xor_sync(0xffffffffu, sum, 1);
                 sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
                 if ((lane & 3) == 0)
-                    sSum[warp][mt * 16 + hf * 8 + (lane >> 2)] = sum;
+                    sSum[warp][mt * 16 + hf * 8 + (lane >> 2)] = make_float2(sum, top);
             }
         __syncthreads();
         if (valid > 0) {
-            /* halves of 2^12 p and of ds, transposed: the A operands of dv's and dk's products; ds to shared memory, too */
-            uint32_t dsT[2][4], pT[2][4];
+            /* ds in the place of dp; to shared memory as halves times the row's factor, by a bound of its ds that all warps know:
+               the largest p dp and, as p is at most 1, delta */
+            float most = 0.f;
 #pragma unroll
             for (int mt = 0; mt < 2; mt++)
 #pragma unroll
                 for (int hf = 0; hf < 2; hf++) {
                     const int r = mt * 16 + hf * 8 + (lane >> 2);
-                    float delta = 0.f;                    /* the keys' sums, by all threads in the same order */
+                    float delta = 0.f, top = 0.f;         /* the keys' sums, by all threads in the same order */
 #pragma unroll
-                    for (int k = 0; k < WARPS; k++)
-                        delta += sSum[k][r];
+                    for (int k = 0; k < WARPS; k++) {
+                        const float2 s = sSum[k][r];
+                        delta += s.x;
+                        top = fmaxf(top, s.y);
+                    }
+                    top += fabsf(delta);
+                    const float factor = top < INFINITY ? PowerFor(top, 14) : 1.f;
+                    if (warp == 0 && (lane & 3) == 0)
+                        sOut[r] = SumsFactor(PowerInverse(factor), p.scale);
 #pragma unroll
                     for (int nb = 0; nb < 2; nb++) {
-                        const float a = w[mt][nb][hf * 2], d = w[mt][nb][hf * 2 + 1];
                         /* a key past the end stays 0 where delta is not finite */
                         const int key = nb * 8 + (lane & 3) * 2;
-                        const uint32_t ds = PackHalf2(key < valid ? a * (g[mt][nb][hf * 2] - delta) : 0.f,
-                                                      key + 1 < valid ? d * (g[mt][nb][hf * 2 + 1] - delta) : 0.f);
+                        float & a = g[mt][nb][hf * 2], & d = g[mt][nb][hf * 2 + 1];
+                        a = key < valid ? w[mt][nb][hf * 2] * (a - delta) : 0.f;
+                        d = key + 1 < valid ? w[mt][nb][hf * 2 + 1] * (d - delta) : 0.f;
+                        most = fmaxf(most, fmaxf(fabsf(a), fabsf(d)));
                         const uint32_t at = dsS + (key0 >> 6) * SH_CHUNK + r * ROW_BYTES + (((((key0 & 63) >> 3) + nb) ^ (r & 7)) << 4) + (lane & 3) * 4;
-                        asm volatile("st.shared.b32 [%0], %1;" :: "r"(at), "r"(ds) : "memory");
-                        dsT[mt][hf * 2 + nb] = MoveTrans(ds);
-                        pT[mt][hf * 2 + nb] = MoveTrans(PackHalf2(a * P_SCALE, d * P_SCALE));
+                        asm volatile("st.shared.b32 [%0], %1;" :: "r"(at), "r"(PackHalf2(a * factor, d * factor)) : "memory");
                     }
                 }
+            most = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(most)));
+            if (DsPast(most, factorK)) {
+                const float now = PowerFor(most, DS_TOP), f = now * PowerInverse(factorK);
+                factorK = now;
+#pragma unroll
+                for (int i = 0; i < D / 8; i++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++)
+                        dk[i][e] *= f;
+            }
+            /* halves of 2^12 p and of ds, transposed: the A operands of dv's and dk's products */
+            uint32_t dsT[2][4], pT[2][4];
+#pragma unroll
+            for (int mt = 0; mt < 2; mt++)
+#pragma unroll
+                for (int hf = 0; hf < 2; hf++)
+#pragma unroll
+                    for (int nb = 0; nb < 2; nb++) {
+                        dsT[mt][hf * 2 + nb] = MoveTrans(PackHalf2(g[mt][nb][hf * 2] * factorK, g[mt][nb][hf * 2 + 1] * factorK));
+                        pT[mt][hf * 2 + nb] = MoveTrans(PackHalf2(w[mt][nb][hf * 2] * P_SCALE, w[mt][nb][hf * 2 + 1] * P_SCALE));
+                    }
 #pragma unroll
             for (int i = 0; i < D / 16; i++)
 #pragma unroll
@@ -284,10 +318,11 @@ XattnGradShortKernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
         for (int hf = 0; hf < 2; hf++) {
             const int i = (c - gq * perHead) * SH_ROWS + dqRow + hf * 8 + (lane >> 2);
             __half * row = p.dq + b * p.lDQ.batch + (kvHead * p.sh.group + gq) * p.lDQ.head + i * p.lDQ.row + dqCol;
+            const float out = sOut[dqRow + hf * 8 + (lane >> 2)];
             uint32_t h[DQ_COLS / 8];
 #pragma unroll
             for (int n = 0; n < DQ_COLS / 8; n++)
-                h[n] = PackHalf2(dq[n][hf * 2] * p.scale, dq[n][hf * 2 + 1] * p.scale);
+                h[n] = PackHalf2(dq[n][hf * 2] * out, dq[n][hf * 2 + 1] * out);
             if (DQ_COLS >= 32) {
                 /* the four lanes of a row turn their pairs of four blocks of columns into a block of eight columns each */
 #pragma unroll
@@ -315,6 +350,7 @@ XattnGradShortKernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
         }
     }
     __syncthreads();                                      /* k has been read by all */
+    const float outK = SumsFactor(PowerInverse(factorK), p.scale);
     if (valid > 0) {
         /* dv and dk in the place of v and k, and out */
 #pragma unroll
@@ -327,7 +363,7 @@ XattnGradShortKernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
                 asm volatile("st.shared.b32 [%0], %1;" :: "r"(vT + at),
                              "r"(live ? PackHalf2(dv[i][hf * 2] * P_SCALE_INV, dv[i][hf * 2 + 1] * P_SCALE_INV) : 0u) : "memory");
                 asm volatile("st.shared.b32 [%0], %1;" :: "r"(kT + at),
-                             "r"(live ? PackHalf2(dk[i][hf * 2] * p.scale, dk[i][hf * 2 + 1] * p.scale) : 0u) : "memory");
+                             "r"(live ? PackHalf2(dk[i][hf * 2] * outK, dk[i][hf * 2 + 1] * outK) : 0u) : "memory");
             }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();

@@ -518,12 +518,15 @@ XattnGradStepKernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
     __syncthreads();
 
     float dq[MT][D / 8][4];
+    float factor[MT][2];                      /* of each row's ds in this warp's dq (ntb_xattn.cuh) */
     {
 #pragma unroll
-        for (int mt = 0; mt < MT; mt++)
+        for (int mt = 0; mt < MT; mt++) {
+            factor[mt][0] = factor[mt][1] = DS_UNSET;
 #pragma unroll
             for (int i = 0; i < D / 8; i++)
                 dq[mt][i][0] = dq[mt][i][1] = dq[mt][i][2] = dq[mt][i][3] = 0.f;
+        }
         float lse2[MT][2], delta[MT][2];
 #pragma unroll
         for (int mt = 0; mt < MT; mt++)
@@ -636,6 +639,50 @@ XattnGradStepKernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
             }
             float w[MT][2][4], g[MT][2][4];
             weights(kT, vT, valid, w, g);
+            /* ds in the place of dp, the largest of each row, and of all */
+            float top[MT][2], most = 0.f;
+            bool past = false;
+#pragma unroll
+            for (int mt = 0; mt < MT; mt++)
+#pragma unroll
+                for (int hf = 0; hf < 2; hf++) {
+                    float t = 0.f;
+#pragma unroll
+                    for (int nb = 0; nb < 2; nb++)
+#pragma unroll
+                        for (int e = 0; e < 2; e++) {
+                            /* a key past the end stays 0 where delta is not finite */
+                            float & d = g[mt][nb][hf * 2 + e];
+                            d = nb * 8 + (lane & 3) * 2 + e < valid ? w[mt][nb][hf * 2 + e] * (d - delta[mt][hf]) : 0.f;
+                            t = fmaxf(t, fabsf(d));
+                        }
+                    t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 1));
+                    t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 2));
+                    top[mt][hf] = t;
+                    most = fmaxf(most, t);
+                    past = past || DsPast(t, factor[mt][hf]);
+                }
+            if (__any_sync(0xffffffffu, past)) {
+#pragma unroll
+                for (int mt = 0; mt < MT; mt++) {
+                    float f[2] = { 1.f, 1.f };
+#pragma unroll
+                    for (int hf = 0; hf < 2; hf++)
+                        if (DsPast(top[mt][hf], factor[mt][hf])) {
+                            const float now = PowerFor(top[mt][hf], DS_TOP);
+                            f[hf] = now * PowerInverse(factor[mt][hf]);
+                            factor[mt][hf] = now;
+                        }
+#pragma unroll
+                    for (int i = 0; i < D / 8; i++) {
+                        dq[mt][i][0] *= f[0]; dq[mt][i][1] *= f[0];
+                        dq[mt][i][2] *= f[1]; dq[mt][i][3] *= f[1];
+                    }
+                }
+            }
+            /* dk of these keys is made whole here: one factor for the warp's ds, from their largest */
+            most = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(most)));
+            const float factorK = most < INFINITY ? PowerFor(most, 14) : 1.f, outK = SumsFactor(PowerInverse(factorK), p.scale);
             /* halves of 2^12 p and of ds: as they are the A operand of dq's product, transposed those of dk's and dv's */
             uint32_t ds[MT][4], dsT[MT][4], pT[MT][4];
 #pragma unroll
@@ -644,15 +691,10 @@ XattnGradStepKernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
                 for (int nb = 0; nb < 2; nb++)
 #pragma unroll
                     for (int hf = 0; hf < 2; hf++) {
-                        const float a = w[mt][nb][hf * 2], c = w[mt][nb][hf * 2 + 1];
-                        /* a key past the end stays 0 where delta is not finite */
-                        const int key = nb * 8 + (lane & 3) * 2;
-                        const float da = key < valid ? a * (g[mt][nb][hf * 2] - delta[mt][hf]) : 0.f;
-                        const float dc = key + 1 < valid ? c * (g[mt][nb][hf * 2 + 1] - delta[mt][hf]) : 0.f;
-                        const uint32_t dsh = PackHalf2(da, dc);
-                        ds[mt][nb * 2 + hf] = dsh;
-                        dsT[mt][hf * 2 + nb] = MoveTrans(dsh);
-                        pT[mt][hf * 2 + nb] = MoveTrans(PackHalf2(a * P_SCALE, c * P_SCALE));
+                        const float da = g[mt][nb][hf * 2], dc = g[mt][nb][hf * 2 + 1];
+                        ds[mt][nb * 2 + hf] = PackHalf2(da * factor[mt][hf], dc * factor[mt][hf]);
+                        dsT[mt][hf * 2 + nb] = MoveTrans(PackHalf2(da * factorK, dc * factorK));
+                        pT[mt][hf * 2 + nb] = MoveTrans(PackHalf2(w[mt][nb][hf * 2] * P_SCALE, w[mt][nb][hf * 2 + 1] * P_SCALE));
                     }
 #pragma unroll
             for (int i = 0; i < D / 16; i++) {
@@ -669,7 +711,7 @@ XattnGradStepKernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
 #pragma unroll
             for (int which = 0; which < 2; which++) {
                 const uint32_t src = which == 0 ? doS : qS, dst = which == 0 ? vT : kT;
-                const float f = which == 0 ? P_SCALE_INV : p.scale;
+                const float f = which == 0 ? P_SCALE_INV : outK;
 #pragma unroll
                 for (int i = 0; i < D / 16; i++) {
                     float acc[2][4] = { { 0.f, 0.f, 0.f, 0.f }, { 0.f, 0.f, 0.f, 0.f } };
@@ -722,7 +764,8 @@ XattnGradStepKernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
 #pragma unroll
                 for (int hf = 0; hf < 2; hf++) {
                     const int r = mt * 16 + hf * 8 + (lane >> 2);
-                    *(float2 *)(part + (warp * R + r) * D + i * 8 + (lane & 3) * 2) = make_float2(dq[mt][i][hf * 2], dq[mt][i][hf * 2 + 1]);
+                    const float power = PowerInverse(factor[mt][hf]);
+                    *(float2 *)(part + (warp * R + r) * D + i * 8 + (lane & 3) * 2) = make_float2(dq[mt][i][hf * 2] * power, dq[mt][i][hf * 2 + 1] * power);
                 }
     }
     __syncthreads();
