@@ -246,7 +246,8 @@ int ntb_embedding_grad(int devID, void * stream, const int * ids, const void * d
  *        *norm = sqrt(sum over all tensors and elements of g^2),     out = g * min(1, maxNorm / *norm)
  *
  * grads, out, dtypes, counts: HOST arrays of `count` entries (device pointers, X_FLOAT16 or X_FLOAT, element
- * counts); out[i] may be grads[i] (in place); different entries must not overlap. norm: one float on the
+ * counts); out[i] may be grads[i] (in place); otherwise nothing written may overlap what is read, and no entry
+ * another that is written: NTB_ERR_ARG. norm: one float on the
  * device. A norm that is not finite (as a float) leaves the gradients' values as they are (the caller reads *norm and skips
  * the step); maxNorm infinite only takes the norm. maxNorm must not be negative or NaN. The sum is
  * fp64 (fp32 within eight exact products of halves); its order is fixed by the sizes. work: device scratch

@@ -15,6 +15,8 @@
  * floats in 260 tensors take 374 us for both: 2.5 GB read twice and written once, 6.7 TB/s with what L2 gives.
  */
 #include "ntb_xattn.cuh"
+#include <algorithm>
+#include <new>
 
 namespace ntb {
 
@@ -240,6 +242,40 @@ int Ctas(const DeviceCtx & ctx, int chunks)
     return chunks < 1 ? 1 : chunks < most ? chunks : most;
 }
 
+/*
+ * Whether what is written for one entry overlaps what is written for another, or what an entry is read from, but for an
+ * entry in place: CTAs read and write in no order, so such a call's result would depend on timing. The spans of a list that
+ * lies in a pool are in order already.
+ */
+struct ClipSpan {
+    uintptr_t lo, hi;
+};
+bool ClipOverlaps(int count, const void * const * grads, void * const * out, const int * dtypes, const long long * counts, ClipSpan * spans)
+{
+    auto span = [&](const void * p, int i) {
+        const uintptr_t lo = (uintptr_t)p;
+        return ClipSpan{ lo, lo + (uintptr_t)counts[i] * (dtypes[i] == NTB_X_FLOAT16 ? 2 : 4) };
+    };
+    auto before = [](const ClipSpan & a, const ClipSpan & b) { return a.lo < b.lo; };
+    int n = 0;
+    for (int i = 0; i < count; i++)
+        if (counts[i] > 0)
+            spans[n++] = span(out[i], i);
+    if (!std::is_sorted(spans, spans + n, before))
+        std::sort(spans, spans + n, before);
+    for (int i = 1; i < n; i++)
+        if (spans[i].lo < spans[i - 1].hi)
+            return true;
+    for (int i = 0; i < count; i++)
+        if (counts[i] > 0 && grads[i] != out[i]) {
+            const ClipSpan g = span(grads[i], i);
+            const ClipSpan * s = std::upper_bound(spans, spans + n, g, before);        /* the first written behind g's start */
+            if ((s < spans + n && s->lo < g.hi) || (s > spans && s[-1].hi > g.lo))
+                return true;
+        }
+    return false;
+}
+
 template <int MAX>
 int ClipGroups(const DeviceCtx & ctx, int count, const void * const * grads, void * const * out, const int * dtypes, const long long * counts,
                float maxNorm, float * norm, double * partial, cudaStream_t stream)
@@ -323,6 +359,14 @@ extern "C" int ntb_clip_grad_norm(int devID, void * stream, int count, const voi
         if (chunks > 0x7fff0000LL)
             return NTB_ERR_LIMIT;
     }
+    ClipSpan few[CL_FEW], * spans = count <= CL_FEW ? few : new (std::nothrow) ClipSpan[count];
+    if (!spans)
+        return NTB_ERR_LIMIT;
+    const bool overlaps = ClipOverlaps(count, grads, out, dtypes, counts, spans);
+    if (spans != few)
+        delete[] spans;
+    if (overlaps)
+        return NTB_ERR_ARG;
     XattnDevice dev(devID);
     if (!dev.ok)
         return NTB_ERR_CUDA;

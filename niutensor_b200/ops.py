@@ -389,7 +389,8 @@ _CLIP_TYPES = {torch.float32, torch.float16}
 def ClipGradNorm(grads, max_norm, out=None):
     """The 2-norm of a list of gradients together, as a float tensor on their device, and the gradients times
     min(1, max_norm / norm): in place, or into the tensors of out. Packed fp16 and fp32 CUDA tensors of any
-    shapes on one device, each listed once. A norm that is not finite leaves the values as they are. Two launches,
+    shapes on one device, each listed once; what is written overlaps neither what is read, but for a tensor in place,
+    nor another tensor of the list. A norm that is not finite leaves the values as they are. Two launches,
     no copy to the device, no synchronisation."""
     n = len(grads)
     _check(n > 0, "Empty input tensors!")
