@@ -1120,7 +1120,10 @@ extern "C" int ntb_cross_attention_grad(int devID, void * stream, const void * q
     int rc = XattnShapeOf(call.sh, dtype, batch, headsQ, headsKV, lenQ, lenK, dim, queryLens, keyLens, scale);
     if (rc != NTB_OK)
         return rc;
-    if (batch == 0 || headsKV == 0 || headsQ == 0 || (lenQ == 0 && lenK == 0))
+    /* without query heads dk and dv are the sums of nothing, as without queries */
+    if (headsQ == 0)
+        lenQ = call.sh.lenQ = 0;
+    if (batch == 0 || headsKV == 0 || (lenQ == 0 && lenK == 0))
         return NTB_OK;
     if (!layouts || (lenQ > 0 && (!q || !out || !lse || !dout || !dq)) || (lenK > 0 && (!k || !v || !dk || !dv)))
         return NTB_ERR_ARG;
