@@ -587,7 +587,7 @@ __global__ void __launch_bounds__(FEW_THREADS) FewTokensKernel(const FewParams p
         /* clear the rows of the words that do not occur */
         unsigned * seen = (unsigned *)words;
         const int ctas = gridDim.x - p.sumCtas * p.colBlocks;
-        const int each = (p.vocab + ctas - 1) / ctas;
+        const int each = (int)(((long long)p.vocab + ctas - 1) / ctas);
         const long long first = (long long)(blockIdx.x - p.sumCtas * p.colBlocks) * each;
         const int end = first + each < p.vocab ? (int)(first + each) : p.vocab;
         for (long long lo64 = first; lo64 < end; lo64 += FEW_CLEAR_ROWS) {
@@ -602,7 +602,7 @@ __global__ void __launch_bounds__(FEW_THREADS) FewTokensKernel(const FewParams p
                     atomicOr(seen + ((id - lo) >> 5), 1u << ((id - lo) & 31));
             }
             __syncthreads();
-            for (int v = lo + warp; v < hi; v += FEW_WARPS)
+            for (long long v = lo + warp; v < hi; v += FEW_WARPS)           /* it passes hi, which may be 2^31 - 2 */
                 if (((seen[(v - lo) >> 5] >> ((v - lo) & 31)) & 1u) == 0u)
                     ClearWarp((unsigned char *)((TW *)p.dw + v * p.ldw), (long long)p.dim * sizeof(TW), lane);
         }
@@ -731,8 +731,6 @@ cudaError_t LaunchFew(FewParams p, bool vec, int clearing, cudaStream_t stream)
     const int cols = vec ? FEW_COLS<EmVec<TO>::N> : FEW_COLS<1>;
     p.colBlocks = (p.dim + cols - 1) / cols;
     const long long grid = (long long)p.sumCtas * p.colBlocks + clearing;
-    if (grid > 0x7fffffffLL)
-        return cudaErrorInvalidValue;
     const cudaError_t err = vec ? LaunchPdl(FewTokensKernel<TO, TW, true>, (int)grid, FEW_THREADS, 0, stream, p)
                                 : LaunchPdl(FewTokensKernel<TO, TW, false>, (int)grid, FEW_THREADS, 0, stream, p);
     CountLaunch();
@@ -805,6 +803,9 @@ int SortCtas(int tokens)
     return tokens <= 16384 ? 8 : SORT_CTAS;
 }
 
+/* column indices run up to a CTA's columns past the end in 32 bits */
+constexpr int EM_MOST_COLS = 0x7fffff00;
+
 bool RowsAligned(const void * p, long long pitch, int dim, int size)
 {
     return ((uintptr_t)p & 15) == 0 && (pitch * size) % 16 == 0 && (dim * (long long)size) % 16 == 0;
@@ -862,6 +863,8 @@ extern "C" int ntb_embedding(int devID, void * stream, const int * ids, const vo
         return NTB_OK;
     if (!ids || !out || (vocab > 0 && !w))
         return NTB_ERR_ARG;
+    if (dim > EM_MOST_COLS)
+        return NTB_ERR_LIMIT;
     XattnDevice dev(devID);
     if (!dev.ok)
         return NTB_ERR_CUDA;
@@ -904,7 +907,15 @@ extern "C" int ntb_embedding_grad(int devID, void * stream, const int * ids, con
     if (workBytes < ntb_embedding_grad_work(tokens, dim) || (tokens > 0 && (!work || ((uintptr_t)work & 15))))
         return NTB_ERR_ARG;
     /* the sort packs a token's number and its word into 32 bits each, with one value past the last word */
-    if (vocab == 0x7fffffff || tokens > 0x7fffff00)
+    if (vocab == 0x7fffffff || tokens > 0x7fffff00 || dim > EM_MOST_COLS)
+        return NTB_ERR_LIMIT;
+    const bool halves = dtypeOut == NTB_X_FLOAT16, halfW = dtypeW == NTB_X_FLOAT16;
+    const bool wide = !halves ? WideRows<float, float>(dout, ldo, dw, ldw, dim)
+        : !halfW ? WideRows<__half, float>(dout, ldo, dw, ldw, dim) : WideRows<__half, __half>(dout, ldo, dw, ldw, dim);
+    const bool few = tokens <= (wide ? FEW_TOKENS : FEW_TOKENS / 2);
+    /* CTAs along a launch's x where one launch does it all, blocks of columns along y where the list is sorted */
+    const long long threads = wide ? dim / (halves ? EmVec<__half>::N : EmVec<float>::N) : dim;
+    if (few ? (long long)((tokens + FEW_WARPS - 1) / FEW_WARPS) * (dim / (wide && halves ? 256 : 128) + 1) > 0x7fff0000LL : (threads + 255) / 256 > 65535)
         return NTB_ERR_LIMIT;
     XattnDevice dev(devID);
     if (!dev.ok)
@@ -913,10 +924,7 @@ extern "C" int ntb_embedding_grad(int devID, void * stream, const int * ids, con
     if (!ctx)
         return NTB_ERR_CUDA;
     cudaStream_t st = (cudaStream_t)stream;
-    const bool halves = dtypeOut == NTB_X_FLOAT16, halfW = dtypeW == NTB_X_FLOAT16;
-    const bool wide = !halves ? WideRows<float, float>(dout, ldo, dw, ldw, dim)
-        : !halfW ? WideRows<__half, float>(dout, ldo, dw, ldw, dim) : WideRows<__half, __half>(dout, ldo, dw, ldw, dim);
-    if (tokens <= (wide ? FEW_TOKENS : FEW_TOKENS / 2)) {
+    if (few) {
         FewParams f;
         memset(&f, 0, sizeof(f));
         f.ids = ids;
@@ -929,7 +937,7 @@ extern "C" int ntb_embedding_grad(int devID, void * stream, const int * ids, con
         f.sumCtas = (tokens + FEW_WARPS - 1) / FEW_WARPS;
         int clearing = 0;
         if (beta == 0.f) {
-            const int most = 4 * ctx->smCount, want = (vocab + FEW_WARPS - 1) / FEW_WARPS;
+            const int most = 4 * ctx->smCount, want = (int)(((long long)vocab + FEW_WARPS - 1) / FEW_WARPS);
             clearing = want < most ? want : most;
         }
         const cudaError_t e = !halves ? LaunchFew<float, float>(f, wide, clearing, st)
