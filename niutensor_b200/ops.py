@@ -47,6 +47,10 @@ def _stream(t):
 _raw_stream = torch._C._cuda_getCurrentRawStream
 
 
+#: sizes are ints in the library, and ctypes would cut longer ones off without a word
+_INT_MAX = 0x7fffffff
+
+
 def _common_checks(a, b, c):
     _check(a is not None and b is not None and c is not None, "Empty input tensors!")
     _check(a.is_cuda and b.is_cuda and c.is_cuda,
@@ -263,6 +267,7 @@ def _cross_attention_checks(q, k, v, query_lens, key_lens, scale, others=()):
             _check(t.dim() == 4, "Input tensors must have a order = 4!")
     qs, ks = q.shape, k.shape
     d = qs[3]
+    _check(max(qs) <= _INT_MAX and max(ks) <= _INT_MAX, "an extent exceeds 32 bits")
     _check(ks == v.shape and ks[0] == qs[0] and ks[3] == d, "Unmatched tensors in multiplication!")
     _check(qs[1] == 0 or (ks[1] > 0 and qs[1] % ks[1] == 0), "the key heads must divide the query heads")
     _check(d % 8 == 0 and 8 <= d <= 128, "the head size must be a multiple of 8 up to 128")
@@ -351,6 +356,7 @@ def Embedding(w, ids, scale=1.0, pos=None):
                "positions must be a packed matrix of the words' type and width")
         rows = pos.shape[0]
         _check(tokens == 0 or (rows > 0 and tokens % rows == 0), "Incorrect tensor sizes!")
+    _check(max(tokens, vocab, d) <= _INT_MAX, "an extent exceeds 32 bits")
     out = w.new_empty(ids.shape + (d,))
     rc = capi.lib().ntb_embedding(dev, _raw_stream(dev), ids.data_ptr(), w.data_ptr(), _ptr(pos) if rows else None, out.data_ptr(), dtype,
                                   tokens, vocab, d, pitch if vocab > 1 else d, d, rows, scale)
@@ -374,6 +380,7 @@ def GradEmbedding(ids, dedc, dedw, scale=1.0, beta=1.0):
     _check(dedc.is_contiguous() and dedc.shape == ids.shape + (d,), "Incorrect tensor sizes!")
     _check(beta == 0.0 or beta == 1.0, "beta must be 0 or 1")
     tokens = ids.numel()
+    _check(max(tokens, vocab, d) <= _INT_MAX, "an extent exceeds 32 bits")
     lib = capi.lib()
     need = lib.ntb_embedding_grad_work(tokens, d)
     work = torch.empty(need, dtype=torch.uint8, device=dedw.device)
