@@ -152,6 +152,8 @@ XattnStepKernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
             ok = MbarWaitWarp(SmemAddr(&barFull[st]), (uint32_t)(j / STAGES) & 1u, abortPtr, p.status, 200);
             if (!ok)
                 break;
+            /* the first lane waited; every lane observes the copy's completion itself before it reads what was copied */
+            (void)MbarTryWait(SmemAddr(&barFull[st]), (uint32_t)(j / STAGES) & 1u, 0);
             const uint32_t kT = ring + st * 2 * SM::TILE, vT = kT + SM::TILE;
             const int valid = nk - (tile0 + j) * ST_KEYS - key0;              /* of this warp's 16 keys */
             if (valid > 0) {
