@@ -164,7 +164,9 @@ int ntb_attention_dropout(int devID, void * stream,
  * Calls with at most 32 query rows for a key head ((headsQ / headsKV) * lenQ: a decoding step, the
  * hypotheses of a beam as lenQ rows of one sentence) read k and v once for all of them; fewer rows
  * than fill the GPU split the keys over a cluster. Sums and statistics are fp32; weights are
- * rounded to half for the second product. Results do not depend on timing. No workspace.
+ * rounded to half for the second product. The tensor core's fp32 sums round toward zero: up to 2^18 keys (2^20 with at
+ * most 32 rows) a result falls short by less than 2^-12 of itself, beyond that by that much again for as many
+ * keys more. Results do not depend on timing. No workspace.
  */
 typedef struct ntb_heads_layout {
     long long batch, head, row;      /* strides in elements */

@@ -597,11 +597,10 @@ int DispatchXattn(const DeviceCtx & ctx, const XattnCall & call, cudaStream_t st
        (two CTAs per SM) spread wider */
     const bool two = units >= 2 && heads * ((units + 1) / 2) >= ctx.smCount;
     const long long items = two ? heads * ((units + 1) / 2) : heads * units;
-    /* split the keys until the GPU is full, while a part keeps two tiles; and into parts short enough (131072 keys)
-       that the tensor core's accumulator, which rounds toward zero at every instruction, stays good */
+    /* split the keys until the GPU is full, while a part keeps two tiles; and into parts of few enough instructions */
     int splits = 1;
     const int keyTiles = (s.lenK + XT - 1) / XT;
-    while (splits < 8 && ((items * splits * 2 <= 2LL * ctx.smCount && keyTiles >= splits * 4) || keyTiles / splits > 1024))
+    while (splits < 8 && ((items * splits * 2 <= 2LL * ctx.smCount && keyTiles >= splits * 4) || keyTiles > splits * XATTN_PART_TILES))
         splits *= 2;
     if (s.dim <= 64)
         return two ? LaunchXattn<64, 2>(ctx, call, p, splits, stream) : LaunchXattn<64, 1>(ctx, call, p, splits, stream);

@@ -58,6 +58,10 @@ namespace {
 
 constexpr int XT = 128;                               /* rows of a query tile and keys of a key tile */
 constexpr int XBOX_BYTES = XT * ROW_BYTES;            /* 128 rows x 64 halves: one swizzled box of an operand tile */
+/* Tiles of a walk that one part takes before it is split, as far as 8 parts go, whatever the GPU's load. The tensor core's
+   fp32 accumulator rounds toward zero at every instruction of 16 keys, which costs a sum some 2^-23.5 of itself each: 2^-12.5 over
+   256 tiles (measured: 1024 tiles fall short by 7e-4, more than a half's rounding). */
+constexpr int XATTN_PART_TILES = 256;
 constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
 
 /* The reference that the forward kernels take off the exponents (of 2): XATTN_BELOW under the row's maximum when it

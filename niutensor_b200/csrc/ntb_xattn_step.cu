@@ -849,13 +849,15 @@ int LaunchGradStep(const XattnGradCall & call, const StepGradParams & base, cuda
     return (err == cudaSuccess && cudaGetLastError() == cudaSuccess) ? NTB_OK : NTB_ERR_CUDA;
 }
 
-/* split the keys until there are about two CTAs an SM, while a part keeps two tiles */
+/* split the keys until there are about two CTAs an SM, while a part keeps two tiles; and into parts of few enough
+   instructions (one a warp and tile; ntb_xattn.cuh says why) */
+constexpr int ST_PART_TILES = XATTN_PART_TILES * XT / 16;
 int StepSplits(const DeviceCtx & ctx, const XattnShape & s)
 {
     const long long heads = (long long)s.batch * s.headsKV;
     const int tiles = (s.lenK + ST_KEYS - 1) / ST_KEYS;
     int splits = 1;
-    while (splits < 8 && heads * splits < 2LL * ctx.smCount && tiles >= splits * 4)
+    while (splits < 8 && ((heads * splits < 2LL * ctx.smCount && tiles >= splits * 4) || tiles > splits * ST_PART_TILES))
         splits *= 2;
     return splits;
 }
@@ -874,7 +876,7 @@ int GradStepSplits(const DeviceCtx & ctx, const XattnShape & s, int places)
     for (int n = 1; n == 1 || (n <= 8 && tiles >= 2 * n); n *= 2) {
         const long long slots = (long long)places * ctx.smCount;
         const long long cost = (heads * n + slots - 1) / slots * ((tiles + n - 1) / n + 4);
-        if (n == 1 || cost < best) {
+        if (n == 1 || cost < best || tiles > splits * ST_PART_TILES) {
             best = cost;
             splits = n;
         }
