@@ -161,9 +161,8 @@ __global__ void __launch_bounds__(CL_THREADS) NormKernel(const __grid_constant__
     }
 }
 
-/* four CTAs an SM: with 40 registers and three the 209 M floats take 397 us instead of 386 */
 template <int MAX>
-__global__ void __launch_bounds__(CL_THREADS, 4) ClipKernel(const __grid_constant__ ClipList<MAX> l)
+__global__ void __launch_bounds__(CL_THREADS) ClipKernel(const __grid_constant__ ClipList<MAX> l)
 {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -184,11 +183,17 @@ __global__ void __launch_bounds__(CL_THREADS, 4) ClipKernel(const __grid_constan
     if (blockIdx.x == 0 && threadIdx.x == 0 && l.norm != nullptr)
         *l.norm = (float)norm;
     const bool clip = norm > (double)l.maxNorm && !isinf((float)norm);       /* as the caller sees it */
-    const double ratio = (double)l.maxNorm / norm;
+    /* A factor below a float's normal range would lose its bits, or all of them, where a clipped value is an ordinary float:
+       a power of two goes first then, exactly where the result is not below a float's normal range itself. (The factor as a
+       double, and all registers that takes, cost every call 3 %.) */
+    double ratio = (double)l.maxNorm / norm;
+    float f0 = 1.f;
+    if (clip && ratio < 7.8886090522101181e-31) {                            /* 2^-100 */
+        const bool least = ratio < 9.273015376718553e-69;                   /* 2^-226 */
+        f0 = least ? 2.9387358770557188e-39f : 7.8886090522101181e-31f;      /* 2^-128, 2^-100 */
+        ratio *= least ? 3.4028236692093846e38 : 1.2676506002282294e30;
+    }
     const float f = clip ? (float)ratio : 1.f;
-    /* a factor below a float's normal range would lose its bits, or all of them, where a clipped value is an ordinary float:
-       then it stays fp64, one element at a time */
-    const bool tiny = clip && ratio < 1.1754943508222875e-38;                /* 2^-126 */
     for (int k = blockIdx.x; k < l.chunks; k += gridDim.x) {
         const int chunk = l.chunks - 1 - k;
         const ClipTensor & t = l.t[TensorOf(l, chunk)];
@@ -197,11 +202,9 @@ __global__ void __launch_bounds__(CL_THREADS, 4) ClipKernel(const __grid_constan
         const ChunkRange r = RangeOf(t, chunk);
         const bool half = t.half != 0;
         const int size = half ? 2 : 4;
-        if (tiny || (((uintptr_t)t.in ^ (uintptr_t)t.out) & 15) != 0) {
-            for (long long i = r.lo + threadIdx.x; i < r.hi; i += CL_THREADS) {
-                const float g = Element(t.in, i, half);
-                SetElement(t.out, i, half, tiny ? (float)(g * ratio) : g * f);
-            }
+        if ((((uintptr_t)t.in ^ (uintptr_t)t.out) & 15) != 0) {
+            for (long long i = r.lo + threadIdx.x; i < r.hi; i += CL_THREADS)
+                SetElement(t.out, i, half, Element(t.in, i, half) * f0 * f);
             continue;
         }
         const uint4 * v = (const uint4 *)((const char *)t.in + r.body * size);
@@ -223,19 +226,19 @@ __global__ void __launch_bounds__(CL_THREADS, 4) ClipKernel(const __grid_constan
                 for (int e = 0; e < 4; e++) {
                     if (half) {
                         const float2 g = __half22float2(*(const __half2 *)&w[e]);
-                        w[e] = PackHalf2(g.x * f, g.y * f);
+                        w[e] = PackHalf2(g.x * f0 * f, g.y * f0 * f);
                     }
                     else
-                        w[e] = __float_as_uint(__uint_as_float(w[e]) * f);
+                        w[e] = __float_as_uint(__uint_as_float(w[e]) * f0 * f);
                 }
                 __stcs(o + i, make_uint4(w[0], w[1], w[2], w[3]));
             }
         }
         const long long tail = r.body + (long long)r.packs * r.perPack;
         if (threadIdx.x < r.body - r.lo)
-            SetElement(t.out, r.lo + threadIdx.x, half, Element(t.in, r.lo + threadIdx.x, half) * f);
+            SetElement(t.out, r.lo + threadIdx.x, half, Element(t.in, r.lo + threadIdx.x, half) * f0 * f);
         if (threadIdx.x < r.hi - tail)
-            SetElement(t.out, tail + threadIdx.x, half, Element(t.in, tail + threadIdx.x, half) * f);
+            SetElement(t.out, tail + threadIdx.x, half, Element(t.in, tail + threadIdx.x, half) * f0 * f);
     }
 }
 

@@ -1,5 +1,6 @@
-"""Clipping by factors below a float's normal range: the norm is within 2^-21, the product is formed in 64 bits and rounded
-to a float once (2^-24 of itself, at most 2^-149)."""
+"""Clipping by factors below a float's normal range: the norm is within 2^-21 and the factor, of which a power of two is taken
+out, within 2^-24 of itself; the product with that power is exact where the result is normal, and the last product rounds
+once (2^-24, below the normal range 2^-149 at most)."""
 import math
 
 import pytest
