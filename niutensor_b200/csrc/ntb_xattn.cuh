@@ -221,9 +221,10 @@ __device__ __forceinline__ uint64_t Mul2(uint64_t a, uint64_t b)
 /*
  * The gradient kernels' ds = p (dp - delta) go into their products as halves. They are smaller than what they are
  * summed to by p, about 1 / lenK, and left as they are would be subnormal or 0 where dq and dk are ordinary halves, or,
- * with large v and a small scale, infinite. So every row of a product's ds carries a power of two, taken out of its sums in
- * fp32, that brings its largest to [2^DS_TOP, 2^(DS_TOP + 1)) when it is set, and is set again when ds have grown past
- * DS_MOST. ds down to 2^-21 of the largest are then off by 2^-11 of themselves, smaller ones by 2^-32 of the largest.
+ * with large v and a small scale, infinite. So the ds of a product carry a power of two, taken out of its sums in fp32:
+ * where they are met one after the other a row's, that brings its largest to [2^DS_TOP, 2^(DS_TOP + 1)) when it is set and is
+ * set again when ds have grown past DS_MOST; where the largest is known before, one that brings that to [2^14, 2^15). ds down to
+ * 2^-21 of the largest are then off by 2^-11 of themselves, smaller ones by 2^-32 of the largest.
  */
 constexpr float DS_MOST = 32768.f, DS_UNSET = 1208925819614629174706176.f;      /* 2^15; 2^80: nothing but zeros so far */
 constexpr int DS_TOP = 7;
@@ -249,6 +250,14 @@ __device__ __forceinline__ uint32_t PackHalf2(float lo, float hi)
 {
     const __half2 h = __floats2half2_rn(lo, hi);
     return *(const uint32_t *)&h;
+}
+
+/* the same with the largest half for what is larger (NaN stays NaN) */
+__device__ __forceinline__ uint32_t PackHalf2Finite(float lo, float hi)
+{
+    uint32_t r;
+    asm("cvt.rn.satfinite.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
 }
 
 __device__ __forceinline__ void LoadShared16(uint32_t addr, uint32_t * v)

@@ -31,9 +31,12 @@
  * instructions came from L2 for every tile, 0.5 to 1 us of the 8 a short item takes (sentences 69.4 -> 65.2 us).
  *
  * Rounding: p is at most 1 and may be tiny (1 / lenK); for dv it is rounded to half as 2^12 p, exact powers
- * of two away from half's subnormals. ds is rounded to half times a power of two of its row (of the query's for dq, of
- * the key's for dk; ntb_xattn.cuh says why), which follows the row's largest ds as the walk goes on: a vote of
- * the softmax threads in every step, and where one of them calls for it, the accumulators scaled. Sums are fp32.
+ * of two away from half's subnormals. ds is rounded to half times a power of two (ntb_xattn.cuh says why). In the first
+ * kernel that is a row's and follows the row's largest ds as the walk goes on: a vote of the softmax threads in every step,
+ * and where one of them calls for it, the accumulators scaled. The second kernel has one for all ds of a key head, from the
+ * largest that the first has met: its exponent, a bit each, takes the place of the low bits of eight rows' delta (2^-23 of
+ * delta, whose fp32 sum is off by more). A ds of the second kernel past that largest is the rounding of scores and dp, where
+ * they cancel: it saturates. With a vote in the second kernel, too, documents took 467 us instead of 434. Sums are fp32.
  */
 #include "ntb_xattn.cuh"
 
@@ -71,10 +74,10 @@ template <int D> struct XattnGradSmem {
     /* first kernel: a ring of k and v tiles (q and do are in tensor memory) */
     static constexpr int SLOTS = 7;
     static constexpr int Q_TOTAL = SLOTS * TILE + 1024;
-    /* second kernel: k, v, rings of q, of do, and of the query rows' (lse, delta); barriers; a word a row */
+    /* second kernel: k, v, rings of q, of do, and of the query rows' (lse, delta); barriers */
     static constexpr int QSLOTS = 3, DOSLOTS = 2, STATSLOTS = 2, STAT = 2 * XT * 4;
     static constexpr int KV_RING = 2 * TILE, KV_STATS = KV_RING + (QSLOTS + DOSLOTS) * TILE, KV_BARS = KV_STATS + STATSLOTS * STAT;
-    static constexpr int KV_WORDS = KV_BARS + 256, KV_TOTAL = KV_WORDS + XT * 4;
+    static constexpr int KV_TOTAL = KV_BARS + 256;
     static_assert(SLOTS * TILE >= XT * D * 4 && (QSLOTS + DOSLOTS) * TILE >= 2 * XT * D * 4, "the split's partial sums take the place of the rings");
     static_assert(KV_TOTAL <= 232448, "shared memory of a CTA");
 };
@@ -217,7 +220,7 @@ XattnGradQKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
     __shared__ __align__(8) uint64_t barFull[SLOTS], barEvent[GR_EVENTS], barRows, barQ, barS, barSRead, barDP, barDS, barDone, barFix;
     __shared__ uint32_t tmemBaseSlot;
     __shared__ int abortFlag;
-    __shared__ float sDelta[XT];
+    __shared__ float sDelta[XT], sMost[8];
 
     const int warp = threadIdx.x >> 5;
     const int lane = threadIdx.x & 31;
@@ -278,6 +281,18 @@ XattnGradQKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
     const bool single = keyTiles == 1;
     /* the last tile reaches past the sequence's keys into rows that exist: those rows of k are cleared */
     const bool fix = n > 0 && tile1 * XT > nk && nk < p.sh.lenK;
+
+    float deltaLeft = 0.f;
+    /* by the first warp, when all have left their largest ds in sMost: the exponent of the item's */
+    auto leaveMost = [&]() {
+        float most = 0.f;
+        if (lane < 8)
+            for (int t = 0; t < p.splits; t++)
+                most = fmaxf(most, p.splits > 1 ? LoadRemote(MapShared(SmemAddr(&sMost[lane]), t)) : sMost[lane]);
+        const uint32_t e = __reduce_max_sync(0xffffffffu, __float_as_uint(most)) >> 23;
+        if (lane < 8)
+            p.work[(long long)item * (2 * XT) + XT + lane] = __uint_as_float((__float_as_uint(deltaLeft) & ~1u) | (e >> lane & 1u));
+    };
 
     if (warp == GR_PRODUCER) {
         if (lane == 0 && n > 0) {
@@ -456,14 +471,14 @@ XattnGradQKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
             if (hf == 0 && rank == 0) {
                 float * w = p.work + (long long)item * (2 * XT);
                 w[r] = lse2 - P_SCALE_LOG2;
-                w[XT + r] = -delta * P_SCALE_INV;
+                w[XT + r] = deltaLeft = -delta * P_SCALE_INV;
             }
         };
         if (!single)
             leaveRow();
         const uint32_t sT = tmemBase + laneBase + TMEM_S + hf * 64, dpT = tmemBase + laneBase + TMEM_DP + hf * 64;
         const uint32_t dqT = tmemBase + laneBase + TMEM_DQ;
-        float factor = 1.f;                                  /* of this row's ds */
+        float factor = 1.f, most = 0.f;                      /* of this row's ds; their largest */
         /* no warp leaves out a step's barriers, whatever became of its waits (after one that ran out the next return at once) */
         for (int j = 0; j < n; j++) {
             const uint32_t ph = (uint32_t)j & 1u;
@@ -521,6 +536,7 @@ XattnGradQKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                 if (j > 0)
                     PackDs(dpT + c * 16, x + c * 32);
             }
+            most = fmaxf(most, top * PowerInverse(factor));
             /* the step before's product is done: its sums may be scaled */
             SettleDs<D>(x, top, factor, rowLive, j == 0, hf, &sDelta[r], dpT, dqT);
             TcFenceBefore();
@@ -531,6 +547,9 @@ XattnGradQKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         TcFenceAfter();
         const bool sums = n > 0 && ok;
         const float power = PowerInverse(factor), out = SumsFactor(power, p.scale);
+        most = __uint_as_float(__reduce_max_sync(0xffffffffu, rowLive ? __float_as_uint(most) : 0u));
+        if (lane == 0)
+            sMost[warp] = most;
 #pragma unroll 1
         for (int c = hf * (D / 64); c < (hf + 1) * (D / 64); c++) {       /* 32 columns a step; this half's D / 2 */
             uint32_t o[32];
@@ -546,6 +565,8 @@ XattnGradQKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         if (p.splits == 1) {
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             GradBarrier();                       /* all eight warps come here, whatever became of their waits */
+            if (warp == 0)
+                leaveMost();
             if (ok && hf == 0 && lane == 0 && q0 + sub * 32 < p.sh.lenQ) {
 #pragma unroll
                 for (int dc = 0; dc < DC; dc++)
@@ -564,6 +585,8 @@ XattnGradQKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
     }
     if (p.splits > 1) {
         ClusterSync();
+        if (warp == 0 && rank == 0)
+            leaveMost();
         if (warp < 8) {
             const int rowsEach = XT / p.splits, chunks = D / 8;
             for (int i = threadIdx.x; i < rowsEach * chunks; i += 256) {
@@ -603,10 +626,10 @@ XattnGradKVKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         uint64_t k, v, s, p, dp, ds, done;
         uint32_t tmem;
         int abort;
+        int most[8];                                         /* the warps' largest exponents of ds */
     };
     static_assert(sizeof(Bars) <= 256, "place of the barriers");
     Bars & bars = *(Bars *)(kvSmem + SM::KV_BARS);
-    float * sWord = (float *)(kvSmem + SM::KV_WORDS);        /* what the two threads of a row tell each other */
 
     const int warp = threadIdx.x >> 5;
     const int lane = threadIdx.x & 31;
@@ -841,16 +864,33 @@ XattnGradKVKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         const uint32_t laneBase = (uint32_t)(sub * 32) << 16;
         const int r = sub * 32 + lane;
         const uint32_t sT = tmemBase + laneBase + TMEM_S + hf * 64, dpT = tmemBase + laneBase + TMEM_DP + hf * 64;
-        const bool rowLive = k0 + r < nk;
-        float factor = 1.f;                                  /* of this key's ds */
+        /* the factor of this head's ds, by the largest that the first kernel met in its query tiles. An infinity there comes
+           of a delta or dp that makes every dk of the head infinite or NaN: here NaN. */
+        int e = 0;
+        for (int t = threadIdx.x; t < steps; t += 256) {
+            const int g = t / qTiles, qt = t - g * qTiles;
+            const uint4 * w = (const uint4 *)(p.work + (((long long)b * p.sh.headsQ + kvHead * p.sh.group + g) * p.tilesPerHead + qt) * (2 * XT) + XT);
+            const uint4 lo = __ldcg(w), hi = __ldcg(w + 1);
+            e = max(e, (int)((lo.x & 1u) | (lo.y & 1u) << 1 | (lo.z & 1u) << 2 | (lo.w & 1u) << 3 |
+                             (hi.x & 1u) << 4 | (hi.y & 1u) << 5 | (hi.z & 1u) << 6 | (hi.w & 1u) << 7));
+        }
+        e = __reduce_max_sync(0xffffffffu, e);
+        if (lane == 0)
+            bars.most[warp] = e;
+        GradBarrier();
+        for (int w = 0; w < 8; w++)
+            e = max(e, bars.most[w]);
+        const float factor = e < 255 ? PowerFor(__uint_as_float((uint32_t)e << 23), 14) : NAN;
+        const uint64_t factor2 = Pair(factor, factor), unscale2 = Pair(factor * P_SCALE_INV, factor * P_SCALE_INV);
         bool ok = true;
-        /* as in the first kernel, no warp leaves out a step's barriers */
         for (int i = 0; i < n; i++) {
             const uint32_t ph = (uint32_t)i & 1u;
             const float4 * lse4 = (const float4 *)(kvSmem + SM::KV_STATS + (i % STATSLOTS) * SM::STAT) + hf * 16, * delta4 = lse4 + XT / 4;
             /* every lane observes the copy's completion itself before it reads what was copied */
             ok = WaitNowWarp(SmemAddr(&bars.statFull[i % STATSLOTS]), (uint32_t)(i / STATSLOTS) & 1u, abortPtr, p.status) &&
-                 WaitNowWarp(SmemAddr(&bars.s), ph, abortPtr, p.status) && ok;
+                 WaitNowWarp(SmemAddr(&bars.s), ph, abortPtr, p.status);
+            if (!ok)
+                break;
             /* these scores were issued behind the last product that reads the step before's do */
             if (threadIdx.x == 0 && i >= 1)
                 MbarArrive(SmemAddr(&bars.doEmpty[(i - 1) % DOSLOTS]));
@@ -876,47 +916,42 @@ XattnGradKVKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
             TmemWaitStore();
             TcFenceBefore();
             ArriveWarp(SmemAddr(&bars.p), lane);
-            ok = WaitNowWarp(SmemAddr(&bars.dp), ph, abortPtr, p.status) && ok;
+            ok = WaitNowWarp(SmemAddr(&bars.dp), ph, abortPtr, p.status);
+            if (!ok)
+                break;
             /* and this product behind the one that reads its q, which all softmax threads let go ahead */
             if (threadIdx.x == 0 && i >= 1) {
                 MbarArrive(SmemAddr(&bars.qEmpty[(i - 1) % QSLOTS]));
                 MbarArrive(SmemAddr(&bars.statEmpty[(i - 1) % STATSLOTS]));
             }
             TcFenceAfter();
-            const uint64_t inv2 = Pair(P_SCALE_INV, P_SCALE_INV), factor2 = Pair(factor, factor);
-            float top = 0.f;
 #pragma unroll
             for (int c = 0; c < 2; c++) {
-                uint32_t y[32];
+                uint32_t y[32], w[16];
                 TmemLoad32Async(dpT + c * 32, y);
                 TmemWaitLoad();
 #pragma unroll
                 for (int e4 = 0; e4 < 8; e4++) {
                     const float4 de = delta4[c * 8 + e4];        /* -2^-12 delta */
                     const int e = e4 * 4, xe = c * 32 + e;
-                    const uint64_t d0 = Fma2(Pair(__uint_as_float(y[e]), __uint_as_float(y[e + 1])), inv2, Pair(de.x, de.y));
-                    const uint64_t d1 = Fma2(Pair(__uint_as_float(y[e + 2]), __uint_as_float(y[e + 3])), inv2, Pair(de.z, de.w));
-                    float a, b;
-                    Unpair(Mul2(Mul2(Pair(__uint_as_float(x[xe]), __uint_as_float(x[xe + 1])), factor2), d0), a, b);
-                    x[xe] = __float_as_uint(a);
-                    x[xe + 1] = __float_as_uint(b);
-                    Unpair(Mul2(Mul2(Pair(__uint_as_float(x[xe + 2]), __uint_as_float(x[xe + 3])), factor2), d1), a, b);
-                    x[xe + 2] = __float_as_uint(a);
-                    x[xe + 3] = __float_as_uint(b);
+                    const uint64_t d0 = Fma2(Pair(__uint_as_float(y[e]), __uint_as_float(y[e + 1])), unscale2, Mul2(Pair(de.x, de.y), factor2));
+                    const uint64_t d1 = Fma2(Pair(__uint_as_float(y[e + 2]), __uint_as_float(y[e + 3])), unscale2, Mul2(Pair(de.z, de.w), factor2));
+                    float f0, f1, f2, f3;
+                    Unpair(Mul2(Pair(__uint_as_float(x[xe]), __uint_as_float(x[xe + 1])), d0), f0, f1);
+                    Unpair(Mul2(Pair(__uint_as_float(x[xe + 2]), __uint_as_float(x[xe + 3])), d1), f2, f3);
+                    w[e4 * 2] = PackHalf2Finite(f0, f1);
+                    w[e4 * 2 + 1] = PackHalf2Finite(f2, f3);
                 }
-                top = fmaxf(top, LargestDs(x + c * 32));
-                if (i > 0)
-                    PackDs(dpT + c * 16, x + c * 32);
+                TmemStore16Async(dpT + c * 16, w);
             }
-            /* the step before's product for dk is done: its sums may be scaled */
-            SettleDs<D>(x, top, factor, rowLive, i == 0, hf, &sWord[r], dpT, tmemBase + laneBase + TMEM_DK);
+            TmemWaitStore();
             TcFenceBefore();
             ArriveWarp(SmemAddr(&bars.ds), lane);
         }
         if (n > 0 && ok)
             ok = WaitNowWarp(SmemAddr(&bars.done), 0, abortPtr, p.status);
         TcFenceAfter();
-        const bool sums = n > 0 && ok;
+        const bool sums = n > 0 && ok, rowLive = k0 + r < nk;
         /* warps 0-3: dv, in the place of v; warps 4-7: dk, in the place of k */
         const uint32_t accT = tmemBase + laneBase + (hf == 0 ? TMEM_DV : TMEM_DK);
         const uint32_t box = (hf == 0 ? vS : kS) + sub * 32 * ROW_BYTES;

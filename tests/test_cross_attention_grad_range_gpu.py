@@ -100,3 +100,42 @@ def test_rows_of_very_unequal_gradients(shape):
     out, lse = ops.CrossAttention(q, k, v, with_lse=True)
     for g in ops.GradCrossAttention(q, k, v, out, lse, x):
         assert (g == 0).all()
+
+
+@pytest.mark.parametrize("n,m,d", [(200, 300, 64), (700, 500, 128), (300, 5000, 64)])
+def test_ds_that_cancel(n, m, d):
+    """ds that are 0 but for roundings: sentences of one key, values that are all alike, incoming gradients across them. What
+    little is computed stays as small as the roundings are"""
+    from tests.test_cross_attention_gpu import lens
+    from tests.test_cross_attention_grad_gpu import check as check_lengths
+    q, k, v = make(3, 4, 2, n, m, d)
+    check_lengths(q, k, v, None, lens([1, m, 1]))
+    check_lengths(q, k, v, lens([n, 130, 5]), lens([1, 2, 129]))
+    for size in (1.0, 1000.0):
+        same = (v[:, :, :1] * size).expand_as(v).contiguous()
+        check_lengths(q, k, same)
+        flat = torch.full_like(v, 3.0 * size)                         # do across it: every dp cancels
+        do = torch.randn(q.shape, device=DEV, generator=torch.Generator(device=DEV).manual_seed(6))
+        do[..., 1::2] = -do[..., ::2]
+        do = do.half()
+        out, lse = ops.CrossAttention(q, k, flat, with_lse=True)
+        for x in ops.GradCrossAttention(q, k, flat, out, lse, do)[:2]:
+            # p times what dp and delta are off by, 2^-20 of sum |do v| each and delta 2^-11 of it for the rounding of out
+            limit = (do.double().abs().sum(-1).amax() * 3.0 * size * (2.0 ** -11 + 2.0 ** -19)).item()
+            total = n * q.abs().max().item() * 4 if x.shape == k.shape else k.abs().max().item()
+            assert torch.isfinite(x).all() and x.abs().max().item() <= limit * total / d ** 0.5 + 2.0 ** -25
+
+
+@pytest.mark.parametrize("n,m,d", [(4, 300, 64), (40, 60, 64), (200, 300, 64), (300, 5000, 128)])
+def test_infinite_ds_reach_the_gradients(n, m, d):
+    q, k, v = make(2, 2, 2, n, m, d)
+    do = torch.randn_like(q)
+    out, lse = ops.CrossAttention(q, k, v, with_lse=True)
+    clean = ops.GradCrossAttention(q, k, v, out, lse, do)
+    x = do.clone()
+    x[1, 1, n - 1, 3] = INF
+    got = ops.GradCrossAttention(q, k, v, out, lse, x)
+    assert not torch.isfinite(got[1][1, 1]).any() and not torch.isfinite(got[0][1, 1, n - 1]).any()
+    for a, c in zip(got, clean):
+        assert torch.equal(a[0], c[0]) and torch.equal(a[1, 0], c[1, 0])
+    assert torch.equal(got[0][1, 1, :n - 1], clean[0][1, 1, :n - 1])
