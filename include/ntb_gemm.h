@@ -166,7 +166,9 @@ int ntb_attention_dropout(int devID, void * stream,
  * than fill the GPU split the keys over a cluster. Sums and statistics are fp32; weights are
  * rounded to half for the second product. The tensor core's fp32 sums round toward zero: up to 2^18 keys (2^20 with at
  * most 32 rows) a result falls short by less than 2^-12 of itself, beyond that by that much again for as many
- * keys more. Results do not depend on timing. No workspace.
+ * keys more. Results do not depend on timing, nor a row's on other rows. No workspace.
+ * Of the library's two fused attentions this is the faster one, by 1.5 to 6 times where both apply; ntb_attention is the one
+ * with an additive mask and with dropout.
  */
 typedef struct ntb_heads_layout {
     long long batch, head, row;      /* strides in elements */
@@ -185,6 +187,9 @@ int ntb_cross_attention(int devID, void * stream,
  * dq, dk, dv. work: device scratch of ntb_cross_attention_grad_work() bytes on a 16-byte boundary, the
  * caller's, so that calls on several streams or in several captured graphs do not share it; its content
  * need not survive the call (calls with few query rows for a key head or few keys do without, and read all once).
+ * Products take p and ds as halves times powers of two that keep them away from a half's ends; sums are fp32. Where a
+ * sentence has more than 128 keys, delta_i = sum dout_i out_i is formed from `out` as given: its rounding to half, up to
+ * 2^-11 of sum |dout_i out_i|, reaches dq_i by way of the mean of the keys under the weights.
  * No atomics: results do not depend on timing. The reference has no such
  * node; its backward pass runs the chain's own (source/network/XBackwardMath.cpp:714-786 for the products).
  */
@@ -252,7 +257,7 @@ int ntb_embedding_grad(int devID, void * stream, const int * ids, const void * d
  * another that is written: NTB_ERR_ARG. norm: one float on the
  * device. A norm that is not finite (as a float) leaves the gradients' values as they are (the caller reads *norm and skips
  * the step); maxNorm infinite only takes the norm. maxNorm must not be negative or NaN. The sum is
- * fp64 (fp32 within eight exact products of halves); its order is fixed by the sizes. work: device scratch
+ * fp64 (fp32 within eight exact products of halves); its order is fixed by the sizes and the addresses' alignment. work: device scratch
  * of ntb_clip_grad_norm_work(count) bytes on an 8-byte boundary, the caller's. The arrays are read before
  * the call returns; the addresses are part of the launch, so a captured call replays on the same tensors.
  */

@@ -25,7 +25,7 @@
  * of dw whose words do not occur (beta = 0), known from a bit map of the list.
  *
  * Bound by the reads of dout and the writes of dw at large sizes (100000 tokens of 1024 floats, 32000 words: 133 us,
- * 541 MB at 4.1 TB/s, of which the sort is 45), by the launches' latency at small ones (4096 tokens of 512 halves: 25).
+ * 541 MB at 4.1 TB/s, of which the sort is 41), by the launches' latency at small ones (4096 tokens of 512 halves: 25).
  *
  * Sums are fp32 in a fixed order. Ids outside [0, vocab) stand for no word.
  */

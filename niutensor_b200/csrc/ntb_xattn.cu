@@ -593,8 +593,10 @@ int DispatchXattn(const DeviceCtx & ctx, const XattnCall & call, cudaStream_t st
     p.scaleLog2 = call.scale * LOG2E;
     p.status = ctx.status;
     const long long heads = (long long)s.batch * s.headsKV;
-    /* two query tiles to a CTA halve the reads of k and v from L2; below one such CTA per SM, single tiles
-       (two CTAs per SM) spread wider */
+    /* Two query tiles to a CTA halve the reads of k and v from L2; below one such CTA per SM, single tiles (two CTAs per
+       SM) spread wider. Two / one, us: 4 x 16 heads, 2000 rows, 8192 keys of 128 458 / 490; 1 x 16 heads, 2048 rows and keys
+       of 128 54 / 37; 8 x 8 heads, 256 rows, 2048 keys of 64 36 / 22. Over one or two key tiles the rule still takes two where
+       it could take one: 64 x 8 heads, 256 rows, 73 and 256 keys of 64 29 / 22 and 34 / 28. */
     const bool two = units >= 2 && heads * ((units + 1) / 2) >= ctx.smCount;
     const long long items = two ? heads * ((units + 1) / 2) : heads * units;
     /* split the keys until the GPU is full, while a part keeps two tiles; and into parts of few enough instructions */

@@ -51,7 +51,7 @@ struct XattnGradCall {
 
 /* Query rows a key head up to which the kernels of 16-row tiles are used: two tiles are what a warp's registers hold.
    The others pad to 128 rows. Gradients of 32 rows, us, here / there: 64 x 8 heads, 200 keys of 128
-   48 / 88; 1000 of 128 120 / 283; one head, 8192 keys of 64 28 / 22 (here at most eight CTAs share a head). */
+   48 / 86; 1000 of 128 122 / 282; one head, 8192 keys of 64 31 / 24 (here at most eight CTAs share a head). */
 constexpr int XATTN_STEP_ROWS = 32;
 
 namespace {

@@ -23,8 +23,8 @@
  * distributed shared memory.
  *
  * Bound by the steps' products and the shared memory that feeds them, on long walks (2 x 16 query and 4 key heads,
- * 1777 rows, 4100 keys of 128: 405 us, 298 GFLOP of the formulas' five products, 418 of the seven done, 1.03 PFLOP/s;
- * a step takes some 2570 clocks in the first kernel and 3275 in the second), by the loads before an item's first
+ * 1777 rows, 4100 keys of 128: 432 us, 298 GFLOP of the formulas' five products, 418 of the seven done, 0.97 PFLOP/s;
+ * a step takes some 2700 clocks in the first kernel and 3300 in the second), by the loads before an item's first
  * product and the stores behind its last on short ones (64 x 4 heads, 100 to 200 rows and keys of 128: 65 us).
  *
  * What a CTA runs once (the rows' way to tensor memory, the results' out of it) is kept in loops: unrolled, its

@@ -9,7 +9,7 @@
  * The next chunk's rows of q and do travel to registers under the products of this one. delta comes from the weights,
  * as all keys are here (ntb_xattn_grad.cu says what that is good for). Rounding as there: ds, times powers of two (of the
  * query's row for dq, of the warp for dk), and 2^12 p to half, sums in fp32. Bound by the latency of a chunk's four steps, which other CTAs of the SM fill: hence few keys and registers
- * a CTA. 64 x 8 heads, 48 rows, 48 keys of 64: 16.7 us, 22 MB at 1.3 TB/s.
+ * a CTA. 64 x 8 heads, 48 rows, 48 keys of 64: 16.5 us, 22 MB at 1.3 TB/s.
  */
 #include "ntb_xattn.cuh"
 
@@ -421,14 +421,14 @@ int LaunchShort(const XattnGradCall & call, const ShortParams & base, cudaStream
 
 /*
  * Which calls come here, us here / in the kernels they would otherwise go to, head size 64 and 128:
- *   up to 32 rows (otherwise ntb_xattn_step.cu): 64 x 8 heads, 16 rows, 40 keys 10.1 / 12.1 and 15.5 / 18.2; 32 rows,
- *     64 keys 10.6 / 15.5 and 16.2 / 24.7; 8 rows, 128 keys 14.0 / 16.0 and 31 / 24 (that one not). Shared key heads not:
+ *   up to 32 rows (otherwise ntb_xattn_step.cu): 64 x 8 heads, 16 rows, 40 keys 10.1 / 11.8 and 15.7 / 18.2; 32 rows,
+ *     64 keys 10.6 / 15.9 and 16.5 / 24.5; 8 rows, 128 keys 15.1 / 16.2 and 32 / 24 (that one not). Shared key heads not:
  *     their few rows would be a chunk for every query head;
- *   two chunks (otherwise ntb_xattn_grad.cu): 8 heads, 64 rows, 64 keys 7.6 / 11.3 and 10.5 / 14.2; 64 x 8 heads 17 / 45 and
- *     26 / 54; 100 keys 21 / 46 and 49 / 58;
- *   more, as a CTA takes them one after the other, where the heads fill the GPU: 64 x 4 heads, 200 rows, 64 keys 28 / 39 and
- *     37 / 48, 128 keys 33 / 40 and 71 / 50 (not); 64 heads, 200 rows, 64 keys 21 / 15 (not); 64 x 8 heads, 1000 rows, 128 keys
- *     276 / 259 (not).
+ *   two chunks (otherwise ntb_xattn_grad.cu): 8 heads, 64 rows, 64 keys 7.4 / 11.4 and 10.6 / 13.1; 64 x 8 heads 18 / 46 and
+ *     26 / 53; 100 keys 24 / 47 and 50 / 56;
+ *   more, as a CTA takes them one after the other, where the heads fill the GPU: 64 x 4 heads, 200 rows, 64 keys 29 / 40 and
+ *     37 / 46, 128 keys 37 / 41 and 72 / 49 (not); 64 heads, 200 rows, 64 keys 21 / 15 (not); 64 x 8 heads, 1000 rows, 128 keys
+ *     322 / 267 (not).
  */
 bool XattnGradIsShort(const DeviceCtx & ctx, const XattnShape & s)
 {

@@ -10,14 +10,14 @@
  * way). The weights go from the first product's accumulators straight into the second's A operand.
  * Warps join their sums through shared memory, the CTAs of a cluster (1 to 8) through
  * distributed shared memory, in a fixed order: one launch, no workspace, no atomics. 8 x 8 key heads, four query
- * heads each, 16384 keys of 128: 67 us, 403 MB at 6.0 TB/s (93 % of a copy's rate). One sentence's step (32 heads,
- * 41 keys) is 3.2 us on the device, launch and latency.
+ * heads each, 16384 keys of 128: 67 us, 403 MB at 6.0 TB/s (93 % of a copy's rate). One sentence's step (8 heads,
+ * 23 keys of 64) is 3.2 us on the device, launch and latency.
  *
  * XattnGradStepKernel is the backward pass of such calls (training on short targets): every warp makes dk and dv of
  * its 16 keys whole, from the same registers that give its share of dq, so k and v are read once and their
  * gradients written once, by TMA from the place of the tiles they came in. The weights' transposes are taken in
  * registers (movmatrix). The kernels of ntb_xattn_grad.cu would pad the rows to 128 and read everything twice. Bound
- * by k, v and their gradients where keys are many (20 x 16 heads, 16 rows, 2000 keys of 128: 122 us, 5.4 TB/s), by a
+ * by k, v and their gradients where keys are many (20 x 16 heads, 16 rows, 2000 keys of 128: 124 us, 5.3 TB/s), by a
  * CTA's first loads and last sums where they are few (44 x 16 heads, 15 rows, 243 keys of 104: 47 us, 3.2 TB/s).
  */
 #include "ntb_xattn.cuh"
@@ -865,8 +865,8 @@ int StepSplits(const DeviceCtx & ctx, const XattnShape & s)
 }
 
 /* Gradients: the parts with the shortest walk in tiles, over the waves that the GPU's places make of them. A CTA's
-   rows, first loads and sums cost it about four tiles. (64 x 8 heads) x 16 x 1000 x 128 in two parts takes 110 us, in
-   one 119; (20 x 16) x 16 x 2000 x 128 in one 123, in four 137. */
+   rows, first loads and sums cost it about four tiles. (64 x 8 heads) x 16 x 1000 x 128 in two parts takes 111 us, in
+   one 121; (20 x 16) x 16 x 2000 x 128 in one 123, in four 137. */
 int GradStepSplits(const DeviceCtx & ctx, const XattnShape & s, int places)
 {
     const long long heads = (long long)s.batch * s.headsKV;
